@@ -24,6 +24,11 @@ class ConvShape(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("N", "C", "H", "W", "F", "KH", "KW", "SY", "SX", "PY", "PX")]
 
 
+class AdamwHyper(C.Structure):
+    _fields_ = [(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")] + [
+        ("step", C.c_longlong), ("device_step", C.c_void_p), ("state_bits", C.c_int)]
+
+
 _lib = None
 
 
@@ -78,5 +83,8 @@ def lib():
     for name in ("rgb200_conv2d", "rgb200_conv2d_grad_weight", "rgb200_conv2d_grad_input"):
         getattr(L, name + "_workspace").argtypes = [shp, i, C.POINTER(C.c_size_t)]
         getattr(L, name + "_ws").argtypes = [fp, fp, fp, shp, i, vp, C.c_size_t, vp]
+    L.rgb200_adamw_step.argtypes = [vp, i, C.POINTER(AdamwHyper), vp]
+    L.rgb200_adamw_states_read.argtypes = [vp, i, vp]
+    L.rgb200_adamw_states_write.argtypes = [vp, i, vp]
     _lib = L
     return L

@@ -7,20 +7,19 @@ defined by IEEE single operations (the reference states the same discipline at
 repro_gemm_cuda/repro_gemm.cuh:23 and repro_torch/setup.py:24).
 """
 import os
+import re
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "librgb200.so")
-SOURCES = ["rgb200_api.cu", "rgb200_cxx.cu"]
-HEADERS = ["rgb200_math.cuh", "rgb200_mma.cuh", "rgb200_smallk.cuh", "rgb200_rowfused.cuh", "rgb200_prepass.cuh",
-           "rgb200_prepass_cluster.cuh", "rgb200_conv.cuh", "rgb200_conv_direct.cuh",
-           os.path.join("..", "..", "include", "rgb200.h"), os.path.join("..", "..", "include", "repro_gemm.cuh"),
-           os.path.join("..", "..", "include", "repro_conv.cuh")]
+OBJ = os.path.join(CSRC, "obj")
+SOURCES = ["rgb200_api.cu", "rgb200_cxx.cu", "rgb200_optim.cu"]
 
 NVCC_FLAGS = ["-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "--fmad=false",
-              "-Xcompiler", "-fPIC", "-shared", "-cudart", "static"]
+              "-Xcompiler", "-fPIC", "-cudart", "static"]
 
 
 def _nvcc():
@@ -30,22 +29,50 @@ def _nvcc():
     raise RuntimeError("nvcc not found; librgb200.so cannot be built")
 
 
+def _inputs(path, seen=None):
+    """The source and every header it includes by a relative path, directly or through another one."""
+    seen = set() if seen is None else seen
+    path = os.path.normpath(path)
+    if path not in seen and os.path.exists(path):
+        seen.add(path)
+        with open(path) as f:
+            for name in re.findall(r'^\s*#include "([^"]+)"', f.read(), re.M):
+                _inputs(os.path.join(os.path.dirname(path), name), seen)
+    return seen
+
+
+def _newer(target, inputs):
+    return not os.path.exists(target) or any(os.path.getmtime(f) > os.path.getmtime(target) for f in inputs)
+
+
 def stale():
-    if not os.path.exists(LIB):
-        return True
-    t = os.path.getmtime(LIB)
-    return any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in SOURCES + HEADERS)
+    return any(_newer(LIB, _inputs(os.path.join(CSRC, src))) for src in SOURCES)
 
 
 def build(force=False, verbose=False):
-    """Compile the library if it is missing or older than its sources; returns its path."""
-    if force or stale():
-        cmd = [_nvcc()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-o", LIB] + SOURCES
+    """Compile the library if it is missing or older than its sources; returns its path.  Each source becomes an object
+    of its own (compiled side by side, reused while its inputs are unchanged), and the objects are linked."""
+    if not (force or stale()):
+        return LIB
+    os.makedirs(OBJ, exist_ok=True)
+    nvcc = _nvcc()
+
+    def run(cmd):
         res = subprocess.run(cmd, cwd=CSRC, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
         if verbose:
             print(res.stderr)
+
+    def compile_one(src):
+        obj = os.path.join(OBJ, src[:-3] + ".o")
+        if force or _newer(obj, _inputs(os.path.join(CSRC, src))):
+            run([nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-c", "-o", obj, src])
+        return obj
+
+    with ThreadPoolExecutor(len(SOURCES)) as pool:
+        objs = list(pool.map(compile_one, SOURCES))
+    run([nvcc] + NVCC_FLAGS + ["-shared", "-o", LIB] + objs)
     return LIB
 
 

@@ -588,7 +588,7 @@ gemm_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
 // short limit.  Lane 0 must give up after `limit` clocks, store `code` in *status and raise the abort
 // flag; lane 1, waiting with the full limit, must leave early because it sees that flag.
 // out[0] = lane 0 returned false, out[1] = lane 1 returned false, out[2] = clocks lane 0 waited.
-__global__ void bounded_wait_probe_kernel(int* status, long long limit, long long* out) {
+static __global__ void bounded_wait_probe_kernel(int* status, long long limit, long long* out) {
     __shared__ __align__(8) unsigned long long bar;
     __shared__ int abort_flag;
     const uint32_t b = smem_u32(&bar);

@@ -1,0 +1,116 @@
+// Host side of the AdamW entry points declared in include/rgb200.h.  Tensors travel to the kernels by value in the launch
+// parameters, so a call copies nothing to the device, keeps nothing, and can be captured into a CUDA graph.
+#include <new>
+
+#include "../../include/rgb200.h"
+#include "rgb200_optim.cuh"
+
+namespace rgb200 {
+namespace {
+
+cudaError_t check_b200() {
+    int dev, major = 0, minor = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
+    if (e != cudaSuccess) return e;
+    return major == 10 && minor == 0 ? cudaSuccess : cudaErrorNotSupported;
+}
+
+bool good_tensors(const rgb200_adamw_tensor* t, int count, int bits) {
+    if (count < 0 || (count > 0 && !t) || (bits != 8 && bits != 32)) return false;
+    for (int i = 0; i < count; ++i) {
+        if (t[i].count < 0) return false;
+        if (t[i].count == 0) continue;
+        if (!t[i].param || !t[i].grad || !t[i].exp_avg || !t[i].exp_avg_sq) return false;
+        if (bits == 8 && (!t[i].exp_avg_scale || !t[i].exp_avg_sq_scale)) return false;
+    }
+    return true;
+}
+
+// Values per CTA: small sets are spread over the SMs (at least four CTAs each), large ones get up to 4096 values a CTA
+// so that finding its tensor costs a CTA little.
+int pick_chunk(long long total) {
+    int chunk = OPT_MIN_CHUNK;
+    while (chunk < 4 * OPT_MIN_CHUNK && total / (2 * chunk) >= 148 * 4) chunk *= 2;
+    return chunk;
+}
+
+template <int CAP, class Launch>
+cudaError_t for_tables(const rgb200_adamw_tensor* t, int count, int chunk, Launch launch) {
+    OptTable<CAP>* T = new (std::nothrow) OptTable<CAP>;
+    if (!T) return cudaErrorMemoryAllocation;
+    cudaError_t e = cudaSuccess;
+    int i = 0;
+    while (i < count && e == cudaSuccess) {
+        T->count = 0;
+        T->chunk = chunk;
+        long long chunks = 0;
+        for (; i < count && T->count < CAP; ++i) {
+            if (t[i].count == 0) continue;
+            const long long c = (t[i].count + chunk - 1) / chunk;
+            if (c > 0x7FFFFFFFll) { delete T; return cudaErrorInvalidValue; }
+            if (chunks + c > 0x7FFFFFFFll) break;                     // the grid's limit: the rest goes to the next launch
+            T->e[T->count] = OptEntry{t[i].param, t[i].grad, t[i].exp_avg, t[i].exp_avg_sq, t[i].exp_avg_scale, t[i].exp_avg_sq_scale, t[i].count};
+            T->first[T->count++] = (int)chunks;
+            chunks += c;
+        }
+        if (T->count == 0) break;
+        T->first[T->count] = (int)chunks;
+        launch(*T, (unsigned)chunks);
+        e = cudaGetLastError();
+    }
+    delete T;
+    return e;
+}
+
+template <int CAP>
+cudaError_t run_adamw(const rgb200_adamw_tensor* t, int count, int chunk, int bits, OptMode mode, const AdamwHyper& H, cudaStream_t st) {
+    return for_tables<CAP>(t, count, chunk, [&](const OptTable<CAP>& T, unsigned grid) {
+        if (mode == OPT_READ) adamw8_kernel<CAP, OPT_READ><<<grid, OPT_THREADS, 0, st>>>(T, H);
+        else if (mode == OPT_WRITE) adamw8_kernel<CAP, OPT_WRITE><<<grid, OPT_THREADS, 0, st>>>(T, H);
+        else if (bits == 8) adamw8_kernel<CAP, OPT_STEP><<<grid, OPT_THREADS, 0, st>>>(T, H);
+        else adamw32_kernel<CAP><<<grid, OPT_THREADS, 0, st>>>(T, H);
+    });
+}
+
+cudaError_t adamw_call(const rgb200_adamw_tensor* t, int count, int bits, OptMode mode, const AdamwHyper& H, void* stream) {
+    if (!good_tensors(t, count, bits)) return cudaErrorInvalidValue;
+    long long total = 0;
+    for (int i = 0; i < count; ++i) total += t[i].count;
+    cudaError_t e = check_b200();
+    if (e != cudaSuccess || total == 0) return e;
+    const int chunk = pick_chunk(total);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return count <= OPT_SMALL_TABLE ? run_adamw<OPT_SMALL_TABLE>(t, count, chunk, bits, mode, H, st)
+                                    : run_adamw<OPT_LARGE_TABLE>(t, count, chunk, bits, mode, H, st);
+}
+
+}  // namespace
+}  // namespace rgb200
+
+using namespace rgb200;
+
+extern "C" int rgb200_adamw_step(const rgb200_adamw_tensor* tensors, int count, const rgb200_adamw_hyper* h, void* stream) {
+    if (!h || !(h->beta1 >= 0.0 && h->beta1 < 1.0) || !(h->beta2 >= 0.0 && h->beta2 < 1.0) || !(h->eps >= 0.0) || !(h->lr >= 0.0) ||
+        !(h->weight_decay >= 0.0) || (!h->device_step && h->step < 1))
+        return cudaErrorInvalidValue;
+    AdamwHyper H = {};
+    H.lr = h->lr; H.b1 = h->beta1; H.b2 = h->beta2; H.eps = h->eps; H.wd = h->weight_decay;
+    H.step_word = h->device_step;
+    if (!h->device_step) H.s = adamw_scalars(h->lr, h->beta1, h->beta2, h->eps, h->weight_decay, h->step);
+    cudaError_t e = adamw_call(tensors, count, h->state_bits, OPT_STEP, H, stream);
+    if (e == cudaSuccess && h->device_step) {
+        advance_step_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(h->device_step);
+        e = cudaGetLastError();
+    }
+    return e;
+}
+
+extern "C" int rgb200_adamw_states_read(const rgb200_adamw_tensor* tensors, int count, void* stream) {
+    return adamw_call(tensors, count, 8, OPT_READ, AdamwHyper{}, stream);
+}
+
+extern "C" int rgb200_adamw_states_write(const rgb200_adamw_tensor* tensors, int count, void* stream) {
+    return adamw_call(tensors, count, 8, OPT_WRITE, AdamwHyper{}, stream);
+}

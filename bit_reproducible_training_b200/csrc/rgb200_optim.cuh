@@ -1,0 +1,287 @@
+// One AdamW step over many tensors in one launch, with first and second moments in FP32 or as 8-bit codes.
+//
+// The step is a fixed sequence of IEEE single operations per value (the library is built without FMA contraction), so its
+// bits do not depend on how the values are spread over CTAs, launches or GPUs:
+//   p1 = p * (1 - lr wd)
+//   m' = m * b1 + g * (1 - b1)          v' = v * b2 + (g * g) * (1 - b2)
+//   d  = sqrt(v') * (1 / sqrt(1 - b2^n)) + eps
+//   p' = p1 - (m' / d) * (lr / (1 - b1^n))
+// with every parenthesised constant formed in double precision and rounded once to FP32 (AdamwScalars).
+//
+// 8-bit states: blocks of 256 consecutive values of a tensor share one FP32 scale, the block's largest magnitude.
+//   first moment   code q in [-127, 127]   value  ((q/127) |q/127|) * scale     q = RNE(127 sqrt(|m| / scale)) with m's sign
+//   second moment  code q in [0, 255]      value  ((q/255)^2)^2 * scale         q = RNE(255 sqrt(sqrt(v / scale)))
+// Companding by a square (a fourth power) spends the codes on small magnitudes: the relative step of m is 2/q, and sqrt(v),
+// which is what the update divides by, has the same law as m.  A second moment that is not zero never gets the code
+// zero, because the next step would divide by eps alone.  The update itself uses the moments before they are coded.
+// A value that is not finite makes its block's scale NaN, so that the block reads as NaN (FP32 states keep a NaN too).
+//
+// Bound: HBM.  28 bytes a value in FP32 (p, m, v read and written, g read), 16 + 16/256 with 8-bit states.
+#pragma once
+#include <cuda_runtime.h>
+#include <cstdint>
+#include "rgb200_math.cuh"
+
+namespace rgb200 {
+
+constexpr int OPT_THREADS = 256;
+constexpr int OPT_BLOCK = 256;          // values that share a scale
+constexpr int OPT_MIN_CHUNK = 1024;     // values per CTA: a multiple of this
+constexpr int OPT_SMALL_TABLE = 48, OPT_LARGE_TABLE = 448;   // tensors a launch takes by value (448 x 60 bytes < 32 KB)
+
+struct OptEntry {
+    float* p;
+    const float* g;
+    void* m;               // float or int8 codes
+    void* v;               // float or uint8 codes
+    float* sm;             // scales (8-bit states)
+    float* sv;
+    long long n;
+};
+
+template <int CAP>
+struct OptTable {
+    OptEntry e[CAP];
+    int first[CAP + 1];    // first chunk of each tensor; first[count] = number of chunks
+    int count;
+    int chunk;             // values per CTA
+};
+
+struct AdamwScalars { float decay, b1, c1, b2, c2, inv_sqrt_bc2, eps, step_size; };
+
+// b^n by squaring, in double without contraction: the same bits on host and device.
+RGB_HD double pow_int(double b, long long n) {
+    double r = 1.0;
+    for (; n > 0; n >>= 1) {
+        if (n & 1) r = r * b;
+        b = b * b;
+    }
+    return r;
+}
+RGB_HD AdamwScalars adamw_scalars(double lr, double b1, double b2, double eps, double wd, long long step) {
+    AdamwScalars s;
+    s.decay = (float)(1.0 - lr * wd);
+    s.b1 = (float)b1; s.c1 = (float)(1.0 - b1);
+    s.b2 = (float)b2; s.c2 = (float)(1.0 - b2);
+    s.inv_sqrt_bc2 = (float)(1.0 / sqrt(1.0 - pow_int(b2, step)));
+    s.eps = (float)eps;
+    s.step_size = (float)(lr / (1.0 - pow_int(b1, step)));
+    return s;
+}
+
+// Hyper-parameters of a launch: the scalars, or (step_word != null: steps counted on the device, for captured graphs)
+// what they are formed from.
+struct AdamwHyper {
+    AdamwScalars s;
+    double lr, b1, b2, eps, wd;
+    const long long* step_word;
+};
+
+__device__ __forceinline__ void adamw_value(float& p, float g, float& m, float& v, const AdamwScalars& s) {
+    const float p1 = __fmul_rn(p, s.decay);
+    m = __fadd_rn(__fmul_rn(m, s.b1), __fmul_rn(g, s.c1));
+    v = __fadd_rn(__fmul_rn(v, s.b2), __fmul_rn(__fmul_rn(g, g), s.c2));
+    const float d = __fadd_rn(__fmul_rn(__fsqrt_rn(v), s.inv_sqrt_bc2), s.eps);
+    p = __fsub_rn(p1, __fmul_rn(__fdiv_rn(m, d), s.step_size));
+}
+
+// Tensor that chunk `c` belongs to (first[] ascends; empty tensors own no chunk).
+template <int CAP>
+__device__ __forceinline__ int opt_find(const OptTable<CAP>& T, int c) {
+    int lo = 0, hi = T.count;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (T.first[mid] <= c) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ AdamwScalars adamw_load_scalars(const AdamwHyper& H, AdamwScalars* shared) {
+    if (!H.step_word) return H.s;
+    if (threadIdx.x == 0) *shared = adamw_scalars(H.lr, H.b1, H.b2, H.eps, H.wd, *H.step_word + 1);
+    __syncthreads();
+    return *shared;
+}
+
+__device__ __forceinline__ bool aligned_to(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+template <int CAP>
+__global__ void __launch_bounds__(OPT_THREADS)
+adamw32_kernel(const __grid_constant__ OptTable<CAP> T, const __grid_constant__ AdamwHyper H) {
+    __shared__ AdamwScalars shared;
+    const AdamwScalars s = adamw_load_scalars(H, &shared);
+    const int t = opt_find(T, blockIdx.x);
+    const OptEntry& e = T.e[t];
+    const long long at = (long long)((int)blockIdx.x - T.first[t]) * T.chunk;
+    const int here = (int)(e.n - at < T.chunk ? e.n - at : T.chunk);
+    float* p = e.p + at;
+    const float* g = e.g + at;
+    float* m = static_cast<float*>(e.m) + at;
+    float* v = static_cast<float*>(e.v) + at;
+    int done = 0;
+    if (aligned_to(p, 16) && aligned_to(g, 16) && aligned_to(m, 16) && aligned_to(v, 16)) {
+        const int quads = here >> 2;
+        for (int i = threadIdx.x; i < quads; i += OPT_THREADS) {
+            float4 pp = reinterpret_cast<const float4*>(p)[i], gg = reinterpret_cast<const float4*>(g)[i];
+            float4 mm = reinterpret_cast<const float4*>(m)[i], vv = reinterpret_cast<const float4*>(v)[i];
+            adamw_value(pp.x, gg.x, mm.x, vv.x, s);
+            adamw_value(pp.y, gg.y, mm.y, vv.y, s);
+            adamw_value(pp.z, gg.z, mm.z, vv.z, s);
+            adamw_value(pp.w, gg.w, mm.w, vv.w, s);
+            reinterpret_cast<float4*>(p)[i] = pp;
+            reinterpret_cast<float4*>(m)[i] = mm;
+            reinterpret_cast<float4*>(v)[i] = vv;
+        }
+        done = quads << 2;
+    }
+    for (int i = done + threadIdx.x; i < here; i += OPT_THREADS) {
+        float pp = p[i], mm = m[i], vv = v[i];
+        adamw_value(pp, g[i], mm, vv, s);
+        p[i] = pp; m[i] = mm; v[i] = vv;
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// 8-bit codes.  A warp owns one block of 256 values, eight consecutive ones per lane.
+// ------------------------------------------------------------------------------------------
+constexpr float INV127 = (float)(1.0 / 127.0), INV255 = (float)(1.0 / 255.0);
+
+__device__ __forceinline__ float decode_m(int q, float scale) {
+    const float t = __fmul_rn((float)q, INV127);
+    return __fmul_rn(__fmul_rn(t, fabsf(t)), scale);
+}
+__device__ __forceinline__ float decode_v(int q, float scale) {
+    float t = __fmul_rn((float)q, INV255);
+    t = __fmul_rn(t, t);
+    return __fmul_rn(__fmul_rn(t, t), scale);
+}
+// `scale`: the block's largest magnitude, or 1 for a block of zeros.
+__device__ __forceinline__ int encode_m(float m, float scale) {
+    const int q = __float2int_rn(__fmul_rn(__fsqrt_rn(__fdiv_rn(fabsf(m), scale)), 127.0f));
+    return m < 0.0f ? -q : q;
+}
+__device__ __forceinline__ int encode_v(float v, float scale) {
+    const int q = __float2int_rn(__fmul_rn(__fsqrt_rn(__fsqrt_rn(__fdiv_rn(v, scale))), 255.0f));
+    return q == 0 && v > 0.0f ? 1 : q;
+}
+
+// Largest magnitude over the warp's block, NaN if any value is not finite (the bits of non-negative floats order as
+// integers, and infinity and NaN lie above every finite value).
+__device__ __forceinline__ float block_scale(const float (&x)[8]) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7FFFFFFFu);
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    return __uint_as_float(top >= 0x7F800000u ? 0x7FC00000u : top);
+}
+
+__device__ __forceinline__ void load8(const float* p, int live, bool wide, float (&x)[8]) {
+    if (wide && live == 8) {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = j < live ? p[j] : 0.0f;
+    }
+}
+__device__ __forceinline__ void store8(float* p, int live, bool wide, const float (&x)[8]) {
+    if (wide && live == 8) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) if (j < live) p[j] = x[j];
+    }
+}
+__device__ __forceinline__ uint2 load_codes(const uint8_t* q, int live, bool wide) {
+    if (wide && live == 8) return *reinterpret_cast<const uint2*>(q);
+    uint2 r = make_uint2(0u, 0u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (j < live) (j < 4 ? r.x : r.y) |= (uint32_t)q[j] << (8 * (j & 3));
+    return r;
+}
+__device__ __forceinline__ void store_codes(uint8_t* q, int live, bool wide, uint2 c) {
+    if (wide && live == 8) { *reinterpret_cast<uint2*>(q) = c; return; }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (j < live) q[j] = (uint8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
+}
+__device__ __forceinline__ int code_byte(uint2 c, int j) { return (int)(((j < 4 ? c.x : c.y) >> (8 * (j & 3))) & 0xFFu); }
+
+__device__ __forceinline__ void decode_block(uint2 cm, uint2 cv, float sm, float sv, float (&m)[8], float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        m[j] = decode_m((int)(int8_t)code_byte(cm, j), sm);
+        v[j] = decode_v(code_byte(cv, j), sv);
+    }
+}
+
+__device__ __forceinline__ void encode_block(const float (&m)[8], const float (&v)[8], uint8_t* qm, uint8_t* qv, float* sm, float* sv,
+                                             int lane, int live, bool wide) {
+    const float tm = block_scale(m), tv = block_scale(v);
+    uint2 cm = make_uint2(0u, 0u), cv = make_uint2(0u, 0u);
+    const float dm = tm > 0.0f ? tm : 1.0f, dv = tv > 0.0f ? tv : 1.0f;
+    if (!isnan(tm)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) (j < 4 ? cm.x : cm.y) |= ((uint32_t)encode_m(m[j], dm) & 0xFFu) << (8 * (j & 3));
+    }
+    if (!isnan(tv)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) (j < 4 ? cv.x : cv.y) |= ((uint32_t)encode_v(v[j], dv) & 0xFFu) << (8 * (j & 3));
+    }
+    store_codes(qm, live, wide, cm);
+    store_codes(qv, live, wide, cv);
+    if (lane == 0) { *sm = tm; *sv = tv; }
+}
+
+enum OptMode : int { OPT_STEP, OPT_READ, OPT_WRITE };   // update; codes -> values; values -> codes
+
+// OPT_STEP: p, g and the codes.  OPT_READ: the moments' values go to p (first) and g (second, written through a cast
+// away of const by the host's table); OPT_WRITE: they come from there.
+template <int CAP, OptMode MODE>
+__global__ void __launch_bounds__(OPT_THREADS)
+adamw8_kernel(const __grid_constant__ OptTable<CAP> T, const __grid_constant__ AdamwHyper H) {
+    __shared__ AdamwScalars shared;
+    AdamwScalars s = {};
+    if (MODE == OPT_STEP) s = adamw_load_scalars(H, &shared);
+    const int t = opt_find(T, blockIdx.x);
+    const OptEntry& e = T.e[t];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long chunk_at = (long long)((int)blockIdx.x - T.first[t]) * T.chunk;
+    const bool wide = aligned_to(e.p, 16) && aligned_to(e.g, 16) && aligned_to(e.m, 8) && aligned_to(e.v, 8);
+    for (int b = warp; b < T.chunk / OPT_BLOCK; b += OPT_THREADS / 32) {
+        const long long block_at = chunk_at + (long long)b * OPT_BLOCK;
+        if (block_at >= e.n) break;                                     // uniform over the warp
+        const long long at = block_at + lane * 8;
+        const int live = at >= e.n ? 0 : (e.n - at < 8 ? (int)(e.n - at) : 8);
+        float* sm = e.sm + block_at / OPT_BLOCK;
+        float* sv = e.sv + block_at / OPT_BLOCK;
+        uint8_t* qm = static_cast<uint8_t*>(e.m) + at;
+        uint8_t* qv = static_cast<uint8_t*>(e.v) + at;
+        float m[8], v[8];
+        if (MODE != OPT_WRITE) decode_block(load_codes(qm, live, wide), load_codes(qv, live, wide), *sm, *sv, m, v);
+        if (MODE == OPT_STEP) {
+            float p[8], g[8];
+            load8(e.p + at, live, wide, p);
+            load8(e.g + at, live, wide, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                adamw_value(p[j], g[j], m[j], v[j], s);
+                if (j >= live) m[j] = v[j] = 0.0f;                      // lanes past the tensor's end do not set its scale
+            }
+            store8(e.p + at, live, wide, p);
+        } else if (MODE == OPT_READ) {
+            store8(e.p + at, live, wide, m);
+            store8(const_cast<float*>(e.g) + at, live, wide, v);
+        } else {
+            load8(e.p + at, live, wide, m);
+            load8(e.g + at, live, wide, v);
+        }
+        if (MODE != OPT_READ) encode_block(m, v, qm, qv, sm, sv, lane, live, wide);
+    }
+}
+
+static __global__ void advance_step_kernel(long long* step_word) { *step_word += 1; }
+
+}  // namespace rgb200

@@ -1,0 +1,280 @@
+"""AdamW whose step is one launch for all tensors of a parameter group, on top of the C ABI.
+
+Counterpart of the optimizer of the reference's repro_torch (Adam / AdamW over repro_nn_cuda/repro_nn.cuh:12-21), with
+the moments held in FP32 or in 8 bits.  Every value goes through the same fixed sequence of IEEE single operations
+(include/rgb200.h, rgb200_adamw_step), so the parameters' bits depend on the gradients and the hyper-parameters alone.
+CUDA float32 parameters only; there is no CPU path.
+"""
+import ctypes as C
+
+import numpy as np
+import torch
+
+from . import _lib
+from .repro_gemm import ReproGemmError, _stream, cudaSuccess
+
+STATE_BLOCK = 256           # values of a tensor that share one scale (8-bit states)
+
+# one row of the C ABI's rgb200_adamw_tensor
+_ROW = np.dtype([(n, np.uint64) for n in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")] +
+                [("count", np.int64)])
+
+
+def _blocks(n):
+    return -(-n // STATE_BLOCK)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW with decoupled weight decay: ``step()`` is one kernel launch per parameter group (per 448 tensors).
+
+    ``state_bits``: 32, or 8 for codes with one scale per 256 values (2.03 instead of 8 bytes of state a parameter).
+    ``capturable``: steps are counted on the device, so that ``step()`` can be captured into a CUDA graph and replayed; all
+    parameters must then have gradients, and the captured learning rate and other hyper-parameters stay as they were.
+    Without it a step under capture is refused.  Parameters must not overlap in memory.
+
+    ``state_dict()`` holds the moments' values in float32 whatever ``state_bits`` is, and ``load_state_dict`` takes such a
+    dict into either width (values pass through the codes again, which returns the same codes)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, capturable=False):
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        self.state_bits, self.capturable = state_bits, capturable
+        self._tables = {}
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        group = self.param_groups[-1]
+        try:
+            for name in ("lr", "eps", "weight_decay"):
+                if not float(group[name]) >= 0.0:
+                    raise ValueError("%s must not be negative" % name)
+            if len(group["betas"]) != 2 or not all(0.0 <= float(b) < 1.0 for b in group["betas"]):
+                raise ValueError("betas must be two numbers in [0, 1)")
+            seen = set()
+            for p in group["params"]:
+                if id(p) in seen:
+                    raise ValueError("a parameter appears twice in the group")
+                seen.add(id(p))
+                _check_param(p, "parameter")
+            if len({p.device for p in group["params"]}) > 1:
+                raise ValueError("the parameters of one group must be on one device")
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    # -- states --------------------------------------------------------------------------------------------------
+    def _state(self, p):
+        s = self.state[p]
+        if not s:
+            n, dev = p.numel(), p.device
+            s["step"] = 0
+            if self.state_bits == 32:
+                s["exp_avg"], s["exp_avg_sq"] = torch.zeros_like(p), torch.zeros_like(p)
+            else:
+                s["exp_avg"] = torch.zeros(n, dtype=torch.int8, device=dev)
+                s["exp_avg_sq"] = torch.zeros(n, dtype=torch.uint8, device=dev)
+                s["exp_avg_scale"] = torch.zeros(_blocks(n), device=dev)
+                s["exp_avg_sq_scale"] = torch.zeros(_blocks(n), device=dev)
+        return s
+
+    def _names(self):
+        return ("exp_avg", "exp_avg_sq") + (("exp_avg_scale", "exp_avg_sq_scale") if self.state_bits == 8 else ())
+
+    def adopt(self, states, step):
+        """Continues from state tensors the caller already holds, without copying them: for each parameter (in group
+        order) ``(exp_avg, exp_avg_sq)`` in float32, or with 8-bit states ``(exp_avg int8, exp_avg_sq uint8, exp_avg_scale,
+        exp_avg_sq_scale)``.  ``step``: the number of steps done.  The tensors are updated in place from then on.  A step
+        captured into a CUDA graph before goes on using the states it was captured with: capture it again."""
+        params = [p for g in self.param_groups for p in g["params"]]
+        names = self._names()
+        if len(states) != len(params):
+            raise ValueError("%d states for %d parameters" % (len(states), len(params)))
+        if int(step) < 0:
+            raise ValueError("step must not be negative")
+        types = (torch.float32,) * 2 if self.state_bits == 32 else (torch.int8, torch.uint8, torch.float32, torch.float32)
+        for p, st in zip(params, states):
+            if len(st) != len(names):
+                raise ValueError("each state is %s" % ", ".join(names))
+            for t, name, dtype in zip(st, names, types):
+                n = _blocks(p.numel()) if name.endswith("scale") else p.numel()
+                if t.dtype != dtype or t.device != p.device or t.numel() != n or not t.is_contiguous():
+                    raise ValueError("%s must be a contiguous %s tensor of %d values on %s" % (name, dtype, n, p.device))
+        for p, st in zip(params, states):
+            self.state[p] = dict(step=int(step), **dict(zip(names, st)))
+        self._tables.clear()
+
+    def _table(self, index):
+        """The C ABI's rows for one group; parameter and gradient addresses are filled in at each call."""
+        group = self.param_groups[index]
+        t = self._tables.get(index)
+        if t is None or t["params"] != len(group["params"]):
+            states = [self._state(p) for p in group["params"]]
+            rows = np.zeros(len(states), _ROW)
+            for name in self._names():
+                rows[name] = [s[name].data_ptr() for s in states]
+            rows["count"] = [p.numel() for p in group["params"]]
+            steps = {s["step"] for s in states}
+            device_step = None
+            if self.capturable and states:
+                if len(steps) > 1:
+                    raise ValueError("capturable: all parameters of a group must have done the same number of steps")
+                device_step = torch.tensor([steps.pop()], dtype=torch.int64, device=group["params"][0].device)
+            t = self._tables[index] = dict(params=len(states), rows=rows, states=states, device_step=device_step)
+        return t
+
+    def _steps(self, t):
+        if t["device_step"] is not None:
+            n = int(t["device_step"].item())
+            for s in t["states"]:
+                s["step"] = n
+
+    # -- the step ------------------------------------------------------------------------------------------------
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for index, group in enumerate(self.param_groups):
+            if group["params"]:
+                with torch.cuda.device(group["params"][0].device):
+                    self._step_group(index, group)
+        return loss
+
+    def _step_group(self, index, group):
+        params = group["params"]
+        if not self.capturable and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW.step under CUDA graph capture needs capturable=True")
+        t = self._table(index)
+        rows, states, live = t["rows"], t["states"], []
+        grads, ptrs, dev = [], [], params[0].device
+        for i, p in enumerate(params):
+            g = p.grad
+            if g is None:
+                grads.append(0)
+                ptrs.append(0)
+                continue
+            if g.dtype != torch.float32 or g.device != dev or g.layout != torch.strided:
+                raise TypeError("gradients must be dense float32 tensors on the parameter's device")
+            if not g.is_contiguous():
+                g = p.grad = g.contiguous()
+            if not p.is_contiguous():
+                raise ValueError("parameters must stay contiguous")
+            live.append(i)
+            grads.append(g.data_ptr())
+            ptrs.append(p.data_ptr())
+        if self.capturable and len(live) != len(params):
+            raise RuntimeError("capturable: every parameter of the group needs a gradient")
+        if not live:
+            return
+        rows["param"], rows["grad"] = ptrs, grads
+        # the kernel writes through addresses: tell autograd, so that a graph that saved the old values refuses them
+        torch.autograd.graph.increment_version([params[i] for i in live] if len(live) != len(params) else params)
+        if t["device_step"] is not None:
+            self._launch(group, rows, 0, t["device_step"].data_ptr())
+            return
+        by_step = {}
+        for i in live:
+            states[i]["step"] += 1
+            by_step.setdefault(states[i]["step"], []).append(i)
+        for n, which in by_step.items():
+            self._launch(group, rows if len(which) == len(params) else np.ascontiguousarray(rows[which]), n, None)
+
+    def _launch(self, group, rows, n, device_step):
+        b1, b2 = group["betas"]
+        h = _lib.AdamwHyper(float(group["lr"]), float(b1), float(b2), float(group["eps"]), float(group["weight_decay"]), n,
+                            device_step, self.state_bits)
+        rc = _lib.lib().rgb200_adamw_step(rows.ctypes.data, len(rows), C.byref(h), _stream(None))
+        if rc != cudaSuccess:
+            raise ReproGemmError(rc, "adamw_step")
+
+    # -- values of the moments -----------------------------------------------------------------------------------
+    @torch.no_grad()
+    def read_states(self, exp_avgs, exp_avg_sqs):
+        """Writes the moments' values into the given contiguous float32 tensors, one for each parameter in group order."""
+        self._values("rgb200_adamw_states_read", exp_avgs, exp_avg_sqs)
+
+    @torch.no_grad()
+    def write_states(self, exp_avgs, exp_avg_sqs):
+        """The reverse of read_states: the moments become the given values (their nearest codes with 8-bit states)."""
+        self._values("rgb200_adamw_states_write", exp_avgs, exp_avg_sqs)
+
+    def _values(self, call, ms, vs):
+        count = sum(len(g["params"]) for g in self.param_groups)
+        if len(ms) != count or len(vs) != count:
+            raise ValueError("one tensor is needed for each of the %d parameters" % count)
+        at = 0
+        for index, group in enumerate(self.param_groups):
+            params = group["params"]
+            if not params:
+                continue
+            t = self._table(index)
+            gm, gv, dev = ms[at:at + len(params)], vs[at:at + len(params)], params[0].device
+            at += len(params)
+            for x, n in zip(list(gm) + list(gv), list(t["rows"]["count"]) * 2):
+                if x.dtype != torch.float32 or x.device != dev or x.numel() != n or not x.is_contiguous():
+                    raise ValueError("the moments' values are contiguous float32 tensors of the parameters' sizes on their device")
+            with torch.cuda.device(dev):
+                if self.state_bits == 32:
+                    for s, m, v in zip(t["states"], gm, gv):
+                        pairs = ((m, s["exp_avg"]), (v, s["exp_avg_sq"]))
+                        for x, own in pairs:
+                            (x.view(-1).copy_(own.view(-1)) if call.endswith("read") else own.view(-1).copy_(x.view(-1)))
+                    continue
+                rows = t["rows"].copy()
+                rows["param"], rows["grad"] = [m.data_ptr() for m in gm], [v.data_ptr() for v in gv]
+                rc = getattr(_lib.lib(), call)(rows.ctypes.data, len(rows), _stream(None))
+                if rc != cudaSuccess:
+                    raise ReproGemmError(rc, call[7:])
+
+    def state_dict(self):
+        params = [p for g in self.param_groups for p in g["params"]]
+        ms, vs = ([torch.zeros(p.shape, dtype=torch.float32, device=p.device) for p in params] for _ in range(2))
+        self.read_states(ms, vs)
+        for index in range(len(self.param_groups)):
+            if self.param_groups[index]["params"]:
+                self._steps(self._tables[index])
+        at, groups = 0, []
+        for g in self.param_groups:
+            n = len(g["params"])
+            groups.append({**{k: v for k, v in g.items() if k != "params"}, "params": list(range(at, at + n))})
+            at += n
+        state = {i: dict(step=self.state[p]["step"], exp_avg=ms[i], exp_avg_sq=vs[i]) for i, p in enumerate(params)}
+        return {"state": state, "param_groups": groups}
+
+    def load_state_dict(self, state_dict):
+        groups, params = state_dict["param_groups"], [p for g in self.param_groups for p in g["params"]]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError("the loaded state has other parameter groups")
+        ids = [i for g in groups for i in g["params"]]
+        state = state_dict["state"]
+        for p, i in zip(params, ids):
+            for k in ("exp_avg", "exp_avg_sq"):
+                if i in state and state[i][k].numel() != p.numel():
+                    raise ValueError("the loaded state has other sizes")
+        for mine, theirs in zip(self.param_groups, groups):
+            mine.update({k: v for k, v in theirs.items() if k != "params"})
+        ms, vs = [], []
+        for p, i in zip(params, ids):
+            s = self._state(p)
+            got = state.get(i)
+            s["step"] = int(got["step"]) if got else 0
+            for name, to in (("exp_avg", ms), ("exp_avg_sq", vs)):
+                to.append(got[name].to(device=p.device, dtype=torch.float32).contiguous() if got else torch.zeros(p.shape, device=p.device))
+        self.write_states(ms, vs)                    # into the tensors there are: a captured step stays valid
+        for index, t in list(self._tables.items()):
+            steps = {s["step"] for s in t["states"]}
+            if t["device_step"] is not None:
+                if len(steps) > 1:
+                    raise ValueError("capturable: all parameters of a group must have done the same number of steps")
+                t["device_step"].fill_(steps.pop())
+
+
+def _check_param(p, name):
+    if p.dtype != torch.float32:
+        raise TypeError("%s must be float32" % name)
+    if not p.is_cuda:
+        raise RuntimeError("%s is not a CUDA tensor: this library has no CPU path" % name)
+    if not p.is_contiguous():
+        raise ValueError("%s must be contiguous" % name)
