@@ -156,14 +156,35 @@ __device__ __forceinline__ float decode_v(int q, float scale) {
     return __fmul_rn(__fmul_rn(t, t), scale);
 }
 // `scale`: the block's largest magnitude, or 1 for a block of zeros.
-__device__ __forceinline__ int encode_m(float m, float scale) {
-    const int q = __float2int_rn(__fmul_rn(__fsqrt_rn(__fdiv_rn(fabsf(m), scale)), 127.0f));
+__device__ __forceinline__ int encode_m_exact(float m, float scale) {
+    return __float2int_rn(__fmul_rn(__fsqrt_rn(__fdiv_rn(fabsf(m), scale)), 127.0f));
+}
+__device__ __forceinline__ int encode_v_exact(float v, float scale) {
+    return __float2int_rn(__fmul_rn(__fsqrt_rn(__fsqrt_rn(__fdiv_rn(v, scale))), 255.0f));
+}
+__device__ __forceinline__ float sqrt_fast(float x) {
+    float r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// The definition's quotient and roots, correctly rounded, would cost more time than the memory traffic.  `inv` = 1 / scale and the
+// hardware's approximate root (relative error 2^-23) give the companded value within 255 * 8 * 2^-24 < 1.3e-4 of the
+// definition's, so the code can differ only where the value lies that close to a border between two codes; those (one
+// in two thousand) take the definition's operations.  inv = 0 marks a scale whose reciprocal leaves the normal range.
+constexpr float CODE_BORDER = 0.5f - 2.5e-4f;
+__device__ __forceinline__ int encode_m(float m, float scale, float inv) {
+    const float t = sqrt_fast(fabsf(m) * inv) * 127.0f, r = rintf(t);
+    int q = (int)r;
+    if (fabsf(t - r) > CODE_BORDER || inv == 0.0f) q = encode_m_exact(m, scale);
     return m < 0.0f ? -q : q;
 }
-__device__ __forceinline__ int encode_v(float v, float scale) {
-    const int q = __float2int_rn(__fmul_rn(__fsqrt_rn(__fsqrt_rn(__fdiv_rn(v, scale))), 255.0f));
+__device__ __forceinline__ int encode_v(float v, float scale, float inv) {
+    const float t = sqrt_fast(sqrt_fast(v * inv)) * 255.0f, r = rintf(t);
+    int q = (int)r;
+    if (fabsf(t - r) > CODE_BORDER || inv == 0.0f) q = encode_v_exact(v, scale);
     return q == 0 && v > 0.0f ? 1 : q;
 }
+__device__ __forceinline__ float code_inverse(float scale) { return scale > 0x1p-100f && scale < 0x1p100f ? __frcp_rn(scale) : 0.0f; }
 
 // Largest magnitude over the warp's block, NaN if any value is not finite (the bits of non-negative floats order as
 // integers, and infinity and NaN lie above every finite value).
@@ -222,13 +243,14 @@ __device__ __forceinline__ void encode_block(const float (&m)[8], const float (&
     const float tm = block_scale(m), tv = block_scale(v);
     uint2 cm = make_uint2(0u, 0u), cv = make_uint2(0u, 0u);
     const float dm = tm > 0.0f ? tm : 1.0f, dv = tv > 0.0f ? tv : 1.0f;
+    const float im = code_inverse(dm), iv = code_inverse(dv);
     if (!isnan(tm)) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) (j < 4 ? cm.x : cm.y) |= ((uint32_t)encode_m(m[j], dm) & 0xFFu) << (8 * (j & 3));
+        for (int j = 0; j < 8; ++j) (j < 4 ? cm.x : cm.y) |= ((uint32_t)encode_m(m[j], dm, im) & 0xFFu) << (8 * (j & 3));
     }
     if (!isnan(tv)) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) (j < 4 ? cv.x : cv.y) |= ((uint32_t)encode_v(v[j], dv) & 0xFFu) << (8 * (j & 3));
+        for (int j = 0; j < 8; ++j) (j < 4 ? cv.x : cv.y) |= ((uint32_t)encode_v(v[j], dv, iv) & 0xFFu) << (8 * (j & 3));
     }
     store_codes(qm, live, wide, cm);
     store_codes(qv, live, wide, cv);

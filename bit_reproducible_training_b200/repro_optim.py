@@ -6,12 +6,15 @@ the moments held in FP32 or in 8 bits.  Every value goes through the same fixed 
 CUDA float32 parameters only; there is no CPU path.
 """
 import ctypes as C
+import sys
 
 import numpy as np
 import torch
 
 from . import _lib
 from .repro_gemm import ReproGemmError, _stream, cudaSuccess
+
+_torch_optimizer = sys.modules[torch.optim.Optimizer.__module__]        # torch.optim hides the module's own name
 
 STATE_BLOCK = 256           # values of a tensor that share one scale (8-bit states)
 
@@ -113,14 +116,15 @@ class AdamW(torch.optim.Optimizer):
             rows = np.zeros(len(states), _ROW)
             for name in self._names():
                 rows[name] = [s[name].data_ptr() for s in states]
-            rows["count"] = [p.numel() for p in group["params"]]
+            counts = [s["exp_avg"].numel() for s in states]
+            rows["count"] = counts
             steps = {s["step"] for s in states}
             device_step = None
             if self.capturable and states:
                 if len(steps) > 1:
                     raise ValueError("capturable: all parameters of a group must have done the same number of steps")
                 device_step = torch.tensor([steps.pop()], dtype=torch.int64, device=group["params"][0].device)
-            t = self._tables[index] = dict(params=len(states), rows=rows, states=states, device_step=device_step)
+            t = self._tables[index] = dict(params=len(states), rows=rows, counts=counts, states=states, device_step=device_step)
         return t
 
     def _steps(self, t):
@@ -130,8 +134,18 @@ class AdamW(torch.optim.Optimizer):
                 s["step"] = n
 
     # -- the step ------------------------------------------------------------------------------------------------
-    @torch.no_grad()
     def step(self, closure=None):
+        # torch wraps step() of every optimizer in a profiler range and its hooks, which takes longer than the step of a small
+        # model; here the wrapped form runs only when a hook is registered (or the profiler is on)
+        if (self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or torch.autograd.profiler._is_profiler_enabled or
+                getattr(_torch_optimizer, "_global_optimizer_pre_hooks", None) or
+                getattr(_torch_optimizer, "_global_optimizer_post_hooks", None)):
+            return _hooked_step(self, closure)
+        return self._step(closure)
+
+    step.hooked = True                  # tells torch.optim.Optimizer not to wrap it again
+
+    def _step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -143,43 +157,43 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _step_group(self, index, group):
-        params = group["params"]
         if not self.capturable and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW.step under CUDA graph capture needs capturable=True")
         t = self._table(index)
-        rows, states, live = t["rows"], t["states"], []
-        grads, ptrs, dev = [], [], params[0].device
-        for i, p in enumerate(params):
-            g = p.grad
-            if g is None:
-                grads.append(0)
-                ptrs.append(0)
-                continue
-            if g.dtype != torch.float32 or g.device != dev or g.layout != torch.strided:
-                raise TypeError("gradients must be dense float32 tensors on the parameter's device")
-            if not g.is_contiguous():
-                g = p.grad = g.contiguous()
-            if not p.is_contiguous():
-                raise ValueError("parameters must stay contiguous")
-            live.append(i)
-            grads.append(g.data_ptr())
-            ptrs.append(p.data_ptr())
-        if self.capturable and len(live) != len(params):
-            raise RuntimeError("capturable: every parameter of the group needs a gradient")
-        if not live:
-            return
-        rows["param"], rows["grad"] = ptrs, grads
+        params, states, rows, counts = group["params"], t["states"], t["rows"], t["counts"]
+        grads = [p.grad for p in params]
+        live = [i for i, g in enumerate(grads) if g is not None]
+        if len(live) != len(params):
+            if self.capturable:
+                raise RuntimeError("capturable: every parameter of the group needs a gradient")
+            if not live:
+                return
+            params, states, grads = ([x[i] for i in live] for x in (params, states, grads))
+            rows, counts = np.ascontiguousarray(rows[live]), [counts[i] for i in live]
+        T, dev = torch.Tensor, {params[0].get_device()}
+        # whole-list checks: a call's host time is what bounds a step over many small tensors
+        if {g.dtype for g in grads} != {torch.float32} or {g.layout for g in grads} != {torch.strided} or set(map(T.get_device, grads)) != dev:
+            raise TypeError("gradients must be dense float32 tensors on the parameter's device")
+        if not all(map(T.is_contiguous, grads)):
+            grads = [g.detach().contiguous() for g in grads]          # alive until the launch below is enqueued
+        if {p.dtype for p in params} != {torch.float32} or set(map(T.get_device, params)) != dev or not all(map(T.is_contiguous, params)):
+            raise ValueError("parameters must stay contiguous float32 tensors on the device they were on")
+        if list(map(T.numel, params)) != counts or list(map(T.numel, grads)) != counts:
+            raise ValueError("parameters and gradients must keep the size the states were made for")
+        rows["param"], rows["grad"] = list(map(T.data_ptr, params)), list(map(T.data_ptr, grads))
         # the kernel writes through addresses: tell autograd, so that a graph that saved the old values refuses them
-        torch.autograd.graph.increment_version([params[i] for i in live] if len(live) != len(params) else params)
+        torch.autograd.graph.increment_version(params)
         if t["device_step"] is not None:
             self._launch(group, rows, 0, t["device_step"].data_ptr())
             return
-        by_step = {}
-        for i in live:
-            states[i]["step"] += 1
-            by_step.setdefault(states[i]["step"], []).append(i)
-        for n, which in by_step.items():
-            self._launch(group, rows if len(which) == len(params) else np.ascontiguousarray(rows[which]), n, None)
+        steps = [s["step"] + 1 for s in states]
+        for s, n in zip(states, steps):
+            s["step"] = n
+        if min(steps) == max(steps):
+            self._launch(group, rows, steps[0], None)
+            return
+        for n in sorted(set(steps)):
+            self._launch(group, np.ascontiguousarray(rows[[i for i, k in enumerate(steps) if k == n]]), n, None)
 
     def _launch(self, group, rows, n, device_step):
         b1, b2 = group["betas"]
@@ -269,6 +283,9 @@ class AdamW(torch.optim.Optimizer):
                 if len(steps) > 1:
                     raise ValueError("capturable: all parameters of a group must have done the same number of steps")
                 t["device_step"].fill_(steps.pop())
+
+
+_hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)
 
 
 def _check_param(p, name):

@@ -283,3 +283,27 @@ def test_step_on_another_stream():
     b.step()
     torch.cuda.synchronize()
     assert np.array_equal(bits(ps[0]), bits(qs[0]))
+
+
+def test_hooks_and_schedulers_work():
+    ps, gs = make([64], 13)
+    ps[0].grad = gs[0]
+    opt = repro_optim.AdamW(ps, **HYPER)
+    seen = []
+    opt.register_step_pre_hook(lambda o, a, k: seen.append("before"))
+    opt.register_step_post_hook(lambda o, a, k: seen.append("after"))
+    sched = torch.optim.lr_scheduler.StepLR(opt, 1, gamma=0.5)
+    assert opt.step(lambda: 5.0) == 5.0
+    sched.step()
+    assert seen == ["before", "after"] and opt.param_groups[0]["lr"] == HYPER["lr"] * 0.5 and opt.state[ps[0]]["step"] == 1
+
+
+def test_a_parameter_that_changed_its_size_is_refused():
+    ps, gs = make([64, 8], 14)
+    for p, g in zip(ps, gs):
+        p.grad = g
+    opt = repro_optim.AdamW(ps, **HYPER)
+    opt.step()
+    ps[0].data = torch.zeros(32, device="cuda")
+    with pytest.raises(ValueError):
+        opt.step()
