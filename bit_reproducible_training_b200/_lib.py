@@ -29,6 +29,12 @@ class AdamwHyper(C.Structure):
         ("step", C.c_longlong), ("device_step", C.c_void_p), ("state_bits", C.c_int)]
 
 
+class BlockNorm(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("rows", "dim", "groups", "kind")] + [("scale", C.c_float), ("eps", C.c_float)] + [
+        (n, C.c_void_p) for n in ("x", "y", "weight", "bias", "post_weight", "gate", "r", "h", "stats", "dr", "dh", "dx", "dy",
+                                  "dweight", "dbias", "dpost_weight", "dgate")]
+
+
 _lib = None
 
 
@@ -86,5 +92,9 @@ def lib():
     L.rgb200_adamw_step.argtypes = [vp, i, C.POINTER(AdamwHyper), vp]
     L.rgb200_adamw_states_read.argtypes = [vp, i, vp]
     L.rgb200_adamw_states_write.argtypes = [vp, i, vp]
+    L.rgb200_block_norm_forward.argtypes = [C.POINTER(BlockNorm), vp]
+    L.rgb200_block_norm_backward_workspace.argtypes = [i, i, i]
+    L.rgb200_block_norm_backward_workspace.restype = C.c_size_t
+    L.rgb200_block_norm_backward.argtypes = [C.POINTER(BlockNorm), vp, C.c_size_t, vp]
     _lib = L
     return L

@@ -1,0 +1,133 @@
+// Host side of the block-norm entry points declared in include/rgb200_train.h.
+#include "../../include/rgb200_train.h"
+#include "rgb200_host.h"
+#include "rgb200_norm.cuh"
+
+namespace rgb200 {
+namespace {
+
+// Threads of a row, from its length alone.
+int norm_threads(int dim) {
+    int t = 32;
+    while (t * NORM_VALUES < dim) t *= 2;
+    return t;
+}
+
+bool good_norm(const rgb200_block_norm* n) {
+    if (!n || n->rows < 0 || n->dim < 1 || n->dim > NORM_MAX_DIM || n->groups < 1 || (n->kind != RGB200_NORM_RMS && n->kind != RGB200_NORM_LAYER)) return false;
+    if (!(n->eps >= 0.0f) || n->scale != n->scale) return false;
+    if (n->rows % n->groups != 0) return false;
+    if (!n->gate && n->groups != 1) return false;
+    if (n->rows > 0 && (!n->x || !n->weight || (!n->y && (n->post_weight || n->gate)))) return false;    // no rows: no tensors needed
+    return true;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Row ranges of the backward pass, from the sizes alone: as many as fill the GPU's 148 SMs with two rows of 256 threads each (or
+// their equivalent), at least eight rows long so that their column sums stay a small part of the traffic.
+struct NormParts { int per_group, rows, total; };
+NormParts norm_parts(int rows, int dim, int groups) {
+    NormParts p = {0, 0, 0};
+    if (rows == 0) return p;
+    const int group_rows = rows / groups, tpr = norm_threads(dim);
+    long long want = 148ll * (tpr >= 512 ? 1024 / tpr : 512 / tpr) / groups;
+    if (want < 1) want = 1;
+    if (want > (group_rows + 7) / 8) want = (group_rows + 7) / 8;
+    p.rows = (int)((group_rows + want - 1) / want);
+    p.per_group = (group_rows + p.rows - 1) / p.rows;
+    p.total = p.per_group * groups;
+    return p;
+}
+
+NormParams norm_params(const rgb200_block_norm* n) {
+    NormParams P = {};
+    P.x = n->x; P.y = n->y; P.w = n->weight; P.b = n->bias; P.pw = n->post_weight; P.gate = n->gate;
+    P.r = n->r; P.h = n->h; P.stats = n->stats;
+    P.rows = n->rows; P.dim = n->dim; P.groups = n->groups;
+    P.group_rows = n->rows > 0 ? n->rows / n->groups : 1;
+    P.layer = n->kind == RGB200_NORM_LAYER; P.scale = n->scale; P.eps = n->eps;
+    P.dr = n->dr; P.dh = n->dh; P.dx = n->dx; P.dy = n->dy;
+    P.dw = n->dweight; P.db = n->dbias; P.dpw = n->dpost_weight; P.dgate = n->dgate;
+    P.wide = n->dim % 4 == 0;
+    for (const void* p : {(const void*)n->x, (const void*)n->y, (const void*)n->weight, (const void*)n->bias, (const void*)n->post_weight, (const void*)n->gate,
+                          (const void*)n->r, (const void*)n->h, (const void*)n->dr, (const void*)n->dh, (const void*)n->dx, (const void*)n->dy})
+        if (!aligned16(p)) P.wide = 0;
+    return P;
+}
+
+template <int TPR, int V>
+void launch_norm(const NormParams& P, bool backward, cudaStream_t st) {
+    constexpr int CTA = norm_cta(TPR), GROUPS = CTA / TPR;
+    const int items = backward ? P.parts_total : P.rows, grid = (items - 1) / GROUPS + 1;
+    if (!backward) {
+        if (!P.y) block_norm_kernel<TPR, V, NORM_ONLY><<<grid, CTA, 0, st>>>(P);
+        else if (!P.pw) block_norm_kernel<TPR, V, NORM_RESIDUAL><<<grid, CTA, 0, st>>>(P);
+        else block_norm_kernel<TPR, V, NORM_POST><<<grid, CTA, 0, st>>>(P);
+    } else {
+        if (!P.y) block_norm_backward_kernel<TPR, V, NORM_ONLY><<<grid, CTA, 0, st>>>(P);
+        else if (!P.pw) block_norm_backward_kernel<TPR, V, NORM_RESIDUAL><<<grid, CTA, 0, st>>>(P);
+        else block_norm_backward_kernel<TPR, V, NORM_POST><<<grid, CTA, 0, st>>>(P);
+    }
+}
+
+template <int V>
+void dispatch_norm(const NormParams& P, bool backward, cudaStream_t st) {
+    switch (norm_threads(P.dim)) {
+        case 32: return launch_norm<32, V>(P, backward, st);
+        case 64: return launch_norm<64, V>(P, backward, st);
+        case 128: return launch_norm<128, V>(P, backward, st);
+        case 256: return launch_norm<256, V>(P, backward, st);
+        case 512: return launch_norm<512, V>(P, backward, st);
+        default: return launch_norm<1024, V>(P, backward, st);
+    }
+}
+
+}  // namespace
+}  // namespace rgb200
+
+using namespace rgb200;
+
+extern "C" int rgb200_block_norm_forward(const rgb200_block_norm* n, void* stream) {
+    if (!good_norm(n)) return cudaErrorInvalidValue;
+    if (n->rows > 0 && (!n->h || (n->y && !n->r))) return cudaErrorInvalidValue;
+    cudaError_t e = check_b200();
+    if (e != cudaSuccess || n->rows == 0) return e;
+    const NormParams P = norm_params(n);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (P.dim % 4 == 0) dispatch_norm<4>(P, false, st);
+    else dispatch_norm<1>(P, false, st);
+    return cudaGetLastError();
+}
+
+extern "C" size_t rgb200_block_norm_backward_workspace(int rows, int dim, int groups) {
+    if (rows < 0 || dim < 1 || dim > NORM_MAX_DIM || groups < 1 || rows % groups != 0) return 0;
+    const size_t n = (size_t)norm_parts(rows, dim, groups).total * 3 * dim * sizeof(float);
+    return n < 256 ? 256 : n;
+}
+
+extern "C" int rgb200_block_norm_backward(const rgb200_block_norm* n, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!good_norm(n) || !workspace || workspace_bytes < rgb200_block_norm_backward_workspace(n->rows, n->dim, n->groups) || !aligned16(workspace))
+        return cudaErrorInvalidValue;
+    if (n->rows > 0 && (!n->dh || !n->stats || (n->y && !n->r))) return cudaErrorInvalidValue;
+    if ((n->dy && !n->y) || (n->dpost_weight && !n->post_weight) || (n->dgate && !n->gate)) return cudaErrorInvalidValue;
+    cudaError_t e = check_b200();
+    if (e != cudaSuccess) return e;
+    NormParams P = norm_params(n);
+    const NormParts parts = norm_parts(n->rows, n->dim, n->groups);
+    P.parts = static_cast<float*>(workspace);
+    P.rows_per_part = parts.rows; P.parts_per_group = parts.per_group; P.parts_total = parts.total;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (n->rows > 0) {
+        if (P.dim % 4 == 0) dispatch_norm<4>(P, true, st);
+        else dispatch_norm<1>(P, true, st);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
+    if (P.dgate || P.dpw) {
+        if (P.groups > 1)
+            norm_group_sums_kernel<<<dim3((P.dim + 255) / 256, P.groups < 4096 ? P.groups : 4096), 256, 0, st>>>(P);
+    }
+    if (P.dw || P.db || P.dpw || P.dgate)
+        norm_column_sums_kernel<<<dim3((P.dim + 31) / 32, P.dgate || P.dpw ? 3 : 2), 32 * NORM_SUM_WARPS, 0, st>>>(P);
+    return cudaGetLastError();
+}

@@ -1,21 +1,13 @@
-// Host side of the AdamW entry points declared in include/rgb200.h.  Tensors travel to the kernels by value in the launch
+// Host side of the AdamW entry points declared in include/rgb200_train.h.  Tensors travel to the kernels by value in the launch
 // parameters, so a call copies nothing to the device, keeps nothing, and can be captured into a CUDA graph.
 #include <new>
 
-#include "../../include/rgb200.h"
+#include "../../include/rgb200_train.h"
+#include "rgb200_host.h"
 #include "rgb200_optim.cuh"
 
 namespace rgb200 {
 namespace {
-
-cudaError_t check_b200() {
-    int dev, major = 0, minor = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
-    if (e != cudaSuccess) return e;
-    return major == 10 && minor == 0 ? cudaSuccess : cudaErrorNotSupported;
-}
 
 bool good_tensors(const rgb200_adamw_tensor* t, int count, int bits) {
     if (count < 0 || (count > 0 && !t) || (bits != 8 && bits != 32)) return false;

@@ -146,45 +146,47 @@ adamw32_kernel(const __grid_constant__ OptTable<CAP> T, const __grid_constant__ 
 // ------------------------------------------------------------------------------------------
 constexpr float INV127 = (float)(1.0 / 127.0), INV255 = (float)(1.0 / 255.0);
 
-__device__ __forceinline__ float decode_m(int q, float scale) {
-    const float t = __fmul_rn((float)q, INV127);
+// Conversions between codes and floats go through the mantissa of 2^23 + q and 1.5 * 2^23 + q (exact, and the addition
+// rounds to nearest-even as the definition does): the conversion instructions share the slow pipe with the roots and reciprocals, of
+// which a value needs five already.
+constexpr float TWO23 = 8388608.0f, ROUNDER = 12582912.0f;
+__device__ __forceinline__ float code_value(uint32_t word, int j, float offset) {      // float(byte j of word) - offset + 2^23
+    return __fsub_rn(__uint_as_float(__byte_perm(word, 0x4B000000u, 0x7650u | j)), offset);
+}
+__device__ __forceinline__ float decode_m(uint32_t word, int j, float scale) {         // word: codes with their sign bits flipped
+    const float t = __fmul_rn(code_value(word, j, TWO23 + 128.0f), INV127);
     return __fmul_rn(__fmul_rn(t, fabsf(t)), scale);
 }
-__device__ __forceinline__ float decode_v(int q, float scale) {
-    float t = __fmul_rn((float)q, INV255);
+__device__ __forceinline__ float decode_v(uint32_t word, int j, float scale) {
+    float t = __fmul_rn(code_value(word, j, TWO23), INV255);
     t = __fmul_rn(t, t);
     return __fmul_rn(__fmul_rn(t, t), scale);
 }
-// `scale`: the block's largest magnitude, or 1 for a block of zeros.
-__device__ __forceinline__ int encode_m_exact(float m, float scale) {
-    return __float2int_rn(__fmul_rn(__fsqrt_rn(__fdiv_rn(fabsf(m), scale)), 127.0f));
+// `scale`: the block's largest magnitude, or 1 for a block of zeros.  The definition's companded values, signed for m.
+__device__ __forceinline__ float compand_m_exact(float m, float scale) {
+    return copysignf(__fmul_rn(__fsqrt_rn(__fdiv_rn(fabsf(m), scale)), 127.0f), m);
 }
-__device__ __forceinline__ int encode_v_exact(float v, float scale) {
-    return __float2int_rn(__fmul_rn(__fsqrt_rn(__fsqrt_rn(__fdiv_rn(v, scale))), 255.0f));
+__device__ __forceinline__ float compand_v_exact(float v, float scale) {
+    return __fmul_rn(__fsqrt_rn(__fsqrt_rn(__fdiv_rn(v, scale))), 255.0f);
 }
 __device__ __forceinline__ float sqrt_fast(float x) {
     float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 // The definition's quotient and roots, correctly rounded, would cost more time than the memory traffic.  `inv` = 1 / scale and the
 // hardware's approximate root (relative error 2^-23) give the companded value within 255 * 8 * 2^-24 < 1.3e-4 of the
-// definition's, so the code can differ only where the value lies that close to a border between two codes; those (one
-// in two thousand) take the definition's operations.  inv = 0 marks a scale whose reciprocal leaves the normal range.
-constexpr float CODE_BORDER = 0.5f - 2.5e-4f;
-__device__ __forceinline__ int encode_m(float m, float scale, float inv) {
-    const float t = sqrt_fast(fabsf(m) * inv) * 127.0f, r = rintf(t);
-    int q = (int)r;
-    if (fabsf(t - r) > CODE_BORDER || inv == 0.0f) q = encode_m_exact(m, scale);
-    return m < 0.0f ? -q : q;
-}
-__device__ __forceinline__ int encode_v(float v, float scale, float inv) {
-    const float t = sqrt_fast(sqrt_fast(v * inv)) * 255.0f, r = rintf(t);
-    int q = (int)r;
-    if (fabsf(t - r) > CODE_BORDER || inv == 0.0f) q = encode_v_exact(v, scale);
-    return q == 0 && v > 0.0f ? 1 : q;
-}
+// definition's, so a code can differ only where the value lies that close to a border between two codes; lanes that
+// hold such a value redo it with the definition's operations.  inv = 0 marks a scale whose reciprocal leaves the normal range.
+constexpr float CODE_BORDER = 0.5f - 2.0e-4f;
+__device__ __forceinline__ float compand_m(float m, float inv) { return copysignf(sqrt_fast(fabsf(m) * inv) * 127.0f, m); }
+__device__ __forceinline__ float compand_v(float v, float inv) { return sqrt_fast(sqrt_fast(v * inv)) * 255.0f; }
 __device__ __forceinline__ float code_inverse(float scale) { return scale > 0x1p-100f && scale < 0x1p100f ? __frcp_rn(scale) : 0.0f; }
+__device__ __forceinline__ float border_distance(float t) { return fabsf(t - ((t + ROUNDER) - ROUNDER)); }
+__device__ __forceinline__ uint32_t code_bits(float t) { return __float_as_uint(t + ROUNDER); }   // the code in the low byte
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
 
 // Largest magnitude over the warp's block, NaN if any value is not finite (the bits of non-negative floats order as
 // integers, and infinity and NaN lie above every finite value).
@@ -228,30 +230,46 @@ __device__ __forceinline__ void store_codes(uint8_t* q, int live, bool wide, uin
     for (int j = 0; j < 8; ++j)
         if (j < live) q[j] = (uint8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
 }
-__device__ __forceinline__ int code_byte(uint2 c, int j) { return (int)(((j < 4 ? c.x : c.y) >> (8 * (j & 3))) & 0xFFu); }
 
 __device__ __forceinline__ void decode_block(uint2 cm, uint2 cv, float sm, float sv, float (&m)[8], float (&v)[8]) {
+    cm.x ^= 0x80808080u;
+    cm.y ^= 0x80808080u;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        m[j] = decode_m((int)(int8_t)code_byte(cm, j), sm);
-        v[j] = decode_v(code_byte(cv, j), sv);
+        m[j] = decode_m(j < 4 ? cm.x : cm.y, j & 3, sm);
+        v[j] = decode_v(j < 4 ? cv.x : cv.y, j & 3, sv);
     }
 }
 
 __device__ __forceinline__ void encode_block(const float (&m)[8], const float (&v)[8], uint8_t* qm, uint8_t* qv, float* sm, float* sv,
                                              int lane, int live, bool wide) {
     const float tm = block_scale(m), tv = block_scale(v);
-    uint2 cm = make_uint2(0u, 0u), cv = make_uint2(0u, 0u);
-    const float dm = tm > 0.0f ? tm : 1.0f, dv = tv > 0.0f ? tv : 1.0f;
+    const float dm = tm > 0.0f ? tm : 1.0f, dv = tv > 0.0f ? tv : 1.0f;      // NaN: 1, and the codes below are dropped
     const float im = code_inverse(dm), iv = code_inverse(dv);
-    if (!isnan(tm)) {
+    float x[8], y[8], worst = im == 0.0f || iv == 0.0f ? 1.0f : 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) (j < 4 ? cm.x : cm.y) |= ((uint32_t)encode_m(m[j], dm, im) & 0xFFu) << (8 * (j & 3));
+    for (int j = 0; j < 8; ++j) {
+        x[j] = compand_m(m[j], im);
+        y[j] = compand_v(v[j], iv);
+        worst = fmaxf(worst, fmaxf(border_distance(x[j]), border_distance(y[j])));
     }
-    if (!isnan(tv)) {
+    if (worst > CODE_BORDER) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) (j < 4 ? cv.x : cv.y) |= ((uint32_t)encode_v(v[j], dv, iv) & 0xFFu) << (8 * (j & 3));
+        for (int j = 0; j < 8; ++j) {
+            if (im == 0.0f || border_distance(x[j]) > CODE_BORDER) x[j] = compand_m_exact(m[j], dm);
+            if (iv == 0.0f || border_distance(y[j]) > CODE_BORDER) y[j] = compand_v_exact(v[j], dv);
+        }
     }
+    uint32_t a[8], b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        a[j] = code_bits(x[j]);
+        b[j] = code_bits(v[j] > 0.0f ? fmaxf(y[j], 1.0f) : y[j]);            // a second moment that is not zero: at least code 1
+    }
+    uint2 cm = make_uint2(pack4(a[0], a[1], a[2], a[3]), pack4(a[4], a[5], a[6], a[7]));
+    uint2 cv = make_uint2(pack4(b[0], b[1], b[2], b[3]), pack4(b[4], b[5], b[6], b[7]));
+    if (isnan(tm)) cm = make_uint2(0u, 0u);
+    if (isnan(tv)) cv = make_uint2(0u, 0u);
     store_codes(qm, live, wide, cm);
     store_codes(qv, live, wide, cv);
     if (lane == 0) { *sm = tm; *sv = tv; }
@@ -262,7 +280,7 @@ enum OptMode : int { OPT_STEP, OPT_READ, OPT_WRITE };   // update; codes -> valu
 // OPT_STEP: p, g and the codes.  OPT_READ: the moments' values go to p (first) and g (second, written through a cast
 // away of const by the host's table); OPT_WRITE: they come from there.
 template <int CAP, OptMode MODE>
-__global__ void __launch_bounds__(OPT_THREADS)
+__global__ void __launch_bounds__(OPT_THREADS, 5)
 adamw8_kernel(const __grid_constant__ OptTable<CAP> T, const __grid_constant__ AdamwHyper H) {
     __shared__ AdamwScalars shared;
     AdamwScalars s = {};

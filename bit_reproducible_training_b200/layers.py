@@ -14,6 +14,7 @@ import torch
 
 from . import repro_conv as rc
 from . import repro_gemm as rg
+from . import repro_norm as rn
 
 _slices = 3
 _bias_grad = None
@@ -102,3 +103,62 @@ class Conv2d(torch.nn.Conv2d):
         if self.groups != 1 or self.dilation != (1, 1) or isinstance(self.padding, str) or self.padding_mode != "zeros":
             raise NotImplementedError("Conv2d supports stride and zero padding only")
         return _ConvFn.apply(x.contiguous(), self.weight, self.bias, self.stride, self.padding)
+
+
+class _BlockNormFn(torch.autograd.Function):
+    """block_norm and its gradients (repro_norm); r is an output of its own when there is a y."""
+
+    @staticmethod
+    def forward(ctx, x, y, weight, bias, post_weight, gate, residual_scale, kind, eps):
+        r, h, stats = rn.block_norm(x, y, weight=weight, bias=bias, post_weight=post_weight, gate=gate, residual_scale=residual_scale,
+                                    kind=kind, eps=eps, keep_stats=True)
+        ctx.save_for_backward(r, y, stats, weight, bias, post_weight, gate)
+        ctx.set_materialize_grads(False)
+        ctx.how = dict(residual_scale=residual_scale, kind=kind, eps=eps)
+        return h if y is None else (r, h)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        r, y, stats, weight, bias, post_weight, gate = ctx.saved_tensors
+        dr, dh = (None, grads[0]) if y is None else grads
+        if dh is None:
+            if dr is None:
+                return (None,) * 9
+            dh = torch.zeros_like(r)                 # only the residual stream is used
+        names = ("x", "y", "weight", "bias", "post_weight", "gate")
+        g = rn.block_norm_backward(dh, dr, r, y, stats, weight=weight, bias=bias, post_weight=post_weight, gate=gate,
+                                   wanted=[n for n, need in zip(names, ctx.needs_input_grad) if need], **ctx.how)
+        return g.x, g.y, g.weight, g.bias, g.post_weight, g.gate, None, None, None
+
+
+def block_norm(x, y=None, *, weight, bias=None, post_weight=None, gate=None, residual_scale=1.0, kind="rms", eps=1e-5):
+    """(r, h): the residual stream r = residual_scale * x + gate * (post_weight * N(y)) behind a block with output y, and
+    h = weight * N(r) + bias for the next block, differentiable in every tensor.  Without y, r is x.  See repro_norm.block_norm."""
+    tensors = (x, y, weight, bias, post_weight, gate)
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+        return rn.block_norm(x, y, weight=weight, bias=bias, post_weight=post_weight, gate=gate, residual_scale=residual_scale, kind=kind, eps=eps)[:2]
+    out = _BlockNormFn.apply(*tensors, residual_scale, kind, eps)
+    return (x, out) if y is None else out
+
+
+class BlockNorm(torch.nn.Module):
+    """The parameters of block_norm for rows of `dim` values: `post` adds the norm behind the block, `gate` a learned gate for
+    each channel (a gate computed elsewhere, [groups, dim], is passed to forward instead).  forward(x, y=None) -> (r, h)."""
+
+    def __init__(self, dim, kind="rms", bias=False, post=False, gate=False, residual_scale=1.0, eps=1e-5):
+        super().__init__()
+        if kind not in rn.KINDS:
+            raise ValueError("kind must be 'rms' or 'layer'")
+        self.kind, self.residual_scale, self.eps = kind, residual_scale, eps
+        self.weight = torch.nn.Parameter(torch.ones(dim))
+        self.bias = torch.nn.Parameter(torch.zeros(dim)) if bias else None
+        self.post_weight = torch.nn.Parameter(torch.ones(dim)) if post else None
+        self.gate = torch.nn.Parameter(torch.ones(dim)) if gate else None
+
+    def forward(self, x, y=None, gate=None):
+        if gate is not None and self.gate is not None:
+            raise ValueError("this module has a gate of its own")
+        has_y = y is not None
+        return block_norm(x, y, weight=self.weight, bias=self.bias, post_weight=self.post_weight if has_y else None,
+                          gate=(self.gate if gate is None else gate) if has_y else gate, residual_scale=self.residual_scale, kind=self.kind, eps=self.eps)

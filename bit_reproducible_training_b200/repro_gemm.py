@@ -154,7 +154,11 @@ _ws_cache = {}
 
 
 def _workspace(nbytes, device):
-    """One growing scratch tensor per device and stream, the role torch.empty plays in bindings.cpp:57."""
+    """One growing scratch tensor per device and stream, the role torch.empty plays in bindings.cpp:57.  A call that is
+    captured into a CUDA graph gets a tensor of its own from the graph's pool: two graphs captured on one stream may be
+    replayed at the same time."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device.index, torch.cuda.current_stream(device).cuda_stream)
     ws = _ws_cache.get(key)
     if ws is None or ws.numel() < nbytes:

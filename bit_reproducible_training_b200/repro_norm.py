@@ -1,0 +1,116 @@
+"""The norm behind a block, its gate, the residual stream and the norm in front of the next block, on the C ABI.
+
+    u = post_weight * N(y)        (u = y without a post weight)
+    r = residual_scale * x + gate * u
+    h = weight * N(r) + bias      (h = weight * N(x) + bias without y)
+
+One pass over the rows forward, one backward; ``layers.block_norm`` and ``layers.BlockNorm`` are the differentiable forms.
+CUDA float32 tensors only; sums are taken in an order that depends on the sizes alone.
+"""
+import ctypes as C
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from .repro_gemm import ReproGemmError, _check, _ptr, _stream, _workspace, cudaSuccess
+
+KINDS = {"rms": 0, "layer": 1}
+MAX_DIM = 8192
+
+
+@dataclass
+class NormGrads:
+    """What block_norm_backward returns; None where no gradient was asked for."""
+    x: torch.Tensor = None
+    y: torch.Tensor = None
+    weight: torch.Tensor = None
+    bias: torch.Tensor = None
+    post_weight: torch.Tensor = None
+    gate: torch.Tensor = None
+
+
+def _same_device(tensors):
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise ValueError("all tensors must be on one device")
+
+
+def _sizes(x, y, weight, bias, post_weight, gate, kind, eps):
+    if kind not in KINDS:
+        raise ValueError("kind must be 'rms' or 'layer'")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_DIM:
+        raise ValueError("the last dimension must have 1 to %d values" % MAX_DIM)
+    if not eps >= 0.0:
+        raise ValueError("eps must not be negative")
+    dim = x.shape[-1]
+    rows = x.numel() // dim
+    if y is None and (post_weight is not None or gate is not None):
+        raise ValueError("post_weight and gate need y")
+    if y is not None and y.shape != x.shape:
+        raise ValueError("y must have the shape of x")
+    groups = 1
+    if gate is not None:
+        if gate.dim() not in (1, 2) or gate.shape[-1] != dim:
+            raise ValueError("gate must be [dim] or [groups, dim]")
+        groups = 1 if gate.dim() == 1 else gate.shape[0]
+        if groups < 1 or rows % groups != 0:
+            raise ValueError("the rows must divide into the gate's groups")
+    _same_device((x, y, weight, bias, post_weight, gate))
+    return rows, dim, groups
+
+
+def block_norm(x, y=None, *, weight, bias=None, post_weight=None, gate=None, residual_scale=1.0, kind="rms", eps=1e-5, keep_stats=False):
+    """(r, h, stats) with r = x when y is None, and stats None unless kept for block_norm_backward.
+
+    x, y: [..., dim]; weight, bias, post_weight: [dim]; gate: [dim] or [groups, dim], each row of the gate for rows / groups
+    consecutive rows of x (a batch of equally long sequences: groups = batch)."""
+    rows, dim, groups = _sizes(x, y, weight, bias, post_weight, gate, kind, eps)
+    shape = x.shape
+    x = _check(x, rows * dim, "x")
+    y = None if y is None else _check(y, rows * dim, "y")
+    weight = _check(weight, dim, "weight")
+    bias = None if bias is None else _check(bias, dim, "bias")
+    post_weight = None if post_weight is None else _check(post_weight, dim, "post_weight")
+    gate = None if gate is None else _check(gate, groups * dim, "gate")
+    h = torch.empty(shape, dtype=torch.float32, device=x.device)
+    r = x if y is None else torch.empty(shape, dtype=torch.float32, device=x.device)
+    stats = torch.empty((4, rows), dtype=torch.float32, device=x.device) if keep_stats else None
+    n = _lib.BlockNorm(rows, dim, groups, KINDS[kind], residual_scale, eps, _ptr(x), _ptr(y), _ptr(weight), _ptr(bias), _ptr(post_weight),
+                       _ptr(gate), None if y is None else _ptr(r), _ptr(h), _ptr(stats))
+    with torch.cuda.device(x.device):
+        rc = _lib.lib().rgb200_block_norm_forward(C.byref(n), _stream(None))
+    if rc != cudaSuccess:
+        raise ReproGemmError(rc, "block_norm_forward")
+    return r, h, stats
+
+
+def block_norm_backward(dh, dr, r, y, stats, *, weight, bias=None, post_weight=None, gate=None, residual_scale=1.0, kind="rms", eps=1e-5,
+                        wanted=("x", "y", "weight", "bias", "post_weight", "gate")):
+    """Gradients of block_norm from dh and dr (the gradient that reaches r from the residual stream; may be None).
+    r, y, stats: what the forward call returned and took.  `wanted` names the gradients to form."""
+    rows, dim, groups = _sizes(r, y, weight, bias, post_weight, gate, kind, eps)
+    _same_device((r, dh, dr, stats))
+    shape = r.shape
+    r, dh, stats, weight = _check(r, rows * dim, "r"), _check(dh, rows * dim, "dh"), _check(stats, 4 * rows, "stats"), _check(weight, dim, "weight")
+    dr = None if dr is None else _check(dr, rows * dim, "dr")
+    y = None if y is None else _check(y, rows * dim, "y")
+    post_weight = None if post_weight is None else _check(post_weight, dim, "post_weight")
+    gate_shape = None if gate is None else gate.shape
+    gate = None if gate is None else _check(gate, groups * dim, "gate")
+
+    def out(name, given, of):
+        return torch.empty(of, dtype=torch.float32, device=r.device) if name in wanted and given else None
+
+    g = NormGrads(out("x", True, shape), out("y", y is not None, shape), out("weight", True, dim), out("bias", bias is not None, dim),
+                  out("post_weight", post_weight is not None, dim), out("gate", gate is not None, gate_shape))
+    L = _lib.lib()
+    with torch.cuda.device(r.device):
+        ws = _workspace(L.rgb200_block_norm_backward_workspace(rows, dim, groups), r.device)
+        n = _lib.BlockNorm(rows, dim, groups, KINDS[kind], residual_scale, eps, _ptr(r), _ptr(y), _ptr(weight), None, _ptr(post_weight), _ptr(gate),
+                           _ptr(r), None, _ptr(stats), _ptr(dr), _ptr(dh), _ptr(g.x), _ptr(g.y), _ptr(g.weight), _ptr(g.bias),
+                           _ptr(g.post_weight), _ptr(g.gate))
+        rc = L.rgb200_block_norm_backward(C.byref(n), _ptr(ws), ws.numel(), _stream(None))
+    if rc != cudaSuccess:
+        raise ReproGemmError(rc, "block_norm_backward")
+    return g

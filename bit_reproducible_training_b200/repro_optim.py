@@ -2,7 +2,7 @@
 
 Counterpart of the optimizer of the reference's repro_torch (Adam / AdamW over repro_nn_cuda/repro_nn.cuh:12-21), with
 the moments held in FP32 or in 8 bits.  Every value goes through the same fixed sequence of IEEE single operations
-(include/rgb200.h, rgb200_adamw_step), so the parameters' bits depend on the gradients and the hyper-parameters alone.
+(include/rgb200_train.h, rgb200_adamw_step), so the parameters' bits depend on the gradients and the hyper-parameters alone.
 CUDA float32 parameters only; there is no CPU path.
 """
 import ctypes as C

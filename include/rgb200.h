@@ -10,6 +10,9 @@
  * that is passed in (a cudaStream_t cast to void*; NULL = the default stream).  Return values are
  * cudaError_t codes as int (0 = success, 1 = cudaErrorInvalidValue, 801 = cudaErrorNotSupported).
  *
+ * The operators around the products of a training step (fused linear epilogue, block norms, linear cross entropy,
+ * AdamW) are declared in rgb200_train.h.
+ *
  * File:line citations name the interface of the reference project that each declaration stands
  * in for (paths inside that project).
  */
@@ -225,43 +228,6 @@ int rgb200_conv2d_grad_weight_ws(const float* dy, const float* x, float* dw, con
                                  void* workspace, size_t workspace_bytes, void* stream);
 int rgb200_conv2d_grad_input_ws(const float* dy, const float* weight, float* dx, const rgb200_conv_shape* shape, int slices,
                                 void* workspace, size_t workspace_bytes, void* stream);
-
-/* ------------------------------------------------------------------------------------------------
- * AdamW over many tensors in one launch, moments in FP32 or as 8-bit codes.
- * Stands beside the reference's Adam / AdamW (repro_nn_cuda/repro_nn.cuh:12-21), which takes one FP32 tensor per call.
- * Per value, every operation an IEEE single operation in this order (constants in parentheses formed in
- * double, rounded once), n the step's number counted from 1:
- *   p1 = p (1 - lr wd);  m' = m b1 + g (1 - b1);  v' = v b2 + (g g)(1 - b2)
- *   p' = p1 - (m' / (sqrt(v') (1 / sqrt(1 - b2^n)) + eps)) (lr / (1 - b1^n))
- * so the result does not depend on how tensors are cut, ordered or spread over calls, streams or GPUs.
- * 8-bit states: 256 consecutive values of a tensor share one FP32 scale (the largest magnitude of the block);
- * a first moment is an int8 code q standing for (q/127) |q/127| scale, a second moment a uint8 code standing for
- * (q/255)^4 scale, rounded to the nearest code in q, a non-zero second moment never to code 0.  A block that
- * holds a value that is not finite gets a NaN scale.
- * Asynchronous on `stream` and allocation-free.  The tensors of one call must not overlap.
- * 1 (invalid value): a null pointer with count > 0, a negative count, betas outside [0, 1), negative or NaN
- * lr / eps / weight decay, step < 1 without device_step, state_bits not 8 or 32. */
-typedef struct rgb200_adamw_tensor {
-    float* param;
-    const float* grad;
-    void* exp_avg;            /* float[count], or int8[count] codes */
-    void* exp_avg_sq;         /* float[count], or uint8[count] codes */
-    float* exp_avg_scale;     /* 8-bit states: float[ceil(count / 256)]; else ignored */
-    float* exp_avg_sq_scale;
-    long long count;
-} rgb200_adamw_tensor;
-typedef struct rgb200_adamw_hyper {
-    double lr, beta1, beta2, eps, weight_decay;
-    long long step;           /* this step's number, from 1; ignored with device_step */
-    long long* device_step;   /* or NULL: device word with the number of steps done; read, then advanced by this call
-                               * (for steps captured into a CUDA graph) */
-    int state_bits;           /* 32 or 8 */
-} rgb200_adamw_hyper;
-int rgb200_adamw_step(const rgb200_adamw_tensor* tensors, int count, const rgb200_adamw_hyper* hyper, void* stream);
-/* The values that 8-bit states stand for, written to param (first moments) and grad (second moments), and the
- * reverse: codes and scales of the values found there.  Used for checkpoints that either state width can load. */
-int rgb200_adamw_states_read(const rgb200_adamw_tensor* tensors, int count, void* stream);
-int rgb200_adamw_states_write(const rgb200_adamw_tensor* tensors, int count, void* stream);
 
 /* Host-side helpers matching repro_gemm_cuda/repro_test_util.h:20-24 (FNV-1a-64 over raw bytes) and
  * repro_gemm_cuda/repro_gemm_math.cuh:59,74,96 (the three scalar functions, computed by this

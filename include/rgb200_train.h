@@ -1,0 +1,86 @@
+/*
+ * rgb200 - C ABI of the operators around the reproducible products of a training step  (librgb200.so)
+ *
+ * Same conventions as rgb200.h: plain device pointers and sizes, all work enqueued on the stream that is passed in (a
+ * cudaStream_t cast to void*), nothing allocated, nothing kept between calls, cudaError_t codes as int
+ * (0 = success, 1 = cudaErrorInvalidValue, 801 = cudaErrorNotSupported).  Sums of floats are taken in an order that depends
+ * on the sizes alone, so the output bits depend on the inputs and the sizes, not on the stream, the call or the GPU.
+ */
+#ifndef RGB200_TRAIN_H
+#define RGB200_TRAIN_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* ------------------------------------------------------------------------------------------------
+ * AdamW over many tensors in one launch, moments in FP32 or as 8-bit codes.
+ * Stands beside the reference's Adam / AdamW (repro_nn_cuda/repro_nn.cuh:12-21), which takes one FP32 tensor per call.
+ * Per value, every operation an IEEE single operation in this order (constants in parentheses formed in
+ * double, rounded once), n the step's number counted from 1:
+ *   p1 = p (1 - lr wd);  m' = m b1 + g (1 - b1);  v' = v b2 + (g g)(1 - b2)
+ *   p' = p1 - (m' / (sqrt(v') (1 / sqrt(1 - b2^n)) + eps)) (lr / (1 - b1^n))
+ * so the result does not depend on how tensors are cut, ordered or spread over calls, streams or GPUs.
+ * 8-bit states: 256 consecutive values of a tensor share one FP32 scale (the largest magnitude of the block);
+ * a first moment is an int8 code q standing for (q/127) |q/127| scale, a second moment a uint8 code standing for
+ * (q/255)^4 scale, rounded to the nearest code in q, a non-zero second moment never to code 0.  A block that
+ * holds a value that is not finite gets a NaN scale.
+ * Asynchronous on `stream` and allocation-free.  The tensors of one call must not overlap.
+ * 1 (invalid value): a null pointer with count > 0, a negative count, betas outside [0, 1), negative or NaN
+ * lr / eps / weight decay, step < 1 without device_step, state_bits not 8 or 32. */
+typedef struct rgb200_adamw_tensor {
+    float* param;
+    const float* grad;
+    void* exp_avg;            /* float[count], or int8[count] codes */
+    void* exp_avg_sq;         /* float[count], or uint8[count] codes */
+    float* exp_avg_scale;     /* 8-bit states: float[ceil(count / 256)]; else ignored */
+    float* exp_avg_sq_scale;
+    long long count;
+} rgb200_adamw_tensor;
+typedef struct rgb200_adamw_hyper {
+    double lr, beta1, beta2, eps, weight_decay;
+    long long step;           /* this step's number, from 1; ignored with device_step */
+    long long* device_step;   /* or NULL: device word with the number of steps done; read, then advanced by this call
+                               * (for steps captured into a CUDA graph) */
+    int state_bits;           /* 32 or 8 */
+} rgb200_adamw_hyper;
+int rgb200_adamw_step(const rgb200_adamw_tensor* tensors, int count, const rgb200_adamw_hyper* hyper, void* stream);
+/* The values that 8-bit states stand for, written to param (first moments) and grad (second moments), and the
+ * reverse: codes and scales of the values found there.  Used for checkpoints that either state width can load. */
+int rgb200_adamw_states_read(const rgb200_adamw_tensor* tensors, int count, void* stream);
+int rgb200_adamw_states_write(const rgb200_adamw_tensor* tensors, int count, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * The norm behind a block, its gate, the residual stream and the norm in front of the next block (no counterpart in
+ * the reference).  All tensors FP32, rows of `dim` contiguous values:
+ *   u = post_weight * N(y)  (u = y when post_weight is NULL)      r = scale x + gate * u      h = weight * N(r) + bias
+ * and h = weight * N(x) + bias when y is NULL (r is then not written).  N subtracts the mean (layer kind) and divides by
+ * sqrt(mean of squares + eps).  gate holds `groups` rows of `dim` values, each for rows / groups consecutive rows; with
+ * groups 1 it is one value a channel.
+ * stats (float[4 * rows]; forward: may be NULL) carries the rows' means and reciprocal deviations to the backward call, which
+ * takes the gradients dr (of r from elsewhere; may be NULL) and dh, and writes those outputs that are not NULL: dx[rows, dim],
+ * dy, dweight[dim], dbias[dim], dpost_weight[dim], dgate[groups, dim].  r may be the forward call's x when y is NULL.
+ * Sums are taken in an order that depends on (rows, dim, groups) alone.  Asynchronous and allocation-free; dim at most 8192.
+ * The workspace (16-byte aligned) may be reused by any later call on the same stream.
+ * 1 (invalid value): sizes outside those limits, rows not a multiple of groups, negative or NaN eps, post_weight or gate or
+ * dy without y, gradients of absent tensors, missing tensors, a short workspace. */
+enum { RGB200_NORM_RMS = 0, RGB200_NORM_LAYER = 1 };
+typedef struct rgb200_block_norm {
+    int rows, dim, groups, kind;
+    float scale, eps;
+    const float *x, *y, *weight, *bias, *post_weight, *gate;
+    float *r, *h, *stats;
+    const float *dr, *dh;
+    float *dx, *dy, *dweight, *dbias, *dpost_weight, *dgate;
+} rgb200_block_norm;
+int rgb200_block_norm_forward(const rgb200_block_norm* norm, void* stream);
+size_t rgb200_block_norm_backward_workspace(int rows, int dim, int groups);
+int rgb200_block_norm_backward(const rgb200_block_norm* norm, void* workspace, size_t workspace_bytes, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* RGB200_TRAIN_H */

@@ -1,4 +1,4 @@
-"""The AdamW step and the 8-bit codes restated in numpy float32, operation by operation, as include/rgb200.h defines them
+"""The AdamW step and the 8-bit codes restated in numpy float32, operation by operation, as include/rgb200_train.h defines them
 (numpy rounds each float32 operation once, like the kernels)."""
 import numpy as np
 
