@@ -29,6 +29,10 @@ class AdamwHyper(C.Structure):
         ("step", C.c_longlong), ("device_step", C.c_void_p), ("state_bits", C.c_int)]
 
 
+class Epilogue(C.Structure):
+    _fields_ = [("bias", C.c_void_p), ("residual", C.c_void_p), ("pre_activation", C.c_void_p), ("activation", C.c_int)]
+
+
 class BlockNorm(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("rows", "dim", "groups", "kind")] + [("scale", C.c_float), ("eps", C.c_float)] + [
         (n, C.c_void_p) for n in ("x", "y", "weight", "bias", "post_weight", "gate", "r", "h", "stats", "dr", "dh", "dx", "dy",
@@ -92,6 +96,10 @@ def lib():
     L.rgb200_adamw_step.argtypes = [vp, i, C.POINTER(AdamwHyper), vp]
     L.rgb200_adamw_states_read.argtypes = [vp, i, vp]
     L.rgb200_adamw_states_write.argtypes = [vp, i, vp]
+    L.rgb200_gemm_epilogue_fp32_ws.argtypes = [fp, fp, fp, i, i, i, cfgp, C.POINTER(Epilogue), vp, C.c_size_t, vp]
+    L.rgb200_activation_backward_workspace.argtypes = [i, i]
+    L.rgb200_activation_backward_workspace.restype = C.c_size_t
+    L.rgb200_activation_backward.argtypes = [fp, fp, fp, fp, i, i, i, vp, C.c_size_t, vp]
     L.rgb200_block_norm_forward.argtypes = [C.POINTER(BlockNorm), vp]
     L.rgb200_block_norm_backward_workspace.argtypes = [i, i, i]
     L.rgb200_block_norm_backward_workspace.restype = C.c_size_t

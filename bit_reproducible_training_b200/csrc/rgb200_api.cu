@@ -14,6 +14,8 @@
 #include <vector>
 
 #include "../../include/rgb200.h"
+#include "rgb200_epilogue.h"
+#include "rgb200_gemm.h"
 #include "rgb200_math.cuh"
 #include "rgb200_mma.cuh"
 #include "rgb200_smallk.cuh"
@@ -458,6 +460,9 @@ struct RunArgs {
     // B's digit planes and exponents already sit in the workspace from the previous call on it with the same
     // N, K, S and transposition (row blocks of one product): skip B's pre-pass.
     bool reuse_b = false;
+    // An epilogue behind the rounding (see Epilogue); such a product takes the general kernel whatever its shape.
+    int epi = EPI_NONE;
+    const EpilogueParams* epi_params = nullptr;
 };
 
 template <int S>
@@ -476,7 +481,7 @@ cudaError_t run(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
     cudaError_t e = cudaSuccess;
     // Skinny output (N <= 64) with a k-contiguous A: A's split is fused into the MMA kernel's producer and its
     // digit planes never reach HBM (rgb200_rowfused.cuh); only B goes through the pre-pass.
-    const bool fused_a = !a.hook && !a.trans_a && !a.max_a && !part && !a.scatter && !a.c_image_rows &&
+    const bool fused_a = !a.hook && !a.epi && !a.trans_a && !a.max_a && !part && !a.scatter && !a.c_image_rows &&
                          L.algo == RGB200_ALGO_TENSORCORE && L.N <= RF_NT && L.split == 1 && L.k_blocks > 1 &&
                          L.K % 4 == 0 && (reinterpret_cast<uintptr_t>(a.A) & 15) == 0 && (L.batch == 1 || a.stride_a % 4 == 0);
     // Both operands k-contiguous (the forward product of a linear layer, C = A B^T): one launch splits both
@@ -544,7 +549,7 @@ cudaError_t run(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
 
     if (a.c_image_rows && (L.split != 1 || L.batch != 1 || part)) return cudaErrorInvalidValue;
     CUtensorMap map_a, map_b;
-    if (L.k_blocks == 1 && !part && !a.c_image_rows && !a.scatter) {
+    if (L.k_blocks == 1 && !part && !a.c_image_rows && !a.scatter && !a.epi) {
         // the whole K fits one k block (attention scores and the like): the epilogue-centred kernel
         if ((e = encode_planes_map(&map_a, qa, L.M, L.Kp, S, L.batch, BLOCK_M)) != cudaSuccess) return e;
         if ((e = encode_planes_map(&map_b, qb, L.N, L.Kp, S, L.batch, SK_NT)) != cudaSuccess) return e;
@@ -572,7 +577,7 @@ cudaError_t run(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
         record(3);
         return cudaGetLastError();
     }
-    const int tile_n = a.c_image_rows ? TILE_N_BASE : tile_n_for(S, L.N);
+    const int tile_n = a.epi ? EPI_TILE_N : a.c_image_rows ? TILE_N_BASE : tile_n_for(S, L.N);
     if ((e = encode_planes_map(&map_a, qa, L.M, L.Kp, S, L.batch, BLOCK_M)) != cudaSuccess) return e;
     if ((e = encode_planes_map(&map_b, qb, L.N, L.Kp, S, L.batch, tile_n)) != cudaSuccess) return e;
     GemmParams P;
@@ -601,7 +606,12 @@ cudaError_t run(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
     }
     const long long tiles = (long long)L.batch * L.split * P.m_tiles * P.n_tiles;
     const int grid = (int)(tiles < dev.sm_count ? tiles : dev.sm_count);
-    if (a.c_image_rows)
+    if (a.epi) P.epi = *a.epi_params;
+    if (a.epi && !part) {
+        if ((e = launch_gemm_epilogue(S, a.epi, grid, map_a, map_b, P, a.st)) != cudaSuccess) return e;
+    } else if (part && a.epi && S != 3) {              // K ranges at one or two slices: the tile width the operands were mapped for
+        gemm_i8_tcgen05_kernel<S, TILE_N_BASE><<<grid, GEMM_THREADS, GemmTraits<S, TILE_N_BASE>::SMEM_BYTES, a.st>>>(map_a, map_b, P);
+    } else if (a.c_image_rows)
         gemm_i8_tcgen05_kernel<S, TILE_N_BASE, true><<<grid, GEMM_THREADS, GemmTraits<S, TILE_N_BASE>::SMEM_BYTES, a.st>>>(map_a, map_b, P);
     else if (S == 1 && tile_n == 256)
         gemm_i8_tcgen05_kernel<1, 256><<<grid, GEMM_THREADS, GemmTraits<1, 256>::SMEM_BYTES, a.st>>>(map_a, map_b, P);
@@ -612,7 +622,9 @@ cudaError_t run(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
     record(2);
     if (L.use_partial_ws) {
         const size_t total = (size_t)L.batch * L.M * L.N;
-        launch_round(part, L.split, total, ea, eb, nullptr, nullptr, a.C, L.M, L.N, L.batch, a.stride_c, e0, dev.sm_count, a.st);
+        if (a.epi) {
+            if ((e = launch_round_epilogue(part, L.split, ea, eb, L.M, L.N, a.C, e0, *a.epi_params, dev.sm_count, a.st)) != cudaSuccess) return e;
+        } else launch_round(part, L.split, total, ea, eb, nullptr, nullptr, a.C, L.M, L.N, L.batch, a.stride_c, e0, dev.sm_count, a.st);
     }
     record(3);
     return cudaGetLastError();
@@ -626,6 +638,27 @@ cudaError_t dispatch(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
     }
     return cudaErrorInvalidValue;
 }
+
+}  // namespace
+
+// The product with an epilogue, for the entry points of rgb200_train.h (declared in rgb200_gemm.h).
+cudaError_t gemm_with_epilogue(const float* A, const float* B, float* C, int M, int N, int K, const rgb200_config& cfg, int epi,
+                               const EpilogueParams& E, bool reuse_b, void* ws, size_t ws_bytes, cudaStream_t st) {
+    Layout L;
+    cudaError_t e = plan_layout(M, N, K, K, 1, cfg, false, L, 4611686018427387904.0, epi == EPI_LINEAR);
+    if (e != cudaSuccess) return e;
+    const DeviceInfo* dev = nullptr;
+    if ((e = check_device(L.algo, &dev)) != cudaSuccess) return e;
+    if (L.algo != RGB200_ALGO_TENSORCORE || (epi != EPI_LINEAR && L.split != 1)) return cudaErrorNotSupported;
+    if (!ws || ws_bytes < L.total) return cudaErrorInvalidValue;
+    RunArgs a{A, B, C, nullptr, nullptr, nullptr, 0, 0, 0, cfg.trans_a != 0, cfg.trans_b != 0, static_cast<char*>(ws), st, nullptr};
+    a.epi = epi;
+    a.epi_params = &E;
+    a.reuse_b = reuse_b;
+    return dispatch(L, a, *dev);
+}
+
+namespace {
 
 cudaError_t gemm_ws(const float* A, const float* B, float* C, int M, int N, int K, int batch, long long sa, long long sb,
                     long long sc, const rgb200_config* cfg, void* ws, size_t ws_bytes, void* stream, void* const* events4) {

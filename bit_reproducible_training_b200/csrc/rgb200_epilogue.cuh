@@ -1,0 +1,265 @@
+// Epilogues of the tcgen05 GEMM kernel (rgb200_mma.cuh) and of the rounding kernel behind K ranges:
+//
+//   EPI_LINEAR   y = act(c + bias[col]) + residual[row][col], with c + bias stored beside it on request.
+//   EPI_LSE      per row: m = max over the tile's columns, s = sum exp(c - m); c itself is not stored.
+//   EPI_PROB     row_scale[row] * exp(c - lse[row]), zero at the row's target word.
+//
+// c is the product rounded once to FP32, as the plain entry points return it; every step after it is one FP32 operation in a
+// fixed order, so the bits do not depend on the tiling (EPI_LSE: on the tile width alone).
+//
+// Why here: an output costs 4 bytes of HBM written by the product and 8 more for every elementwise pass behind it.  In
+// the kernel the extra work of a thread (32 columns of one row) overlaps the next tile's MMAs, which take about 1150 clocks for each
+// 128 values of k; the residual and the bias are requested before the wait for the accumulators.
+#pragma once
+#include "rgb200_mma.cuh"
+
+namespace rgb200 {
+
+constexpr int ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4, ACT_COUNT = 5;
+
+// 2 sqrt(2 / pi), and that times 0.044715; gelu_tanh(z) = z / (1 + exp(-(G1 z + G3 z^3))), which is 0.5 z (1 + tanh(half of it)) without
+// the cancellation of 1 + tanh on the negative side.
+constexpr float GELU_G1 = 1.5957691216057308f, GELU_G3 = 0.0713548162726009f;
+constexpr float SQRT_HALF = 0.7071067811865476f, INV_SQRT_2PI = 0.3989422804014327f;
+
+template <int ACT>
+__device__ __forceinline__ float activation(float z) {
+    if (ACT == ACT_RELU) return z <= 0.0f ? 0.0f : z;
+    if (ACT == ACT_SILU) return z / (1.0f + expf(-z));
+    if (ACT == ACT_GELU) return 0.5f * z * (1.0f + erff(z * SQRT_HALF));
+    if (ACT == ACT_GELU_TANH) return z / (1.0f + expf(-z * (GELU_G1 + GELU_G3 * (z * z))));
+    return z;
+}
+
+// Derivative of the activation.  Where exp overflows the sigmoid is 0 and the products with z stay finite for finite z below 1e12.
+template <int ACT>
+__device__ __forceinline__ float activation_slope(float z) {
+    if (ACT == ACT_RELU) return z <= 0.0f ? 0.0f : 1.0f;
+    if (ACT == ACT_SILU) {
+        const float p = 1.0f / (1.0f + expf(-z));
+        return p * (1.0f + z * (1.0f - p));
+    }
+    if (ACT == ACT_GELU) return 0.5f * (1.0f + erff(z * SQRT_HALF)) + z * (expf(-0.5f * (z * z)) * INV_SQRT_2PI);
+    if (ACT == ACT_GELU_TANH) {
+        const float q = z * z, p = 1.0f / (1.0f + expf(-z * (GELU_G1 + GELU_G3 * q)));
+        return p + (p * (1.0f - p)) * (z * (GELU_G1 + 3.0f * GELU_G3 * q));
+    }
+    return 1.0f;
+}
+
+// Runs f with the activation as a compile-time constant: one uniform branch instead of one per value.
+template <class F>
+__device__ __forceinline__ void with_activation(int act, F f) {
+    switch (act) {
+        case ACT_RELU: f(std::integral_constant<int, ACT_RELU>()); break;
+        case ACT_SILU: f(std::integral_constant<int, ACT_SILU>()); break;
+        case ACT_GELU: f(std::integral_constant<int, ACT_GELU>()); break;
+        case ACT_GELU_TANH: f(std::integral_constant<int, ACT_GELU_TANH>()); break;
+        default: f(std::integral_constant<int, ACT_NONE>()); break;
+    }
+}
+
+__device__ __forceinline__ void ld_global_256(const float* p, float (&v)[8]) {
+    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void st_global_256(float* p, const float (&v)[8]) {
+    st_global_256(reinterpret_cast<uint32_t*>(p), __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]),
+                  __float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+}
+
+template <int CPT>
+struct EpilogueRow<EPI_LINEAR, CPT> {
+    float res[CPT];
+    bool sectors;               // the thread's columns are whole 32-byte sectors of C, residual and pre
+
+    __device__ __forceinline__ void request(const GemmParams& P, int row, bool row_ok, int col0, float* slot, int lane) {
+        for (int c = lane; c < CPT; c += 32) slot[c] = P.epi.bias && col0 + c < P.N ? __ldg(P.epi.bias + col0 + c) : 0.0f;
+        const size_t at = (size_t)row * P.N + col0;
+        const uintptr_t bits = reinterpret_cast<uintptr_t>(P.C + at) | (P.epi.residual ? reinterpret_cast<uintptr_t>(P.epi.residual + at) : 0) |
+                               (P.epi.pre ? reinterpret_cast<uintptr_t>(P.epi.pre + at) : 0);
+        sectors = (bits & 31) == 0 && col0 + CPT <= P.N;
+        if (!row_ok || !P.epi.residual) return;
+        if (sectors) {
+#pragma unroll
+            for (int j = 0; j < CPT; j += 8) {
+                float v[8];
+                ld_global_256(P.epi.residual + at + j, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) res[j + i] = v[i];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < CPT; ++j) res[j] = col0 + j < P.N ? P.epi.residual[at + j] : 0.0f;
+        }
+    }
+
+    template <class Value>
+    __device__ __forceinline__ void finish(const GemmParams& P, int row, int col0, int, const float* slot, Value value) {
+        const size_t at = (size_t)row * P.N + col0;
+        with_activation(P.epi.act, [&](auto act) {
+#pragma unroll
+            for (int j = 0; j < CPT; j += 8) {
+                float z[8], y[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    z[i] = value(j + i);
+                    if (P.epi.bias) z[i] += slot[j + i];
+                    y[i] = activation<decltype(act)::value>(z[i]);
+                    if (P.epi.residual) y[i] += res[j + i];
+                }
+                if (sectors) {
+                    if (P.epi.pre) st_global_256(P.epi.pre + at + j, z);
+                    st_global_256(P.C + at + j, y);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (col0 + j + i >= P.N) break;
+                        if (P.epi.pre) P.epi.pre[at + j + i] = z[i];
+                        P.C[at + j + i] = y[i];
+                    }
+                }
+            }
+        });
+    }
+};
+
+// The same on values that a K-range product left as INT64 sums: see round_partial_kernel.  Four neighbours per thread when
+// VEC, which the host sets from N and the addresses.
+template <bool VEC>
+static __global__ void __launch_bounds__(256)
+round_partial_linear_kernel(const long long* __restrict__ partial, int parts, const int* __restrict__ ea, const int* __restrict__ eb, int M, int N,
+                            float* C, int e0, const EpilogueParams E) {
+    constexpr int W = VEC ? 4 : 1;
+    const size_t total = (size_t)M * N;
+    with_activation(E.act, [&](auto act) {
+        for (size_t idx = ((size_t)blockIdx.x * blockDim.x + threadIdx.x) * W; idx < total; idx += (size_t)gridDim.x * blockDim.x * W) {
+            long long t[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) t[j] = 0;
+            for (int p = 0; p < parts; ++p) {
+#pragma unroll
+                for (int j = 0; j < W; ++j) t[j] += partial[(size_t)p * total + idx + j];
+            }
+            const int r = (int)(idx / N), c = (int)(idx - (size_t)r * N);
+            const int e_r = ea[r] + e0;
+            float z[W], y[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                z[j] = bits_f32(round_to_f32_bits(t[j], e_r + eb[c + j]));
+                if (E.bias) z[j] += E.bias[c + j];
+                y[j] = activation<decltype(act)::value>(z[j]);
+            }
+            if (VEC) {
+                if (E.residual) {
+                    const float4 q = *reinterpret_cast<const float4*>(E.residual + idx);
+                    y[0] += q.x; y[W > 1 ? 1 : 0] += q.y; y[W > 2 ? 2 : 0] += q.z; y[W > 3 ? 3 : 0] += q.w;
+                }
+                if (E.pre) *reinterpret_cast<float4*>(E.pre + idx) = make_float4(z[0], z[W > 1 ? 1 : 0], z[W > 2 ? 2 : 0], z[W > 3 ? 3 : 0]);
+                *reinterpret_cast<float4*>(C + idx) = make_float4(y[0], y[W > 1 ? 1 : 0], y[W > 2 ? 2 : 0], y[W > 3 ? 3 : 0]);
+            } else {
+                if (E.residual) y[0] += E.residual[idx];
+                if (E.pre) E.pre[idx] = z[0];
+                C[idx] = y[0];
+            }
+        }
+    });
+}
+
+// ------------------------------------------------------------------------------------------
+// Backward of the epilogue: dZ = dY * act'(Z) and the bias gradient db = column sums of dZ, one pass (HBM: 12 bytes a value, 4 when
+// there is no activation and only db is formed).  A CTA owns 128 columns of a range of rows; each of its eight warps adds
+// every eighth row of the range in order, then the warps' sums and last the ranges' are added in order: an order that depends on
+// (M, N) alone.  Lane columns: neighbours in quads when N % 4 == 0 (an unaligned base only changes how they are loaded).
+// ------------------------------------------------------------------------------------------
+constexpr int ACTB_COLS = 128, ACTB_WARPS = 8;
+
+struct ActBackwardParams {
+    const float *dy, *z;
+    float *dz;                  // null: only the column sums
+    float *parts;               // [ranges][N], or null without a bias gradient
+    int M, N, act, rows_per_range, wide;
+};
+
+template <int V>
+static __global__ void __launch_bounds__(32 * ACTB_WARPS)
+activation_backward_kernel(const ActBackwardParams P) {
+    __shared__ float sums[ACTB_WARPS][ACTB_COLS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int first = blockIdx.y * P.rows_per_range;
+    const int end = P.M - first < P.rows_per_range ? P.M : first + P.rows_per_range;
+    int col[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) col[j] = blockIdx.x * ACTB_COLS + (V == 4 ? lane * 4 + j : j * 32 + lane);
+    const bool wide = V == 4 && P.wide;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    with_activation(P.act, [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
+#pragma unroll 4
+        for (int row = first + warp; row < end; row += ACTB_WARPS) {
+            const size_t at = (size_t)row * P.N;
+            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f}, z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (wide) {
+                if (col[0] < P.N) {
+                    const float4 q = *reinterpret_cast<const float4*>(P.dy + at + col[0]);
+                    d[0] = q.x; d[1] = q.y; d[2] = q.z; d[3] = q.w;
+                    if (ACT != ACT_NONE) {
+                        const float4 t = *reinterpret_cast<const float4*>(P.z + at + col[0]);
+                        z[0] = t.x; z[1] = t.y; z[2] = t.z; z[3] = t.w;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (col[j] < P.N) {
+                        d[j] = P.dy[at + col[j]];
+                        if (ACT != ACT_NONE) z[j] = P.z[at + col[j]];
+                    }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (ACT != ACT_NONE) d[j] = d[j] * activation_slope<ACT>(z[j]);
+                s[j] += d[j];
+            }
+            if (P.dz) {
+                if (wide) {
+                    if (col[0] < P.N) *reinterpret_cast<float4*>(P.dz + at + col[0]) = make_float4(d[0], d[1], d[2], d[3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (col[j] < P.N) P.dz[at + col[j]] = d[j];
+                }
+            }
+        }
+    });
+    if (!P.parts) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums[warp][col[j] - blockIdx.x * ACTB_COLS] = s[j];
+    __syncthreads();
+    const int c = threadIdx.x, out = blockIdx.x * ACTB_COLS + c;
+    if (c < ACTB_COLS && out < P.N) {
+        float t = sums[0][c];
+#pragma unroll
+        for (int k = 1; k < ACTB_WARPS; ++k) t += sums[k][c];
+        P.parts[(size_t)blockIdx.y * P.N + out] = t;
+    }
+}
+
+// Column sums of the ranges' sums, [ranges][N] -> [N]: a CTA owns 32 columns, warp k adds ranges k, k + 8, ... in order, then the warps' sums.
+static __global__ void __launch_bounds__(256)
+range_sums_kernel(const float* __restrict__ parts, int ranges, int N, float* __restrict__ out) {
+    __shared__ float sums[8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+    float s = 0.0f;
+    if (col < N) {
+#pragma unroll 4
+        for (int i = warp; i < ranges; i += 8) s += parts[(size_t)i * N + col];
+    }
+    sums[warp][lane] = s;
+    __syncthreads();
+    if (warp != 0 || col >= N) return;
+    for (int k = 1; k < 8; ++k) s += sums[k][lane];
+    out[col] = s;
+}
+
+}  // namespace rgb200

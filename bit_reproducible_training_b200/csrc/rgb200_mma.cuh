@@ -74,6 +74,27 @@ struct GemmTraits {
     static_assert(STAGES >= 2, "pipeline needs two stages");
 };
 
+// What happens to a rounded output before it is stored, in the kernels built with one of these (rgb200_epilogue.cuh).
+enum Epilogue : int {
+    EPI_NONE = 0,
+    EPI_LINEAR = 1,     // bias, activation, residual
+    EPI_LSE = 2,        // nothing is stored but each row's maximum and sum of exponentials over the tile's columns
+    EPI_PROB = 3        // softmax probabilities from the rows' log-sum-exp, scaled by row, zero at the row's target
+};
+struct EpilogueParams {
+    const float* bias;          // [N] or null
+    const float* residual;      // [M][N] or null; may be C itself
+    float* pre;                 // [M][N] or null: receives the values in front of the activation
+    int act;                    // RGB200_ACT_*
+    // cross entropy: columns are words first_word .. first_word + N - 1 of the vocabulary
+    const long long* target;    // [M]
+    long long first_word;
+    float2* lse_parts;          // [2 * n_tiles][M]: maximum, sum of exp(value - maximum)
+    float* target_logit;        // [M]
+    const float* lse;           // [M]
+    const float* row_scale;     // [M]
+};
+
 struct GemmParams {
     const int* expo_a;       // [batch][M]
     const int* expo_b;       // [batch][N]
@@ -103,6 +124,7 @@ struct GemmParams {
     // layouts of a convolution's results.  A warp's 32 rows are consecutive places, so each column is one
     // 128-byte store.  0 in the row-major kernels.
     int c_image_rows;
+    EpilogueParams epi;      // kernels with an epilogue only
 };
 
 // ------------------------------------------------------------------------------------------
@@ -327,9 +349,15 @@ __device__ __forceinline__ void cursor_next(KCursor& c, const GemmParams& P, lon
     if (c.valid) { c.tc = tile_coord(P, c.tile); c.kb = c.tc.kb_begin; }
 }
 
+// One thread's columns of the finished tile through an epilogue; defined in rgb200_epilogue.cuh, which only the
+// translation unit that builds those kernels includes.
+template <int EPI, int CPT>
+struct EpilogueRow;
+
 // IMAGE_MAJOR_C (the convolutions): the rows of the product are (image, place) pairs and C is stored
 // [image][column][place], see GemmParams::c_image_rows; only the FP32 store of the epilogue differs.
-template <int S, int NT, bool IMAGE_MAJOR_C = false>
+// EPI: see Epilogue; the kernels with one have no INT64 output.
+template <int S, int NT, bool IMAGE_MAJOR_C = false, int EPI = EPI_NONE>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
 gemm_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                        const GemmParams P) {
@@ -348,6 +376,8 @@ gemm_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(gen_base + STAGES * Tr::STAGE_BYTES + 8 * (2 * STAGES + 2));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + STAGES * Tr::STAGE_BYTES + 8 * (2 * STAGES + 3));
     int* eb_slots = reinterpret_cast<int*>(gen_base + STAGES * Tr::STAGE_BYTES + 256);
+    // kernels with an epilogue: as many floats again behind them, one slot of per-column values per epilogue warp
+    [[maybe_unused]] float* col_slots = reinterpret_cast<float*>(eb_slots + EPI_WARPS * (NT / 2));
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long total_tiles = (long long)P.batch * P.split * P.m_tiles * P.n_tiles;
@@ -455,6 +485,9 @@ gemm_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             if (!P.partial)
                 for (int c = lane; c < CPT; c += 32)
                     eb_s[c] = col0 + c < P.N ? __ldg(P.expo_b + (size_t)tc.batch * P.N + col0 + c) : 0;
+            // an epilogue's own operands are requested here too, so that they arrive during the wait
+            typename std::conditional<EPI == EPI_NONE, int, EpilogueRow<EPI, CPT>>::type epi_row;
+            if constexpr (EPI != EPI_NONE) epi_row.request(P, row, row_ok, col0, col_slots + (warp - 2) * CPT, lane);
             __syncwarp();
             ok = mbar_wait(tmem_full_bar, tile_it & 1u, abort_flag, P.status, STATUS_WAIT_TMEM_FULL);
             ok = __all_sync(0xFFFFFFFFu, ok);
@@ -481,6 +514,16 @@ gemm_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             tc_fence_before();
             mbar_arrive(tmem_empty_bar);
             // phase 2: one rounding per output (or the raw sums), overlapped with the next tile's MMAs
+            if constexpr (EPI != EPI_NONE) {
+                if (!row_ok || col0 >= P.N) continue;
+                epi_row.finish(P, row, col0, tc.n_blk * 2 + half, col_slots + (warp - 2) * CPT, [&](int j) {
+                    const int e = ea + P.e0 + eb_s[j];
+                    bool normal;
+                    const uint32_t b = round_to_f32_bits_signed(T[j], e, &normal);
+                    return __uint_as_float(normal ? b : round_to_f32_bits(T[j], e));
+                });
+                continue;
+            }
             if (!P.scatter_rows && (!row_ok || col0 >= P.N)) continue;
             if (P.partial) {
                 long long* dst = P.partial + (((size_t)tc.z * P.batch + tc.batch) * P.M + row) * P.N + col0;

@@ -67,6 +67,73 @@ class Linear(torch.nn.Linear):
         return _LinearFn.apply(x.contiguous(), self.weight, self.bias)
 
 
+class _FusedLinearFn(torch.autograd.Function):
+    """act(X W^T + b) + R with bias, activation and residual in the product's epilogue; backward forms dZ = dY act'(Z) and
+    db in one pass, then dX and dW through the reproducible product."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        m, k, n = x.numel() // x.shape[-1], weight.shape[1], weight.shape[0]
+        keep = activation is not None and any(ctx.needs_input_grad[:3])
+        out = rg.gemm_epilogue(x, weight, m, n, k, False, True, _slices, bias, activation, residual, keep)
+        y, z = out if keep else (out, None)
+        ctx.save_for_backward(x, weight, z)
+        ctx.activation, ctx.slices = activation, _slices
+        return y.view(*x.shape[:-1], n)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, z = ctx.saved_tensors
+        k, n = weight.shape[1], weight.shape[0]
+        m = x.numel() // k
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        dx = dw = dz = db = None
+        if need_x or need_w or need_b:
+            dz, db = rg.activation_backward(dy, z, m, n, ctx.activation, need_x or need_w, need_b)
+        if need_x:
+            dx = rg.gemm(dz, weight, m, k, n, False, False, ctx.slices).view(x.shape)
+        if need_w:
+            dw = rg.gemm(dz, x, n, k, m, True, False, ctx.slices)
+        return dx, dw, db, (dy if need_r else None), None
+
+
+def linear(x, weight, bias=None, activation=None, residual=None):
+    """act(x @ weight.T + bias) + residual in one reproducible product, differentiable in every tensor.
+
+    x [..., in], weight [out, in], bias [out], residual [..., out]; activation None, "relu", "silu", "gelu" (erf) or
+    "gelu_tanh".  The bias gradient is summed in an order that depends on the sizes alone (no set_bias_grad is needed)."""
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError("x must be [..., in] and weight [out, in]")
+    k, n = weight.shape[1], weight.shape[0]
+    if bias is not None and bias.shape != (n,):
+        raise ValueError("bias must be [%d]" % n)
+    shape = (*x.shape[:-1], n)
+    if residual is not None and residual.shape != shape:
+        raise ValueError("residual must have the output's shape")
+    if min(k, n) == 0:
+        raise ValueError("weight must not be empty")
+    rg._activation(activation)
+    if x.numel() == 0:                                   # no tokens: nothing to launch, gradients of zeros
+        return torch.nn.functional.linear(x, weight, bias) + (0 if residual is None else residual)
+    tensors = (x, weight, bias, residual)
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+        return rg.gemm_epilogue(x, weight, x.numel() // k, n, k, False, True, _slices, bias, activation, residual).view(shape)
+    return _FusedLinearFn.apply(*tensors, activation)
+
+
+class FusedLinear(torch.nn.Linear):
+    """torch.nn.Linear followed by an activation and, with forward's `residual`, an addition, as one reproducible product."""
+
+    def __init__(self, in_features, out_features, bias=True, activation=None, **kw):
+        super().__init__(in_features, out_features, bias, **kw)
+        rg._activation(activation)
+        self.activation = activation
+
+    def forward(self, x, residual=None):
+        return linear(x, self.weight, self.bias, self.activation, residual)
+
+
 class _ConvFn(torch.autograd.Function):
     """Y = conv(x, W), dX and dW through the three reproducible calls (layers.py:103-126 in the reference)."""
 

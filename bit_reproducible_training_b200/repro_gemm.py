@@ -218,6 +218,73 @@ def gemm(A, B, M, N, K, trans_a=False, trans_b=False, slices=3, split_k=1, algo=
     return out
 
 
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
+
+def _activation(name):
+    if name not in ACTIVATIONS:
+        raise ValueError("activation must be one of %s" % ", ".join(str(k) for k in ACTIVATIONS))
+    return ACTIVATIONS[name]
+
+
+def gemm_epilogue(A, B, M, N, K, trans_a=False, trans_b=False, slices=3, bias=None, activation=None, residual=None, keep_pre=False,
+                  out=None):
+    """act(op(A) op(B) + bias) + residual as a new [M, N] tensor; with keep_pre also op(A) op(B) + bias.
+
+    The product is the one ``gemm`` returns, bit for bit; bias [N], activation and residual [M, N] are applied in the kernel's
+    epilogue, one FP32 operation each.  out: a contiguous [M, N] tensor to write (it may be the residual)."""
+    A = _check(A, M * K, "A")
+    B = _check(B, K * N, "B")
+    bias = None if bias is None else _check(bias, N, "bias")
+    residual = None if residual is None else _check(residual, M * N, "residual")
+    if any(t is not None and t.device != A.device for t in (B, bias, residual, out)):
+        raise ValueError("all tensors must be on one device")
+    if out is not None and (out.dtype != torch.float32 or out.numel() != M * N or not out.is_contiguous()):
+        raise ValueError("out must be a contiguous float32 tensor of %d elements" % (M * N))
+    act = _activation(activation)
+    cfg = Config(slices=slices, trans_a=trans_a, trans_b=trans_b)
+    rc, plan = make_plan(M, N, K, cfg)
+    if rc != cudaSuccess:
+        raise ReproGemmError(rc, "make_plan")
+    with torch.cuda.device(A.device):
+        ws = _workspace(plan.workspace_bytes, A.device)
+        if out is None:
+            out = torch.empty((M, N), dtype=torch.float32, device=A.device)
+        pre = torch.empty((M, N), dtype=torch.float32, device=A.device) if keep_pre else None
+        e = _lib.Epilogue(_ptr(bias), _ptr(residual), _ptr(pre), act)
+        c = cfg.c()
+        rc = _lib.lib().rgb200_gemm_epilogue_fp32_ws(_ptr(A), _ptr(B), _ptr(out), M, N, K, C.byref(c), C.byref(e), _ptr(ws), ws.numel(),
+                                                     _stream(None))
+    if rc != cudaSuccess:
+        raise ReproGemmError(rc, "gemm_epilogue_fp32_ws")
+    _raise_if_incomplete(ws, "gemm_epilogue")
+    return (out, pre) if keep_pre else out
+
+
+def activation_backward(dY, Z, M, N, activation=None, want_dz=True, want_db=False):
+    """(dZ, db): dZ = dY * act'(Z) as [M, N] and db = column sums of dZ, summed in an order that depends on (M, N) alone.
+    Without an activation dZ is dY itself and Z is not needed."""
+    act = _activation(activation)
+    dY = _check(dY, M * N, "dY")
+    if act and Z is None:
+        raise ValueError("the activation's gradient needs Z")
+    Z = _check(Z, M * N, "Z") if act else None
+    if Z is not None and Z.device != dY.device:
+        raise ValueError("all tensors must be on one device")
+    dZ = dY if not act else torch.empty((M, N), dtype=torch.float32, device=dY.device) if want_dz else None
+    db = torch.empty(N, dtype=torch.float32, device=dY.device) if want_db else None
+    if not act and not want_db or not (want_dz or want_db):
+        return (dZ.view(M, N) if want_dz else None), None
+    L = _lib.lib()
+    with torch.cuda.device(dY.device):
+        ws = _workspace(L.rgb200_activation_backward_workspace(M, N), dY.device) if want_db else None
+        rc = L.rgb200_activation_backward(_ptr(dY), _ptr(Z), _ptr(dZ) if act else None, _ptr(db), M, N, act, _ptr(ws),
+                                          0 if ws is None else ws.numel(), _stream(None))
+    if rc != cudaSuccess:
+        raise ReproGemmError(rc, "activation_backward")
+    return (dZ.view(M, N) if want_dz else None), db
+
+
 def gemm_batched(A, B, batch, M, N, K, trans_a=False, trans_b=False, slices=3):
     """`batch` independent products of densely stacked matrices: A [batch, M*K], B [batch, K*N]."""
     A = _check(A, batch * M * K, "A")

@@ -12,9 +12,34 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "rgb200.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
+
+/* ------------------------------------------------------------------------------------------------
+ * Product with bias, activation and residual in its epilogue:
+ *   Z = op(A) op(B) + bias,   C = act(Z) + residual
+ * op(A) op(B) is the product of rgb200_gemm_fp32_ws bit for bit; each step behind it is one FP32 operation per value.
+ * The reference's Linear adds its bias in a separate pass (repro_torch/repro_torch/layers.py:70-93).
+ * bias [N], residual [M, N] (may be C itself) and pre_activation [M, N] (receives Z) may be NULL.  Activations: gelu is
+ * z/2 (1 + erf(z / sqrt 2)), gelu_tanh z/2 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))), silu z / (1 + exp(-z)).
+ * Plan and workspace are those of rgb200_make_plan.  1: as rgb200_gemm_fp32_ws, or an unknown activation; 801: RGB200_ALGO_REFERENCE.
+ * rgb200_activation_backward: dZ = dY act'(Z) (dZ may be NULL, or dY itself) and db = column sums of dZ (may be NULL; the
+ * workspace, of rgb200_activation_backward_workspace bytes, is needed for db alone).  Z may be NULL without an activation. */
+enum { RGB200_ACT_NONE = 0, RGB200_ACT_RELU = 1, RGB200_ACT_SILU = 2, RGB200_ACT_GELU = 3, RGB200_ACT_GELU_TANH = 4 };
+typedef struct rgb200_epilogue {
+    const float* bias;
+    const float* residual;
+    float* pre_activation;
+    int activation;
+} rgb200_epilogue;
+int rgb200_gemm_epilogue_fp32_ws(const float* A, const float* B, float* C, int M, int N, int K, const rgb200_config* cfg,
+                                 const rgb200_epilogue* epilogue, void* workspace, size_t workspace_bytes, void* stream);
+size_t rgb200_activation_backward_workspace(int M, int N);
+int rgb200_activation_backward(const float* dY, const float* Z, float* dZ, float* db, int M, int N, int activation, void* workspace,
+                               size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * AdamW over many tensors in one launch, moments in FP32 or as 8-bit codes.
