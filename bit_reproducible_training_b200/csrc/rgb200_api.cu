@@ -461,6 +461,7 @@ struct RunArgs {
     // N, K, S and transposition (row blocks of one product): skip B's pre-pass.
     bool reuse_b = false;
     // An epilogue behind the rounding (see Epilogue); such a product takes the general kernel whatever its shape.
+    bool reuse_a = false;      // the same for op(A), with the same M, N, K, S (both operands k-contiguous)
     int epi = EPI_NONE;
     const EpilogueParams* epi_params = nullptr;
 };
@@ -526,7 +527,9 @@ cudaError_t run(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
         record(0);
         const KmajorOperand opa{a.A, a.max_a, qa, ea, L.M, a.stride_a};
         const KmajorOperand opb{a.B, a.max_b, qb, eb, L.N, a.stride_b};
-        launch_kmajor<S>(opa, opb, L.K, L.Kp, L.batch, status, a.st);
+        const KmajorOperand none{nullptr, nullptr, nullptr, nullptr, 0, 0};
+        if (a.reuse_a) launch_kmajor<S>(opb, none, L.K, L.Kp, L.batch, status, a.st);
+        else launch_kmajor<S>(opa, opb, L.K, L.Kp, L.batch, status, a.st);
         record(1);
     } else {
         if ((e = cudaMemsetAsync(a.ws, 0, L.zero_b_bytes, a.st)) != cudaSuccess) return e;   // status word + column maxima of B
@@ -643,17 +646,19 @@ cudaError_t dispatch(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
 
 // The product with an epilogue, for the entry points of rgb200_train.h (declared in rgb200_gemm.h).
 cudaError_t gemm_with_epilogue(const float* A, const float* B, float* C, int M, int N, int K, const rgb200_config& cfg, int epi,
-                               const EpilogueParams& E, bool reuse_b, void* ws, size_t ws_bytes, cudaStream_t st) {
+                               const EpilogueParams& E, bool reuse_a, bool reuse_b, void* ws, size_t ws_bytes, cudaStream_t st) {
     Layout L;
-    cudaError_t e = plan_layout(M, N, K, K, 1, cfg, false, L, 4611686018427387904.0, epi == EPI_LINEAR);
+    const bool any_ranges = epi == EPI_NONE || epi == EPI_LINEAR;
+    cudaError_t e = plan_layout(M, N, K, K, 1, cfg, false, L, 4611686018427387904.0, any_ranges);
     if (e != cudaSuccess) return e;
     const DeviceInfo* dev = nullptr;
     if ((e = check_device(L.algo, &dev)) != cudaSuccess) return e;
-    if (L.algo != RGB200_ALGO_TENSORCORE || (epi != EPI_LINEAR && L.split != 1)) return cudaErrorNotSupported;
+    if (L.algo != RGB200_ALGO_TENSORCORE || (!any_ranges && L.split != 1)) return cudaErrorNotSupported;
     if (!ws || ws_bytes < L.total) return cudaErrorInvalidValue;
     RunArgs a{A, B, C, nullptr, nullptr, nullptr, 0, 0, 0, cfg.trans_a != 0, cfg.trans_b != 0, static_cast<char*>(ws), st, nullptr};
     a.epi = epi;
     a.epi_params = &E;
+    a.reuse_a = reuse_a;
     a.reuse_b = reuse_b;
     return dispatch(L, a, *dev);
 }

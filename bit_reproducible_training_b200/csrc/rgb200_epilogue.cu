@@ -53,6 +53,8 @@ int backward_ranges(int M, int N) {
 
 cudaError_t launch_gemm_epilogue(int slices, int epi, int grid, const CUtensorMap& a, const CUtensorMap& b, const GemmParams& P, cudaStream_t st) {
     if (epi == EPI_LINEAR) return launch_slices<EPI_LINEAR>(slices, grid, a, b, P, st);
+    if (epi == EPI_LSE) return launch_slices<EPI_LSE>(slices, grid, a, b, P, st);
+    if (epi == EPI_PROB) return launch_slices<EPI_PROB>(slices, grid, a, b, P, st);
     return cudaErrorInvalidValue;
 }
 
@@ -76,7 +78,7 @@ extern "C" int rgb200_gemm_epilogue_fp32_ws(const float* A, const float* B, floa
     if (!A || !B || !C || !cfg || !epilogue || epilogue->activation < 0 || epilogue->activation >= ACT_COUNT) return cudaErrorInvalidValue;
     EpilogueParams E = {};
     E.bias = epilogue->bias; E.residual = epilogue->residual; E.pre = epilogue->pre_activation; E.act = epilogue->activation;
-    return gemm_with_epilogue(A, B, C, M, N, K, *cfg, EPI_LINEAR, E, false, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+    return gemm_with_epilogue(A, B, C, M, N, K, *cfg, EPI_LINEAR, E, false, false, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t rgb200_activation_backward_workspace(int M, int N) {

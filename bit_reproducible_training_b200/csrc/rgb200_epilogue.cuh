@@ -124,6 +124,67 @@ struct EpilogueRow<EPI_LINEAR, CPT> {
     }
 };
 
+// Column of the row's target among the thread's columns, or a value outside 0 .. CPT - 1.
+__device__ __forceinline__ int target_column(const GemmParams& P, int row, int col0) {
+    const long long t = P.epi.target[row] - P.epi.first_word - col0;
+    return t < 0 || t > 0x7FFFFFFF ? -1 : (int)t;
+}
+
+template <int CPT>
+struct EpilogueRow<EPI_LSE, CPT> {
+    int target;
+
+    __device__ __forceinline__ void request(const GemmParams& P, int row, bool row_ok, int col0, float*, int) {
+        target = row_ok ? target_column(P, row, col0) : -1;
+    }
+
+    template <class Value>
+    __device__ __forceinline__ void finish(const GemmParams& P, int row, int col0, int part, const float*, Value value) {
+        float v[CPT], top = -INFINITY, sum = 0.0f, hit = 0.0f;
+#pragma unroll
+        for (int j = 0; j < CPT; ++j) {
+            v[j] = col0 + j < P.N ? value(j) : -INFINITY;          // the first column is always inside, so top is finite
+            top = fmaxf(top, v[j]);
+            if (j == target) hit = v[j];
+        }
+#pragma unroll
+        for (int j = 0; j < CPT; ++j) sum += expf(v[j] - top);
+        P.epi.lse_parts[(size_t)part * P.M + row] = make_float2(top, sum);
+        if (target >= 0 && target < CPT && col0 + target < P.N) P.epi.target_logit[row] = hit;
+    }
+};
+
+template <int CPT>
+struct EpilogueRow<EPI_PROB, CPT> {
+    int target;
+    float lse, scale;
+
+    __device__ __forceinline__ void request(const GemmParams& P, int row, bool row_ok, int col0, float*, int) {
+        target = row_ok ? target_column(P, row, col0) : -1;
+        lse = row_ok ? __ldg(P.epi.lse + row) : 0.0f;
+        scale = row_ok ? __ldg(P.epi.row_scale + row) : 0.0f;
+    }
+
+    template <class Value>
+    __device__ __forceinline__ void finish(const GemmParams& P, int row, int col0, int, const float*, Value value) {
+        float* dst = P.C + (size_t)row * P.N + col0;
+        const bool sectors = (reinterpret_cast<uintptr_t>(dst) & 31) == 0 && col0 + CPT <= P.N;
+#pragma unroll
+        for (int j = 0; j < CPT; j += 8) {
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)            // a row without a weight takes no part, whatever its logits are
+                p[i] = j + i == target || scale == 0.0f ? 0.0f : expf(value(j + i) - lse) * scale;
+            if (sectors) st_global_256(dst + j, p);
+            else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (col0 + j + i < P.N) dst[j + i] = p[i];
+            }
+        }
+    }
+};
+
 // The same on values that a K-range product left as INT64 sums: see round_partial_kernel.  Four neighbours per thread when
 // VEC, which the host sets from N and the addresses.
 template <bool VEC>

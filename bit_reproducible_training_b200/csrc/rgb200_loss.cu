@@ -1,0 +1,194 @@
+// Cross entropy of logits X W^T against targets in pieces of the vocabulary, without the logits (include/rgb200_train.h).
+//
+// Forward, for each piece of words: the product X W_piece^T runs with an epilogue that keeps, of each row and each 32 columns, the
+// maximum and the sum of exponentials (8 bytes instead of 128), and the target's logit; a small kernel joins them into the
+// rows' running statistics.  Backward, for each piece: the product again, now leaving P = g softmax without the targets' own
+// entries in FP32 (one piece at a time), then dX += P W_piece (the running dX is the epilogue's residual) and
+// dW_piece = P^T X.  The targets' entries (p - 1) g are kept apart: beside them the rest of a row is small, and in one matrix
+// with them it would lose its low digits to their scale.  They enter as dX's start and as additions to dW at the end.
+//
+// Work: 4 products of 2 N V D operations (one more than with stored logits), each at the rate of the library's products; what is
+// moved beside them is a few passes over one piece of P.
+#include <cstdint>
+
+#include "../../include/rgb200_train.h"
+#include "rgb200_epilogue.h"
+#include "rgb200_gemm.h"
+#include "rgb200_host.h"
+#include "rgb200_loss.cuh"
+#include "rgb200_mma.cuh"
+
+namespace rgb200 {
+namespace {
+
+constexpr size_t XENT_ALIGN = 256;
+size_t round_up(size_t x) { return (x + XENT_ALIGN - 1) / XENT_ALIGN * XENT_ALIGN; }
+
+rgb200_config product_config(int slices, bool ta, bool tb) {
+    rgb200_config c;
+    rgb200_default_config(&c);
+    c.slices = slices; c.trans_a = ta; c.trans_b = tb;
+    return c;
+}
+
+bool product_bytes(int M, int N, int K, int slices, bool ta, bool tb, size_t* bytes) {
+    const rgb200_config c = product_config(slices, ta, tb);
+    rgb200_layout_info info;
+    if (rgb200_layout(M, N, K, 1, &c, &info) != cudaSuccess) return false;
+    *bytes = round_up(info.workspace_bytes);
+    return true;
+}
+
+// Words per piece: near-equal multiples of 64 no wider than `limit`.
+int piece_words(int vocab, int limit) {
+    const int pieces = (vocab + limit - 1) / limit;
+    const int w = ((vocab + pieces - 1) / pieces + 63) / 64 * 64;
+    return w < vocab ? w : vocab;
+}
+int forward_words(int vocab) { return piece_words(vocab, 16384); }
+// P of one piece holds at most 2^26 values (256 MB) while pieces of 1024 words allow it.
+int backward_words(int rows, int vocab) {
+    int limit = 8192;
+    while (limit > 1024 && (long long)limit * rows > (1ll << 26)) limit /= 2;
+    return piece_words(vocab, limit);
+}
+
+struct ForwardLayout { int words; size_t product, parts, running, total; };
+bool forward_layout(int N, int V, int D, int S, ForwardLayout& L) {
+    L.words = forward_words(V);
+    size_t bytes;
+    if (!product_bytes(N, L.words, D, S, false, true, &bytes)) return false;
+    L.product = 0;
+    L.parts = bytes;
+    L.running = L.parts + round_up((size_t)2 * ((L.words + EPI_TILE_N - 1) / EPI_TILE_N) * N * sizeof(float2));
+    L.total = L.running + round_up((size_t)N * sizeof(float2));
+    return true;
+}
+
+struct BackwardLayout { int words; size_t weight, coefficient, inv_count, first, last, p, logits, dx, dw, total, logits_bytes, dx_bytes, dw_bytes; };
+bool backward_layout(int N, int V, int D, int S, BackwardLayout& L) {
+    L.words = backward_words(N, V);
+    if (!product_bytes(N, L.words, D, S, false, true, &L.logits_bytes) || !product_bytes(N, D, L.words, S, false, false, &L.dx_bytes) ||
+        !product_bytes(L.words, D, N, S, true, false, &L.dw_bytes))
+        return false;
+    // the last piece may be narrower, and a narrower product can be planned with more K ranges
+    const int rest = V - (V - 1) / L.words * L.words;
+    size_t b;
+    if (!product_bytes(N, D, rest, S, false, false, &b)) return false;
+    if (b > L.dx_bytes) L.dx_bytes = b;
+    if (!product_bytes(rest, D, N, S, true, false, &b)) return false;
+    if (b > L.dw_bytes) L.dw_bytes = b;
+    L.weight = 0;
+    L.coefficient = L.weight + round_up((size_t)N * 4);
+    L.inv_count = L.coefficient + round_up((size_t)N * 4);
+    L.first = L.inv_count + XENT_ALIGN;
+    L.last = L.first + round_up((size_t)V * 4);
+    L.p = L.last + round_up((size_t)V * 4);
+    L.logits = L.p + round_up((size_t)N * L.words * 4);
+    L.dx = L.logits + L.logits_bytes;
+    L.dw = L.dx + L.dx_bytes;
+    L.total = L.dw + L.dw_bytes;
+    return true;
+}
+
+bool good_sizes(int N, int V, int D, int S) {
+    return N >= 1 && V >= 1 && D >= 1 && S >= 1 && S <= 3 && D <= max_k_per_pass(S) / BLOCK_K * BLOCK_K;
+}
+
+}  // namespace
+}  // namespace rgb200
+
+using namespace rgb200;
+
+extern "C" size_t rgb200_linear_xent_workspace(int N, int V, int D, int slices, int backward) {
+    if (!good_sizes(N, V, D, slices)) return 0;
+    ForwardLayout F;
+    BackwardLayout B;
+    if (backward) return backward_layout(N, V, D, slices, B) ? B.total : 0;
+    return forward_layout(N, V, D, slices, F) ? F.total : 0;
+}
+
+extern "C" int rgb200_linear_xent_forward(const float* X, const float* W, const long long* target, long long ignore_index, int reduction, int N, int V,
+                                          int D, int slices, float* loss, float* nll, float* lse, float* target_logit, void* workspace,
+                                          size_t workspace_bytes, void* stream) {
+    if (!good_sizes(N, V, D, slices) || !X || !W || !target || !nll || !lse || !target_logit || !workspace) return cudaErrorInvalidValue;
+    if (reduction < RGB200_REDUCE_NONE || reduction > RGB200_REDUCE_SUM || (reduction != RGB200_REDUCE_NONE && !loss)) return cudaErrorInvalidValue;
+    ForwardLayout L;
+    if (!forward_layout(N, V, D, slices, L)) return cudaErrorInvalidValue;
+    if (workspace_bytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & (XENT_ALIGN - 1)) != 0) return cudaErrorInvalidValue;
+    cudaError_t e = check_b200();
+    if (e != cudaSuccess) return e;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    char* ws = static_cast<char*>(workspace);
+    const rgb200_config cfg = product_config(slices, false, true);
+    EpilogueParams E = {};
+    E.target = target;
+    E.lse_parts = reinterpret_cast<float2*>(ws + L.parts);
+    E.target_logit = target_logit;
+    for (int at = 0; at < V; at += L.words) {
+        const int words = V - at < L.words ? V - at : L.words;
+        E.first_word = at;
+        // C is not written; the product's other operand checks want an address
+        if ((e = gemm_with_epilogue(X, W + (size_t)at * D, nll, N, words, D, cfg, EPI_LSE, E, at > 0 && words == L.words, false, ws + L.product, L.parts, st)) != cudaSuccess)
+            return e;
+        // the last half tile of a piece has a part only if it has columns
+        const int parts = (words + EPI_TILE_N / 2 - 1) / (EPI_TILE_N / 2);
+        xent_join_kernel<<<(N + XENT_ROWS - 1) / XENT_ROWS, 32 * XENT_WARPS, 0, st>>>(
+            E.lse_parts, parts, reinterpret_cast<float2*>(ws + L.running), N, at == 0, at + words == V, target, ignore_index, V, target_logit, lse, nll);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
+    if (reduction != RGB200_REDUCE_NONE)
+        xent_reduce_kernel<<<1, 1024, 0, st>>>(nll, target, ignore_index, N, reduction == RGB200_REDUCE_MEAN, loss, nullptr);
+    return cudaGetLastError();
+}
+
+extern "C" int rgb200_linear_xent_backward(const float* X, const float* W, const long long* target, long long ignore_index, int reduction, int N, int V,
+                                           int D, int slices, const float* lse, const float* target_logit, const float* dloss, float* dX, float* dW,
+                                           void* workspace, size_t workspace_bytes, void* stream) {
+    if (!good_sizes(N, V, D, slices) || !X || !W || !target || !lse || !target_logit || !dloss || (!dX && !dW) || !workspace) return cudaErrorInvalidValue;
+    if (reduction < RGB200_REDUCE_NONE || reduction > RGB200_REDUCE_SUM) return cudaErrorInvalidValue;
+    BackwardLayout L;
+    if (!backward_layout(N, V, D, slices, L)) return cudaErrorInvalidValue;
+    if (workspace_bytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & (XENT_ALIGN - 1)) != 0) return cudaErrorInvalidValue;
+    cudaError_t e = check_b200();
+    if (e != cudaSuccess) return e;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    char* ws = static_cast<char*>(workspace);
+    float* weight = reinterpret_cast<float*>(ws + L.weight);
+    float* coefficient = reinterpret_cast<float*>(ws + L.coefficient);
+    float* inv_count = reinterpret_cast<float*>(ws + L.inv_count);
+    int* first = reinterpret_cast<int*>(ws + L.first);
+    int* last = reinterpret_cast<int*>(ws + L.last);
+    float* P = reinterpret_cast<float*>(ws + L.p);
+
+    if ((e = cudaMemsetAsync(first, 0x7F, (size_t)V * 4, st)) != cudaSuccess) return e;      // above every row
+    if ((e = cudaMemsetAsync(last, 0xFF, (size_t)V * 4, st)) != cudaSuccess) return e;       // -1
+    if (reduction != RGB200_REDUCE_NONE)
+        xent_reduce_kernel<<<1, 1024, 0, st>>>(nullptr, target, ignore_index, N, reduction == RGB200_REDUCE_MEAN, nullptr, inv_count);
+    xent_rows_kernel<<<(N + 255) / 256, 256, 0, st>>>(target, ignore_index, N, V, lse, target_logit, dloss, reduction == RGB200_REDUCE_NONE, inv_count, weight,
+                                                     coefficient, first, last);
+    if (dX) xent_target_dx_kernel<<<N, 256, 0, st>>>(target, coefficient, W, D, dX);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+
+    EpilogueParams E = {};
+    E.target = target; E.lse = lse; E.row_scale = weight;
+    EpilogueParams add = {};
+    add.residual = dX;
+    for (int at = 0; at < V; at += L.words) {
+        const int words = V - at < L.words ? V - at : L.words;
+        const float* Wp = W + (size_t)at * D;
+        E.first_word = at;
+        if ((e = gemm_with_epilogue(X, Wp, P, N, words, D, product_config(slices, false, true), EPI_PROB, E, at > 0 && words == L.words, false, ws + L.logits,
+                                    L.logits_bytes, st)) != cudaSuccess)
+            return e;
+        if (dX && (e = gemm_with_epilogue(P, Wp, dX, N, D, words, product_config(slices, false, false), EPI_LINEAR, add, false, false, ws + L.dx, L.dx_bytes,
+                                          st)) != cudaSuccess)
+            return e;
+        if (dW && (e = gemm_with_epilogue(P, X, dW + (size_t)at * D, words, D, N, product_config(slices, true, false), EPI_NONE, add, false, at > 0, ws + L.dw,
+                                          L.dw_bytes, st)) != cudaSuccess)
+            return e;
+    }
+    if (dW)
+        xent_target_dw_kernel<<<dim3(N, (D + XENT_DW_COLS - 1) / XENT_DW_COLS), 256, 0, st>>>(target, coefficient, X, first, last, N, V, D, dW);
+    return cudaGetLastError();
+}

@@ -1,0 +1,139 @@
+// Kernels around the products of the linear cross entropy (see rgb200_loss.cu for the sequence).
+#pragma once
+#include <cuda_runtime.h>
+#include <cstdint>
+#include "rgb200_math.cuh"
+
+namespace rgb200 {
+
+constexpr int XENT_ROWS = 32, XENT_WARPS = 16;
+
+// (maximum, sum of exp(value - maximum)) of two sets of values; an empty set is (-inf, 0).
+__device__ __forceinline__ float2 lse_join(float2 a, float2 b) {
+    const float top = fmaxf(a.x, b.x);
+    if (top == -INFINITY) return make_float2(top, 0.0f);
+    return make_float2(top, a.y * expf(a.x - top) + b.y * expf(b.x - top));
+}
+
+// One vocabulary piece's partial statistics [parts][rows] joined into the rows' running ones: a CTA owns 32 rows (lanes), warp k joins
+// parts k, k + 16, ... in order, then the warps' results in order.  last: also log-sum-exp and loss of each row.
+static __global__ void __launch_bounds__(32 * XENT_WARPS)
+xent_join_kernel(const float2* __restrict__ parts, int count, float2* running, int rows, bool first, bool last, const long long* __restrict__ target,
+                 long long ignore, int vocab, const float* __restrict__ target_logit, float* lse, float* nll) {
+    __shared__ float2 joined[XENT_WARPS][XENT_ROWS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * XENT_ROWS + lane;
+    float2 s = make_float2(-INFINITY, 0.0f);
+    if (row < rows) {
+#pragma unroll 4
+        for (int i = warp; i < count; i += XENT_WARPS) s = lse_join(s, parts[(size_t)i * rows + row]);
+    }
+    joined[warp][lane] = s;
+    __syncthreads();
+    if (warp != 0 || row >= rows) return;
+    for (int k = 1; k < XENT_WARPS; ++k) s = lse_join(s, joined[k][lane]);
+    if (!first) s = lse_join(running[row], s);
+    running[row] = s;
+    if (!last) return;
+    const float l = s.x + logf(s.y);
+    lse[row] = l;
+    const long long t = target[row];
+    // a target outside the vocabulary makes the row's loss NaN; an ignored one leaves it 0
+    nll[row] = t == ignore ? 0.0f : t < 0 || t >= vocab ? __int_as_float(0x7FC00000) : l - target_logit[row];
+}
+
+// Sum of the rows' losses (in double, thread t adding rows t, t + 1024, ..., then a tree) over the number of rows that count.
+// loss may be null; inv_count receives 1 / max(1, rows that count) for the mean, 1 for the sum.
+static __global__ void __launch_bounds__(1024)
+xent_reduce_kernel(const float* __restrict__ nll, const long long* __restrict__ target, long long ignore, int rows, bool mean, float* loss, float* inv_count) {
+    __shared__ double sums[1024];
+    __shared__ int counts[1024];
+    double s = 0.0;
+    int n = 0;
+    for (int i = threadIdx.x; i < rows; i += 1024) {
+        if (nll) s += (double)nll[i];
+        n += target[i] != ignore;
+    }
+    sums[threadIdx.x] = s;
+    counts[threadIdx.x] = n;
+    __syncthreads();
+    for (int w = 512; w > 0; w >>= 1) {
+        if (threadIdx.x < w) {
+            sums[threadIdx.x] += sums[threadIdx.x + w];
+            counts[threadIdx.x] += counts[threadIdx.x + w];
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x != 0) return;
+    const double many = mean ? (double)(counts[0] > 1 ? counts[0] : 1) : 1.0;
+    if (loss) *loss = (float)(sums[0] / many);
+    if (inv_count) *inv_count = (float)(1.0 / many);
+}
+
+// Per row: weight g (the loss's gradient, over the number of rows for the mean; 0 for rows that do not count) and the target's
+// coefficient (p - 1) g; and for each word that is a target its first and last row (integer minimum and maximum: any order).
+static __global__ void __launch_bounds__(256)
+xent_rows_kernel(const long long* __restrict__ target, long long ignore, int rows, int vocab, const float* __restrict__ lse,
+                 const float* __restrict__ target_logit, const float* __restrict__ dloss, bool per_row, const float* __restrict__ inv_count, float* weight,
+                 float* coefficient, int* first, int* last) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows) return;
+    const long long t = target[i];
+    const bool counts = t != ignore && t >= 0 && t < vocab;
+    const float g = counts ? (per_row ? dloss[i] : dloss[0] * *inv_count) : 0.0f;
+    weight[i] = g;
+    coefficient[i] = counts ? (expf(target_logit[i] - lse[i]) - 1.0f) * g : 0.0f;
+    if (counts) {
+        atomicMin(first + t, i);
+        atomicMax(last + t, i);
+    }
+}
+
+// dX's start: coefficient times the target's row of W (0 for rows that do not count); the pieces' products are added to it.
+static __global__ void __launch_bounds__(256)
+xent_target_dx_kernel(const long long* __restrict__ target, const float* __restrict__ coefficient, const float* __restrict__ W, int dim, float* dX) {
+    const int row = blockIdx.x;
+    const float c = coefficient[row];
+    const float* w = W + (size_t)(c != 0.0f ? target[row] : 0) * dim;      // a non-zero coefficient has a target inside the vocabulary
+    for (int k = threadIdx.x; k < dim; k += 256) dX[(size_t)row * dim + k] = c != 0.0f ? c * w[k] : 0.0f;
+}
+
+// dW[t] += sum over the rows with target t of coefficient * x.  One CTA for each row that is its target's first, and 128 columns; its
+// eight warps take the range from the first to the last such row in eight equal stretches, each adding its rows in order, then the
+// warps' sums are added in order: the order depends on the targets alone.
+constexpr int XENT_DW_COLS = 128;
+static __global__ void __launch_bounds__(256)
+xent_target_dw_kernel(const long long* __restrict__ target, const float* __restrict__ coefficient, const float* __restrict__ X, const int* __restrict__ first,
+                      const int* __restrict__ last, int rows, int vocab, int dim, float* dW) {
+    __shared__ float sums[8][XENT_DW_COLS];
+    const int row = blockIdx.x;
+    const long long t = target[row];
+    if (t < 0 || t >= vocab || first[t] != row) return;                     // ignored rows were never entered in first
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int stretch = (last[t] - row) / 8 + 1, begin = row + warp * stretch;
+    const int end = begin + stretch < last[t] + 1 ? begin + stretch : last[t] + 1;
+    const int col0 = blockIdx.y * XENT_DW_COLS + lane;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int base = begin; base < end; base += 32) {
+        const int i = base + lane;
+        unsigned hits = __ballot_sync(0xFFFFFFFFu, i < end && target[i] == t);
+        while (hits) {
+            const int k = base + __ffs(hits) - 1;
+            hits &= hits - 1;
+            const float c = coefficient[k];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (col0 + 32 * j < dim) s[j] += c * X[(size_t)k * dim + col0 + 32 * j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums[warp][lane + 32 * j] = s[j];
+    __syncthreads();
+    const int c = threadIdx.x, col = blockIdx.y * XENT_DW_COLS + c;
+    if (c >= XENT_DW_COLS || col >= dim) return;
+    float total = sums[0][c];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) total += sums[k][c];
+    dW[(size_t)t * dim + col] += total;
+}
+
+}  // namespace rgb200

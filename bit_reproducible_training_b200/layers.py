@@ -14,6 +14,7 @@ import torch
 
 from . import repro_conv as rc
 from . import repro_gemm as rg
+from . import repro_loss as rl
 from . import repro_norm as rn
 
 _slices = 3
@@ -229,3 +230,49 @@ class BlockNorm(torch.nn.Module):
         has_y = y is not None
         return block_norm(x, y, weight=self.weight, bias=self.bias, post_weight=self.post_weight if has_y else None,
                           gate=(self.gate if gate is None else gate) if has_y else gate, residual_scale=self.residual_scale, kind=self.kind, eps=self.eps)
+
+
+class _LinearCrossEntropyFn(torch.autograd.Function):
+    """Cross entropy of x W^T in pieces of the vocabulary (repro_loss): keeps two values a row for the backward pass."""
+
+    @staticmethod
+    def forward(ctx, x, weight, target, ignore_index, reduction):
+        loss, lse, target_logit = rl.linear_cross_entropy(x, weight, target, ignore_index, reduction, _slices)
+        ctx.save_for_backward(x, weight, target, lse, target_logit)
+        ctx.how = (ignore_index, reduction, _slices)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        x, weight, target, lse, target_logit = ctx.saved_tensors
+        dx, dw = rl.linear_cross_entropy_backward(dloss, x, weight, target, lse, target_logit, *ctx.how, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return dx, dw, None, None, None
+
+
+def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean"):
+    """Cross entropy of the logits x @ weight.T without storing them, differentiable in x and weight.  x [..., dim], weight
+    [vocabulary, dim], target [...] int64; reduction "mean", "sum" or "none".  See repro_loss.linear_cross_entropy."""
+    if not torch.is_grad_enabled() or not (x.requires_grad or weight.requires_grad):
+        if target.numel():
+            return rl.linear_cross_entropy(x, weight, target, ignore_index, reduction, _slices)[0]
+    n = rl._sizes(x, weight, target, reduction, _slices)[0]
+    if n == 0:                                           # no rows: a loss of 0 (or no losses) and gradients of zeros
+        logits = torch.nn.functional.linear(x, weight)
+        return logits.sum(-1) if reduction == "none" else logits.sum()
+    return _LinearCrossEntropyFn.apply(x, weight, target, ignore_index, reduction)
+
+
+class LinearCrossEntropy(torch.nn.Module):
+    """The output projection of a language model and its loss: forward(x, target).  `weight` [vocabulary, dim] may be shared with
+    an embedding (assign the same Parameter)."""
+
+    def __init__(self, dim, vocabulary, ignore_index=-100, reduction="mean"):
+        super().__init__()
+        if reduction not in rl.REDUCTIONS:
+            raise ValueError("reduction must be 'none', 'mean' or 'sum'")
+        self.ignore_index, self.reduction = ignore_index, reduction
+        self.weight = torch.nn.Parameter(torch.randn(vocabulary, dim) * 0.02)
+
+    def forward(self, x, target):
+        return linear_cross_entropy(x, self.weight, target, self.ignore_index, self.reduction)

@@ -1,0 +1,77 @@
+"""Cross entropy of the logits x @ weight.T against targets in pieces of the vocabulary, on the C ABI.
+
+The [tokens, vocabulary] logits are never stored: the forward pass keeps each row's log-sum-exp and target logit, the
+backward pass forms the probabilities of one piece of words at a time.  ``layers.linear_cross_entropy`` and
+``layers.LinearCrossEntropy`` are the differentiable forms.  CUDA float32 only; there is no CPU path.
+"""
+import torch
+
+from . import _lib
+from .repro_gemm import ReproGemmError, _check, _ptr, _stream, cudaSuccess
+
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _sizes(x, weight, target, reduction, slices):
+    if reduction not in REDUCTIONS:
+        raise ValueError("reduction must be 'none', 'mean' or 'sum'")
+    if slices not in (1, 2, 3):
+        raise ValueError("slices must be 1, 2 or 3")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError("x must be [..., dim] and weight [vocabulary, dim]")
+    if target.dtype != torch.int64:
+        raise TypeError("target must be int64")
+    if target.shape != x.shape[:-1]:
+        raise ValueError("target must have the shape of x without its last dimension")
+    if not (x.device == weight.device == target.device):
+        raise ValueError("all tensors must be on one device")
+    return target.numel(), weight.shape[0], weight.shape[1]
+
+
+def _workspace(n, v, d, slices, backward, device):
+    nbytes = _lib.lib().rgb200_linear_xent_workspace(n, v, d, slices, backward)
+    if nbytes == 0:
+        raise ValueError("sizes not supported: %d tokens, %d words, %d values a token" % (n, v, d))
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean", slices=3):
+    """(loss, lse, target_logit).  x [..., dim], weight [vocabulary, dim], target [...] int64.
+
+    loss: a scalar ("mean" over the rows whose target is not ignore_index, at least 1; or "sum"), or with "none" the rows'
+    losses: 0 where the target is ignore_index and NaN, without a gradient, where it is outside the vocabulary otherwise."""
+    n, v, d = _sizes(x, weight, target, reduction, slices)
+    shape = target.shape
+    x, weight, target = _check(x, n * d, "x"), _check(weight, v * d, "weight"), target.contiguous()
+    out = torch.empty((3, n), dtype=torch.float32, device=x.device)
+    nll, lse, target_logit = out[0], out[1], out[2]
+    loss = torch.empty((), dtype=torch.float32, device=x.device) if reduction != "none" else None
+    with torch.cuda.device(x.device):
+        ws = _workspace(n, v, d, slices, 0, x.device)
+        rc = _lib.lib().rgb200_linear_xent_forward(_ptr(x), _ptr(weight), _ptr(target), ignore_index, REDUCTIONS[reduction], n, v, d, slices, _ptr(loss),
+                                                   _ptr(nll), _ptr(lse), _ptr(target_logit), _ptr(ws), ws.numel(), _stream(None))
+    if rc != cudaSuccess:
+        raise ReproGemmError(rc, "linear_xent_forward")
+    return (nll.view(shape) if loss is None else loss), lse, target_logit
+
+
+def linear_cross_entropy_backward(dloss, x, weight, target, lse, target_logit, ignore_index=-100, reduction="mean", slices=3, want_dx=True, want_dw=True):
+    """(dx, dweight) from the loss's gradient (a scalar, or one value a row with reduction "none") and what the forward call returned."""
+    n, v, d = _sizes(x, weight, target, reduction, slices)
+    shape = x.shape
+    x, weight, target = _check(x, n * d, "x"), _check(weight, v * d, "weight"), target.contiguous()
+    lse, target_logit = _check(lse, n, "lse"), _check(target_logit, n, "target_logit")
+    dloss = _check(dloss, n if reduction == "none" else 1, "dloss")
+    if any(t.device != x.device for t in (dloss, lse, target_logit)):
+        raise ValueError("all tensors must be on one device")
+    dx = torch.empty(shape, dtype=torch.float32, device=x.device) if want_dx else None
+    dw = torch.empty((v, d), dtype=torch.float32, device=x.device) if want_dw else None
+    if not (want_dx or want_dw):
+        return None, None
+    with torch.cuda.device(x.device):
+        ws = _workspace(n, v, d, slices, 1, x.device)
+        rc = _lib.lib().rgb200_linear_xent_backward(_ptr(x), _ptr(weight), _ptr(target), ignore_index, REDUCTIONS[reduction], n, v, d, slices, _ptr(lse),
+                                                    _ptr(target_logit), _ptr(dloss), _ptr(dx), _ptr(dw), _ptr(ws), ws.numel(), _stream(None))
+    if rc != cudaSuccess:
+        raise ReproGemmError(rc, "linear_xent_backward")
+    return dx, dw
