@@ -16,7 +16,7 @@ static_assert(ACT_NONE == RGB200_ACT_NONE && ACT_RELU == RGB200_ACT_RELU && ACT_
 namespace {
 
 template <int S>
-constexpr int epilogue_smem() { return GemmTraits<S, EPI_TILE_N>::SMEM_BYTES + EPI_WARPS * (EPI_TILE_N / 2) * 4; }
+constexpr int epilogue_smem() { return GemmTraits<S, EPI_TILE_N>::SMEM_BYTES + 2 * EPI_WARPS * (EPI_TILE_N / 2) * 4; }
 
 template <int S, int EPI>
 cudaError_t launch(int grid, const CUtensorMap& a, const CUtensorMap& b, const GemmParams& P, cudaStream_t st) {

@@ -94,16 +94,16 @@ struct EpilogueRow<EPI_LINEAR, CPT> {
         }
     }
 
-    template <class Value>
-    __device__ __forceinline__ void finish(const GemmParams& P, int row, int col0, int, const float* slot, Value value) {
+    template <class Values>
+    __device__ __forceinline__ void finish(const GemmParams& P, int row, int col0, int, const float* slot, Values values) {
         const size_t at = (size_t)row * P.N + col0;
         with_activation(P.epi.act, [&](auto act) {
 #pragma unroll
             for (int j = 0; j < CPT; j += 8) {
                 float z[8], y[8];
+                values(j, z);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    z[i] = value(j + i);
                     if (P.epi.bias) z[i] += slot[j + i];
                     y[i] = activation<decltype(act)::value>(z[i]);
                     if (P.epi.residual) y[i] += res[j + i];
@@ -138,14 +138,19 @@ struct EpilogueRow<EPI_LSE, CPT> {
         target = row_ok ? target_column(P, row, col0) : -1;
     }
 
-    template <class Value>
-    __device__ __forceinline__ void finish(const GemmParams& P, int row, int col0, int part, const float*, Value value) {
+    template <class Values>
+    __device__ __forceinline__ void finish(const GemmParams& P, int row, int col0, int part, const float*, Values values) {
         float v[CPT], top = -INFINITY, sum = 0.0f, hit = 0.0f;
 #pragma unroll
-        for (int j = 0; j < CPT; ++j) {
-            v[j] = col0 + j < P.N ? value(j) : -INFINITY;          // the first column is always inside, so top is finite
-            top = fmaxf(top, v[j]);
-            if (j == target) hit = v[j];
+        for (int j = 0; j < CPT; j += 8) {
+            float c[8];
+            values(j, c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[j + i] = col0 + j + i < P.N ? c[i] : -INFINITY;          // the first column is always inside, so top is finite
+                top = fmaxf(top, v[j + i]);
+                if (j + i == target) hit = v[j + i];
+            }
         }
 #pragma unroll
         for (int j = 0; j < CPT; ++j) sum += expf(v[j] - top);
@@ -165,16 +170,17 @@ struct EpilogueRow<EPI_PROB, CPT> {
         scale = row_ok ? __ldg(P.epi.row_scale + row) : 0.0f;
     }
 
-    template <class Value>
-    __device__ __forceinline__ void finish(const GemmParams& P, int row, int col0, int, const float*, Value value) {
+    template <class Values>
+    __device__ __forceinline__ void finish(const GemmParams& P, int row, int col0, int, const float*, Values values) {
         float* dst = P.C + (size_t)row * P.N + col0;
         const bool sectors = (reinterpret_cast<uintptr_t>(dst) & 31) == 0 && col0 + CPT <= P.N;
 #pragma unroll
         for (int j = 0; j < CPT; j += 8) {
             float p[8];
+            values(j, p);
 #pragma unroll
             for (int i = 0; i < 8; ++i)            // a row without a weight takes no part, whatever its logits are
-                p[i] = j + i == target || scale == 0.0f ? 0.0f : expf(value(j + i) - lse) * scale;
+                p[i] = j + i == target || scale == 0.0f ? 0.0f : expf(p[i] - lse) * scale;
             if (sectors) st_global_256(dst + j, p);
             else {
 #pragma unroll

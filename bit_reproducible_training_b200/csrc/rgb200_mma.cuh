@@ -349,6 +349,10 @@ __device__ __forceinline__ void cursor_next(KCursor& c, const GemmParams& P, lon
     if (c.valid) { c.tc = tile_coord(P, c.tile); c.kb = c.tc.kb_begin; }
 }
 
+__device__ __forceinline__ float sum_to_float(long long t) { return __ll2float_rn(t); }
+__device__ __forceinline__ float sum_to_float(int t) { return __int2float_rn(t); }
+static __device__ __noinline__ float round_to_f32_rare(long long t, int e) { return __uint_as_float(round_to_f32_bits(t, e)); }
+
 // One thread's columns of the finished tile through an epilogue; defined in rgb200_epilogue.cuh, which only the
 // translation unit that builds those kernels includes.
 template <int EPI, int CPT>
@@ -376,8 +380,10 @@ gemm_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(gen_base + STAGES * Tr::STAGE_BYTES + 8 * (2 * STAGES + 2));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + STAGES * Tr::STAGE_BYTES + 8 * (2 * STAGES + 3));
     int* eb_slots = reinterpret_cast<int*>(gen_base + STAGES * Tr::STAGE_BYTES + 256);
-    // kernels with an epilogue: as many floats again behind them, one slot of per-column values per epilogue warp
-    [[maybe_unused]] float* col_slots = reinterpret_cast<float*>(eb_slots + EPI_WARPS * (NT / 2));
+    // kernels with an epilogue: twice as many floats again behind them, per epilogue warp a slot of 2^(column exponent) and a
+    // slot of the epilogue's own per-column values
+    [[maybe_unused]] float* scale_slots = reinterpret_cast<float*>(eb_slots + EPI_WARPS * (NT / 2));
+    [[maybe_unused]] float* col_slots = scale_slots + EPI_WARPS * (NT / 2);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long total_tiles = (long long)P.batch * P.split * P.m_tiles * P.n_tiles;
@@ -487,7 +493,24 @@ gemm_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                     eb_s[c] = col0 + c < P.N ? __ldg(P.expo_b + (size_t)tc.batch * P.N + col0 + c) : 0;
             // an epilogue's own operands are requested here too, so that they arrive during the wait
             typename std::conditional<EPI == EPI_NONE, int, EpilogueRow<EPI, CPT>>::type epi_row;
-            if constexpr (EPI != EPI_NONE) epi_row.request(P, row, row_ok, col0, col_slots + (warp - 2) * CPT, lane);
+            [[maybe_unused]] float* scale_s = scale_slots + (warp - 2) * CPT;
+            [[maybe_unused]] bool plain_range = false;
+            if constexpr (EPI != EPI_NONE) {
+                epi_row.request(P, row, row_ok, col0, col_slots + (warp - 2) * CPT, lane);
+                // |T| < 2^62, so with these exponents T, T * 2^(row) and T * 2^(row + column) are all zero or normal floats: the
+                // conversion rounds once and both products are exact
+                int lo = 0x7FFFFFFF, hi = -0x7FFFFFFF;
+                for (int c = lane; c < CPT; c += 32) {
+                    const int e = eb_s[c];
+                    lo = min(lo, e);
+                    hi = max(hi, e);
+                    scale_s[c] = pow2f(min(max(e, -126), 127));
+                }
+                lo = __reduce_min_sync(0xFFFFFFFFu, lo);
+                hi = __reduce_max_sync(0xFFFFFFFFu, hi);
+                const int e_row = ea + P.e0;
+                plain_range = lo >= -126 && hi <= 127 && e_row >= -126 && e_row <= 65 && e_row + lo >= -126 && e_row + hi <= 65;
+            }
             __syncwarp();
             ok = mbar_wait(tmem_full_bar, tile_it & 1u, abort_flag, P.status, STATUS_WAIT_TMEM_FULL);
             ok = __all_sync(0xFFFFFFFFu, ok);
@@ -516,11 +539,17 @@ gemm_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             // phase 2: one rounding per output (or the raw sums), overlapped with the next tile's MMAs
             if constexpr (EPI != EPI_NONE) {
                 if (!row_ok || col0 >= P.N) continue;
-                epi_row.finish(P, row, col0, tc.n_blk * 2 + half, col_slots + (warp - 2) * CPT, [&](int j) {
-                    const int e = ea + P.e0 + eb_s[j];
-                    bool normal;
-                    const uint32_t b = round_to_f32_bits_signed(T[j], e, &normal);
-                    return __uint_as_float(normal ? b : round_to_f32_bits(T[j], e));
+                const int e_row = ea + P.e0;
+                const float row_scale = plain_range ? pow2f(e_row) : 0.0f;
+                // outputs j .. j + 7 of the row, each rounded once to FP32
+                epi_row.finish(P, row, col0, tc.n_blk * 2 + half, col_slots + (warp - 2) * CPT, [&](int j, float (&v)[8]) {
+                    if (plain_range) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(__fmul_rn(sum_to_float(T[j + i]), row_scale), scale_s[j + i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = round_to_f32_rare(T[j + i], e_row + eb_s[j + i]);
+                    }
                 });
                 continue;
             }

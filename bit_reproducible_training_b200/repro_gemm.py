@@ -6,6 +6,7 @@ Names, argument meaning and error behaviour follow repro_gemm_cuda/repro_gemm.cu
 only for device memory and streams; all arithmetic happens in librgb200.so.  There is no CPU path:
 the reference's binding sends CPU tensors to its CPU implementation, this one refuses them.
 """
+import contextlib
 import ctypes as C
 import os
 import enum
@@ -78,6 +79,24 @@ def make_plan(M, N, K, cfg=None, batch=1):
 
 def _ptr(t):
     return C.c_void_p(t.data_ptr()) if t is not None else None
+
+
+def _addr(t):
+    """Address for a ctypes argument or field declared as a pointer (cheaper than a c_void_p of its own)."""
+    return None if t is None else t.data_ptr()
+
+
+_here = contextlib.nullcontext()
+
+
+def _on(device):
+    """Makes `device` current for a call; free of charge where it is current already."""
+    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _raw_stream(device):
+    """torch's current stream on `device` as the integer the C ABI takes."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _stream(stream):
@@ -159,7 +178,7 @@ def _workspace(nbytes, device):
     replayed at the same time."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
+    key = (device.index, _raw_stream(device))
     ws = _ws_cache.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
@@ -204,14 +223,15 @@ def gemm(A, B, M, N, K, trans_a=False, trans_b=False, slices=3, split_k=1, algo=
     (repro_torch/src/bindings.cpp:43-66).  Returns a new [M, N] float32 CUDA tensor."""
     A = _check(A, M * K, "A")
     B = _check(B, K * N, "B")
-    cfg = Config(split_k=split_k, algo=algo, slices=slices, trans_a=trans_a, trans_b=trans_b)
-    rc, plan = make_plan(M, N, K, cfg)
-    if rc != cudaSuccess:
-        raise ReproGemmError(rc, "make_plan")
-    with torch.cuda.device(A.device):
+    L = _lib.lib()
+    cfg, plan = _lib.Config(split_k, 16, 16, 32, int(algo), slices, int(trans_a), int(trans_b)), _lib.Plan()
+    with _on(A.device):
+        rc = L.rgb200_make_plan(M, N, K, C.byref(cfg), C.byref(plan))
+        if rc != cudaSuccess:
+            raise ReproGemmError(rc, "make_plan")
         ws = _workspace(plan.workspace_bytes, A.device)
         out = torch.empty((M, N), dtype=torch.float32, device=A.device)
-        rc = repro_gemm_fp32_ws(A, B, out, M, N, K, cfg, ws)
+        rc = L.rgb200_gemm_fp32_ws(_addr(A), _addr(B), _addr(out), M, N, K, C.byref(cfg), _addr(ws), ws.numel(), _raw_stream(A.device), None)
     if rc != cudaSuccess:
         raise ReproGemmError(rc, "repro_gemm_fp32_ws")
     _raise_if_incomplete(ws, "gemm")
@@ -242,19 +262,19 @@ def gemm_epilogue(A, B, M, N, K, trans_a=False, trans_b=False, slices=3, bias=No
     if out is not None and (out.dtype != torch.float32 or out.numel() != M * N or not out.is_contiguous()):
         raise ValueError("out must be a contiguous float32 tensor of %d elements" % (M * N))
     act = _activation(activation)
-    cfg = Config(slices=slices, trans_a=trans_a, trans_b=trans_b)
-    rc, plan = make_plan(M, N, K, cfg)
-    if rc != cudaSuccess:
-        raise ReproGemmError(rc, "make_plan")
-    with torch.cuda.device(A.device):
+    L = _lib.lib()
+    cfg, plan = _lib.Config(1, 16, 16, 32, 0, slices, int(trans_a), int(trans_b)), _lib.Plan()
+    with _on(A.device):
+        rc = L.rgb200_make_plan(M, N, K, C.byref(cfg), C.byref(plan))
+        if rc != cudaSuccess:
+            raise ReproGemmError(rc, "make_plan")
         ws = _workspace(plan.workspace_bytes, A.device)
         if out is None:
             out = torch.empty((M, N), dtype=torch.float32, device=A.device)
         pre = torch.empty((M, N), dtype=torch.float32, device=A.device) if keep_pre else None
-        e = _lib.Epilogue(_ptr(bias), _ptr(residual), _ptr(pre), act)
-        c = cfg.c()
-        rc = _lib.lib().rgb200_gemm_epilogue_fp32_ws(_ptr(A), _ptr(B), _ptr(out), M, N, K, C.byref(c), C.byref(e), _ptr(ws), ws.numel(),
-                                                     _stream(None))
+        e = _lib.Epilogue(_addr(bias), _addr(residual), _addr(pre), act)
+        rc = L.rgb200_gemm_epilogue_fp32_ws(_addr(A), _addr(B), _addr(out), M, N, K, C.byref(cfg), C.byref(e), _addr(ws), ws.numel(),
+                                            _raw_stream(A.device))
     if rc != cudaSuccess:
         raise ReproGemmError(rc, "gemm_epilogue_fp32_ws")
     _raise_if_incomplete(ws, "gemm_epilogue")
@@ -276,10 +296,10 @@ def activation_backward(dY, Z, M, N, activation=None, want_dz=True, want_db=Fals
     if not act and not want_db or not (want_dz or want_db):
         return (dZ.view(M, N) if want_dz else None), None
     L = _lib.lib()
-    with torch.cuda.device(dY.device):
+    with _on(dY.device):
         ws = _workspace(L.rgb200_activation_backward_workspace(M, N), dY.device) if want_db else None
-        rc = L.rgb200_activation_backward(_ptr(dY), _ptr(Z), _ptr(dZ) if act else None, _ptr(db), M, N, act, _ptr(ws),
-                                          0 if ws is None else ws.numel(), _stream(None))
+        rc = L.rgb200_activation_backward(_addr(dY), _addr(Z), _addr(dZ) if act else None, _addr(db), M, N, act, _addr(ws),
+                                          0 if ws is None else ws.numel(), _raw_stream(dY.device))
     if rc != cudaSuccess:
         raise ReproGemmError(rc, "activation_backward")
     return (dZ.view(M, N) if want_dz else None), db

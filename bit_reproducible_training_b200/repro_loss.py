@@ -7,7 +7,7 @@ backward pass forms the probabilities of one piece of words at a time.  ``layers
 import torch
 
 from . import _lib
-from .repro_gemm import ReproGemmError, _check, _ptr, _stream, cudaSuccess
+from .repro_gemm import ReproGemmError, _addr, _check, _on, _raw_stream, cudaSuccess
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
@@ -46,10 +46,10 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean",
     out = torch.empty((3, n), dtype=torch.float32, device=x.device)
     nll, lse, target_logit = out[0], out[1], out[2]
     loss = torch.empty((), dtype=torch.float32, device=x.device) if reduction != "none" else None
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         ws = _workspace(n, v, d, slices, 0, x.device)
-        rc = _lib.lib().rgb200_linear_xent_forward(_ptr(x), _ptr(weight), _ptr(target), ignore_index, REDUCTIONS[reduction], n, v, d, slices, _ptr(loss),
-                                                   _ptr(nll), _ptr(lse), _ptr(target_logit), _ptr(ws), ws.numel(), _stream(None))
+        rc = _lib.lib().rgb200_linear_xent_forward(_addr(x), _addr(weight), _addr(target), ignore_index, REDUCTIONS[reduction], n, v, d, slices, _addr(loss),
+                                                   _addr(nll), _addr(lse), _addr(target_logit), _addr(ws), ws.numel(), _raw_stream(x.device))
     if rc != cudaSuccess:
         raise ReproGemmError(rc, "linear_xent_forward")
     return (nll.view(shape) if loss is None else loss), lse, target_logit
@@ -68,10 +68,10 @@ def linear_cross_entropy_backward(dloss, x, weight, target, lse, target_logit, i
     dw = torch.empty((v, d), dtype=torch.float32, device=x.device) if want_dw else None
     if not (want_dx or want_dw):
         return None, None
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         ws = _workspace(n, v, d, slices, 1, x.device)
-        rc = _lib.lib().rgb200_linear_xent_backward(_ptr(x), _ptr(weight), _ptr(target), ignore_index, REDUCTIONS[reduction], n, v, d, slices, _ptr(lse),
-                                                    _ptr(target_logit), _ptr(dloss), _ptr(dx), _ptr(dw), _ptr(ws), ws.numel(), _stream(None))
+        rc = _lib.lib().rgb200_linear_xent_backward(_addr(x), _addr(weight), _addr(target), ignore_index, REDUCTIONS[reduction], n, v, d, slices, _addr(lse),
+                                                    _addr(target_logit), _addr(dloss), _addr(dx), _addr(dw), _addr(ws), ws.numel(), _raw_stream(x.device))
     if rc != cudaSuccess:
         raise ReproGemmError(rc, "linear_xent_backward")
     return dx, dw

@@ -13,7 +13,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .repro_gemm import ReproGemmError, _check, _ptr, _stream, _workspace, cudaSuccess
+from .repro_gemm import ReproGemmError, _addr, _check, _on, _raw_stream, _workspace, cudaSuccess
 
 KINDS = {"rms": 0, "layer": 1}
 MAX_DIM = 8192
@@ -31,9 +31,10 @@ class NormGrads:
 
 
 def _same_device(tensors):
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise ValueError("all tensors must be on one device")
+    where = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != where:
+            raise ValueError("all tensors must be on one device")
 
 
 def _sizes(x, y, weight, bias, post_weight, gate, kind, eps):
@@ -76,10 +77,10 @@ def block_norm(x, y=None, *, weight, bias=None, post_weight=None, gate=None, res
     h = torch.empty(shape, dtype=torch.float32, device=x.device)
     r = x if y is None else torch.empty(shape, dtype=torch.float32, device=x.device)
     stats = torch.empty((4, rows), dtype=torch.float32, device=x.device) if keep_stats else None
-    n = _lib.BlockNorm(rows, dim, groups, KINDS[kind], residual_scale, eps, _ptr(x), _ptr(y), _ptr(weight), _ptr(bias), _ptr(post_weight),
-                       _ptr(gate), None if y is None else _ptr(r), _ptr(h), _ptr(stats))
-    with torch.cuda.device(x.device):
-        rc = _lib.lib().rgb200_block_norm_forward(C.byref(n), _stream(None))
+    n = _lib.BlockNorm(rows, dim, groups, KINDS[kind], residual_scale, eps, _addr(x), _addr(y), _addr(weight), _addr(bias), _addr(post_weight),
+                       _addr(gate), None if y is None else _addr(r), _addr(h), _addr(stats))
+    with _on(x.device):
+        rc = _lib.lib().rgb200_block_norm_forward(C.byref(n), _raw_stream(x.device))
     if rc != cudaSuccess:
         raise ReproGemmError(rc, "block_norm_forward")
     return r, h, stats
@@ -105,12 +106,12 @@ def block_norm_backward(dh, dr, r, y, stats, *, weight, bias=None, post_weight=N
     g = NormGrads(out("x", True, shape), out("y", y is not None, shape), out("weight", True, dim), out("bias", bias is not None, dim),
                   out("post_weight", post_weight is not None, dim), out("gate", gate is not None, gate_shape))
     L = _lib.lib()
-    with torch.cuda.device(r.device):
+    with _on(r.device):
         ws = _workspace(L.rgb200_block_norm_backward_workspace(rows, dim, groups), r.device)
-        n = _lib.BlockNorm(rows, dim, groups, KINDS[kind], residual_scale, eps, _ptr(r), _ptr(y), _ptr(weight), None, _ptr(post_weight), _ptr(gate),
-                           _ptr(r), None, _ptr(stats), _ptr(dr), _ptr(dh), _ptr(g.x), _ptr(g.y), _ptr(g.weight), _ptr(g.bias),
-                           _ptr(g.post_weight), _ptr(g.gate))
-        rc = L.rgb200_block_norm_backward(C.byref(n), _ptr(ws), ws.numel(), _stream(None))
+        n = _lib.BlockNorm(rows, dim, groups, KINDS[kind], residual_scale, eps, _addr(r), _addr(y), _addr(weight), None, _addr(post_weight), _addr(gate),
+                           _addr(r), None, _addr(stats), _addr(dr), _addr(dh), _addr(g.x), _addr(g.y), _addr(g.weight), _addr(g.bias),
+                           _addr(g.post_weight), _addr(g.gate))
+        rc = L.rgb200_block_norm_backward(C.byref(n), _addr(ws), ws.numel(), _raw_stream(r.device))
     if rc != cudaSuccess:
         raise ReproGemmError(rc, "block_norm_backward")
     return g

@@ -12,7 +12,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .repro_gemm import ReproGemmError, _stream, cudaSuccess
+from .repro_gemm import ReproGemmError, _on, _raw_stream, cudaSuccess
 
 _torch_optimizer = sys.modules[torch.optim.Optimizer.__module__]        # torch.optim hides the module's own name
 
@@ -152,7 +152,7 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         for index, group in enumerate(self.param_groups):
             if group["params"]:
-                with torch.cuda.device(group["params"][0].device):
+                with _on(group["params"][0].device):
                     self._step_group(index, group)
         return loss
 
@@ -199,7 +199,7 @@ class AdamW(torch.optim.Optimizer):
         b1, b2 = group["betas"]
         h = _lib.AdamwHyper(float(group["lr"]), float(b1), float(b2), float(group["eps"]), float(group["weight_decay"]), n,
                             device_step, self.state_bits)
-        rc = _lib.lib().rgb200_adamw_step(rows.ctypes.data, len(rows), C.byref(h), _stream(None))
+        rc = _lib.lib().rgb200_adamw_step(rows.ctypes.data, len(rows), C.byref(h), _raw_stream(group["params"][0].device))
         if rc != cudaSuccess:
             raise ReproGemmError(rc, "adamw_step")
 
@@ -229,7 +229,7 @@ class AdamW(torch.optim.Optimizer):
             for x, n in zip(list(gm) + list(gv), list(t["rows"]["count"]) * 2):
                 if x.dtype != torch.float32 or x.device != dev or x.numel() != n or not x.is_contiguous():
                     raise ValueError("the moments' values are contiguous float32 tensors of the parameters' sizes on their device")
-            with torch.cuda.device(dev):
+            with _on(dev):
                 if self.state_bits == 32:
                     for s, m, v in zip(t["states"], gm, gv):
                         pairs = ((m, s["exp_avg"]), (v, s["exp_avg_sq"]))
@@ -238,7 +238,7 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 rows = t["rows"].copy()
                 rows["param"], rows["grad"] = [m.data_ptr() for m in gm], [v.data_ptr() for v in gv]
-                rc = getattr(_lib.lib(), call)(rows.ctypes.data, len(rows), _stream(None))
+                rc = getattr(_lib.lib(), call)(rows.ctypes.data, len(rows), _raw_stream(dev))
                 if rc != cudaSuccess:
                     raise ReproGemmError(rc, call[7:])
 
