@@ -1,4 +1,6 @@
 // Host side of the block-norm entry points declared in include/rgb200_train.h.
+#include <mutex>
+
 #include "../../include/rgb200_train.h"
 #include "rgb200_host.h"
 #include "rgb200_norm.cuh"
@@ -24,14 +26,14 @@ bool good_norm(const rgb200_block_norm* n) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Row ranges of the backward pass, from the sizes alone: as many as fill the GPU's 148 SMs with two rows of 256 threads each (or
-// their equivalent), at least eight rows long so that their column sums stay a small part of the traffic.
+// Row ranges of the backward pass, from the sizes alone: as many as fill the GPU's 148 SMs with 512 threads each (or one row
+// of 1024), at least eight rows long so that their column sums stay a small part of the traffic.
 struct NormParts { int per_group, rows, total; };
 NormParts norm_parts(int rows, int dim, int groups) {
     NormParts p = {0, 0, 0};
     if (rows == 0) return p;
     const int group_rows = rows / groups, tpr = norm_threads(dim);
-    long long want = 148ll * (tpr >= 512 ? 1024 / tpr : 512 / tpr) / groups;
+    long long want = 148ll * (tpr <= 512 ? 512 / tpr : 1) / groups;
     if (want < 1) want = 1;
     if (want > (group_rows + 7) / 8) want = (group_rows + 7) / 8;
     p.rows = (int)((group_rows + want - 1) / want);
@@ -56,23 +58,39 @@ NormParams norm_params(const rgb200_block_norm* n) {
     return P;
 }
 
+template <int TPR, int V, int MODE>
+cudaError_t launch_backward(const NormParams& P, int grid, cudaStream_t st) {
+    auto kernel = block_norm_backward_kernel<TPR, V, MODE>;
+    constexpr int BYTES = norm_ring_bytes(TPR, MODE);
+    static std::once_flag once[64];
+    static cudaError_t err[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    std::call_once(once[dev], [&] { err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES); });
+    if (err[dev] != cudaSuccess) return err[dev];
+    kernel<<<grid, norm_cta(TPR), BYTES, st>>>(P);
+    return cudaGetLastError();
+}
+
 template <int TPR, int V>
-void launch_norm(const NormParams& P, bool backward, cudaStream_t st) {
+cudaError_t launch_norm(const NormParams& P, bool backward, cudaStream_t st) {
     constexpr int CTA = norm_cta(TPR), GROUPS = CTA / TPR;
     const int items = backward ? P.parts_total : P.rows, grid = (items - 1) / GROUPS + 1;
     if (!backward) {
         if (!P.y) block_norm_kernel<TPR, V, NORM_ONLY><<<grid, CTA, 0, st>>>(P);
         else if (!P.pw) block_norm_kernel<TPR, V, NORM_RESIDUAL><<<grid, CTA, 0, st>>>(P);
         else block_norm_kernel<TPR, V, NORM_POST><<<grid, CTA, 0, st>>>(P);
-    } else {
-        if (!P.y) block_norm_backward_kernel<TPR, V, NORM_ONLY><<<grid, CTA, 0, st>>>(P);
-        else if (!P.pw) block_norm_backward_kernel<TPR, V, NORM_RESIDUAL><<<grid, CTA, 0, st>>>(P);
-        else block_norm_backward_kernel<TPR, V, NORM_POST><<<grid, CTA, 0, st>>>(P);
+        return cudaGetLastError();
     }
+    if (!P.y) return launch_backward<TPR, V, NORM_ONLY>(P, grid, st);
+    if (!P.pw) return launch_backward<TPR, V, NORM_RESIDUAL>(P, grid, st);
+    return launch_backward<TPR, V, NORM_POST>(P, grid, st);
 }
 
 template <int V>
-void dispatch_norm(const NormParams& P, bool backward, cudaStream_t st) {
+cudaError_t dispatch_norm(const NormParams& P, bool backward, cudaStream_t st) {
     switch (norm_threads(P.dim)) {
         case 32: return launch_norm<32, V>(P, backward, st);
         case 64: return launch_norm<64, V>(P, backward, st);
@@ -95,9 +113,7 @@ extern "C" int rgb200_block_norm_forward(const rgb200_block_norm* n, void* strea
     if (e != cudaSuccess || n->rows == 0) return e;
     const NormParams P = norm_params(n);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (P.dim % 4 == 0) dispatch_norm<4>(P, false, st);
-    else dispatch_norm<1>(P, false, st);
-    return cudaGetLastError();
+    return P.dim % 4 == 0 ? dispatch_norm<4>(P, false, st) : dispatch_norm<1>(P, false, st);
 }
 
 extern "C" size_t rgb200_block_norm_backward_workspace(int rows, int dim, int groups) {
@@ -119,9 +135,8 @@ extern "C" int rgb200_block_norm_backward(const rgb200_block_norm* n, void* work
     P.rows_per_part = parts.rows; P.parts_per_group = parts.per_group; P.parts_total = parts.total;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (n->rows > 0) {
-        if (P.dim % 4 == 0) dispatch_norm<4>(P, true, st);
-        else dispatch_norm<1>(P, true, st);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        e = P.dim % 4 == 0 ? dispatch_norm<4>(P, true, st) : dispatch_norm<1>(P, true, st);
+        if (e != cudaSuccess) return e;
     }
     if (P.dgate || P.dpw) {
         if (P.groups > 1)
