@@ -175,10 +175,12 @@ __device__ __forceinline__ float sqrt_fast(float x) {
     return r;
 }
 // The definition's quotient and roots, correctly rounded, would cost more time than the memory traffic.  `inv` = 1 / scale and the
-// hardware's approximate root (relative error 2^-23) give the companded value within 255 * 8 * 2^-24 < 1.3e-4 of the
-// definition's, so a code can differ only where the value lies that close to a border between two codes; lanes that
-// hold such a value redo it with the definition's operations.  inv = 0 marks a scale whose reciprocal leaves the normal range.
-constexpr float CODE_BORDER = 0.5f - 2.0e-4f;
+// hardware's approximate root (relative error 2^-23) give nearly the same companded value: with u = 2^-24, |m| inv is off by 2 u,
+// half of which the root keeps, 2 u for the root, u for the product, and the definition's own roundings are at most 2 u: 6 u of 127, below
+// 4.6e-5; for v (two roots) 7 u of 255, below 1.1e-4.  A code can differ only where the value lies that close to a border between
+// two codes; lanes that hold such a value redo it with the definition's operations.  inv = 0 marks a scale whose reciprocal
+// leaves the normal range.
+constexpr float BORDER_M = 0.5f - 6.0e-5f, BORDER_V = 0.5f - 1.4e-4f;
 __device__ __forceinline__ float compand_m(float m, float inv) { return copysignf(sqrt_fast(fabsf(m) * inv) * 127.0f, m); }
 __device__ __forceinline__ float compand_v(float v, float inv) { return sqrt_fast(sqrt_fast(v * inv)) * 255.0f; }
 __device__ __forceinline__ float code_inverse(float scale) { return scale > 0x1p-100f && scale < 0x1p100f ? __frcp_rn(scale) : 0.0f; }
@@ -190,10 +192,11 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
 
 // Largest magnitude over the warp's block, NaN if any value is not finite (the bits of non-negative floats order as
 // integers, and infinity and NaN lie above every finite value).
+template <bool SIGNED>
 __device__ __forceinline__ float block_scale(const float (&x)[8]) {
     uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7FFFFFFFu);
+    for (int j = 0; j < 8; ++j) top = max(top, SIGNED ? __float_as_uint(x[j]) & 0x7FFFFFFFu : __float_as_uint(x[j]));
     top = __reduce_max_sync(0xFFFFFFFFu, top);
     return __uint_as_float(top >= 0x7F800000u ? 0x7FC00000u : top);
 }
@@ -243,7 +246,7 @@ __device__ __forceinline__ void decode_block(uint2 cm, uint2 cv, float sm, float
 
 __device__ __forceinline__ void encode_block(const float (&m)[8], const float (&v)[8], uint8_t* qm, uint8_t* qv, float* sm, float* sv,
                                              int lane, int live, bool wide) {
-    const float tm = block_scale(m), tv = block_scale(v);
+    const float tm = block_scale<true>(m), tv = block_scale<false>(v);
     const float dm = tm > 0.0f ? tm : 1.0f, dv = tv > 0.0f ? tv : 1.0f;      // NaN: 1, and the codes below are dropped
     const float im = code_inverse(dm), iv = code_inverse(dv);
     float x[8], y[8], worst = im == 0.0f || iv == 0.0f ? 1.0f : 0.0f;
@@ -251,13 +254,13 @@ __device__ __forceinline__ void encode_block(const float (&m)[8], const float (&
     for (int j = 0; j < 8; ++j) {
         x[j] = compand_m(m[j], im);
         y[j] = compand_v(v[j], iv);
-        worst = fmaxf(worst, fmaxf(border_distance(x[j]), border_distance(y[j])));
+        worst = fmaxf(worst, fmaxf(border_distance(x[j]) - (BORDER_M - BORDER_V), border_distance(y[j])));
     }
-    if (worst > CODE_BORDER) {
+    if (worst >= BORDER_V) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            if (im == 0.0f || border_distance(x[j]) > CODE_BORDER) x[j] = compand_m_exact(m[j], dm);
-            if (iv == 0.0f || border_distance(y[j]) > CODE_BORDER) y[j] = compand_v_exact(v[j], dv);
+            if (im == 0.0f || border_distance(x[j]) >= BORDER_M) x[j] = compand_m_exact(m[j], dm);
+            if (iv == 0.0f || border_distance(y[j]) >= BORDER_V) y[j] = compand_v_exact(v[j], dv);
         }
     }
     uint32_t a[8], b[8];
@@ -277,6 +280,36 @@ __device__ __forceinline__ void encode_block(const float (&m)[8], const float (&
 
 enum OptMode : int { OPT_STEP, OPT_READ, OPT_WRITE };   // update; codes -> values; values -> codes
 
+template <OptMode MODE, bool FULL>
+__device__ __forceinline__ void opt_block(const OptEntry& e, const AdamwScalars& s, long long block_at, long long at, int lane, bool any_wide) {
+    const bool wide = FULL || any_wide;
+    const int live = FULL ? 8 : at >= e.n ? 0 : (e.n - at < 8 ? (int)(e.n - at) : 8);
+    float* sm = e.sm + block_at / OPT_BLOCK;
+    float* sv = e.sv + block_at / OPT_BLOCK;
+    uint8_t* qm = static_cast<uint8_t*>(e.m) + at;
+    uint8_t* qv = static_cast<uint8_t*>(e.v) + at;
+    float m[8], v[8];
+    if (MODE != OPT_WRITE) decode_block(load_codes(qm, live, wide), load_codes(qv, live, wide), *sm, *sv, m, v);
+    if (MODE == OPT_STEP) {
+        float p[8], g[8];
+        load8(e.p + at, live, wide, p);
+        load8(e.g + at, live, wide, g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            adamw_value(p[j], g[j], m[j], v[j], s);
+            if (j >= live) m[j] = v[j] = 0.0f;                          // lanes past the tensor's end do not set its scale
+        }
+        store8(e.p + at, live, wide, p);
+    } else if (MODE == OPT_READ) {
+        store8(e.p + at, live, wide, m);
+        store8(const_cast<float*>(e.g) + at, live, wide, v);
+    } else {
+        load8(e.p + at, live, wide, m);
+        load8(e.g + at, live, wide, v);
+    }
+    if (MODE != OPT_READ) encode_block(m, v, qm, qv, sm, sv, lane, live, wide);
+}
+
 // OPT_STEP: p, g and the codes.  OPT_READ: the moments' values go to p (first) and g (second, written through a cast
 // away of const by the host's table); OPT_WRITE: they come from there.
 template <int CAP, OptMode MODE>
@@ -294,31 +327,9 @@ adamw8_kernel(const __grid_constant__ OptTable<CAP> T, const __grid_constant__ A
         const long long block_at = chunk_at + (long long)b * OPT_BLOCK;
         if (block_at >= e.n) break;                                     // uniform over the warp
         const long long at = block_at + lane * 8;
-        const int live = at >= e.n ? 0 : (e.n - at < 8 ? (int)(e.n - at) : 8);
-        float* sm = e.sm + block_at / OPT_BLOCK;
-        float* sv = e.sv + block_at / OPT_BLOCK;
-        uint8_t* qm = static_cast<uint8_t*>(e.m) + at;
-        uint8_t* qv = static_cast<uint8_t*>(e.v) + at;
-        float m[8], v[8];
-        if (MODE != OPT_WRITE) decode_block(load_codes(qm, live, wide), load_codes(qv, live, wide), *sm, *sv, m, v);
-        if (MODE == OPT_STEP) {
-            float p[8], g[8];
-            load8(e.p + at, live, wide, p);
-            load8(e.g + at, live, wide, g);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                adamw_value(p[j], g[j], m[j], v[j], s);
-                if (j >= live) m[j] = v[j] = 0.0f;                      // lanes past the tensor's end do not set its scale
-            }
-            store8(e.p + at, live, wide, p);
-        } else if (MODE == OPT_READ) {
-            store8(e.p + at, live, wide, m);
-            store8(const_cast<float*>(e.g) + at, live, wide, v);
-        } else {
-            load8(e.p + at, live, wide, m);
-            load8(e.g + at, live, wide, v);
-        }
-        if (MODE != OPT_READ) encode_block(m, v, qm, qv, sm, sv, lane, live, wide);
+        // whole blocks of aligned tensors go without the checks that ragged ends and odd addresses need
+        if (wide && e.n - block_at >= OPT_BLOCK) opt_block<MODE, true>(e, s, block_at, at, lane, true);
+        else opt_block<MODE, false>(e, s, block_at, at, lane, wide);
     }
 }
 
