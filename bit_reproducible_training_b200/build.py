@@ -17,7 +17,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "librgb200.so")
 OBJ = os.path.join(CSRC, "obj")
 SOURCES = ["rgb200_api.cu", "rgb200_cxx.cu", "rgb200_optim.cu", "rgb200_norm.cu", "rgb200_epilogue.cu",
-           "rgb200_loss.cu"]
+           "rgb200_loss.cu", "rgb200_dual.cu"]
 
 NVCC_FLAGS = ["-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "--fmad=false",
               "-Xcompiler", "-fPIC", "-cudart", "static"]

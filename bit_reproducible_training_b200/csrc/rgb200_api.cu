@@ -461,7 +461,9 @@ struct RunArgs {
     // N, K, S and transposition (row blocks of one product): skip B's pre-pass.
     bool reuse_b = false;
     // An epilogue behind the rounding (see Epilogue); such a product takes the general kernel whatever its shape.
-    bool reuse_a = false;      // the same for op(A), with the same M, N, K, S (both operands k-contiguous)
+    bool reuse_a = false;      // op(A)'s planes and exponents are in place (see Prepared in rgb200_gemm.h)
+    int* status = nullptr;     // a word of the caller's in place of the workspace's (see Prepared)
+    bool zero_status = true;
     int epi = EPI_NONE;
     const EpilogueParams* epi_params = nullptr;
 };
@@ -475,14 +477,15 @@ cudaError_t run(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
     int* eb = reinterpret_cast<int*>(a.ws + L.eb);
     uint32_t* max_a = reinterpret_cast<uint32_t*>(a.ws + L.max_a);
     uint32_t* max_b = reinterpret_cast<uint32_t*>(a.ws + L.max_b);
-    int* status = reinterpret_cast<int*>(a.ws + L.status);
+    int* status = a.status ? a.status : reinterpret_cast<int*>(a.ws + L.status);
+    int* clear_status = a.zero_status ? status : nullptr;
     long long* part = L.use_partial_ws ? reinterpret_cast<long long*>(a.ws + L.part) : a.T_out;
     const int e0 = -14 * (S - 1);
 
     cudaError_t e = cudaSuccess;
     // Skinny output (N <= 64) with a k-contiguous A: A's split is fused into the MMA kernel's producer and its
     // digit planes never reach HBM (rgb200_rowfused.cuh); only B goes through the pre-pass.
-    const bool fused_a = !a.hook && !a.epi && !a.trans_a && !a.max_a && !part && !a.scatter && !a.c_image_rows &&
+    const bool fused_a = !a.hook && !a.epi && !a.reuse_a && !a.trans_a && !a.max_a && !part && !a.scatter && !a.c_image_rows &&
                          L.algo == RGB200_ALGO_TENSORCORE && L.N <= RF_NT && L.split == 1 && L.k_blocks > 1 &&
                          L.K % 4 == 0 && (reinterpret_cast<uintptr_t>(a.A) & 15) == 0 && (L.batch == 1 || a.stride_a % 4 == 0);
     // Both operands k-contiguous (the forward product of a linear layer, C = A B^T): one launch splits both
@@ -517,6 +520,17 @@ cudaError_t run(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
         record(0);
         if ((e = a.hook->launch(a.hook->ctx, L, max_a, max_b, qa, qb, ea, eb, a.st)) != cudaSuccess) return e;
         record(1);
+    } else if (a.reuse_a) {
+        // A's planes are in place; B's may be too (the status word then keeps the value of the call that left them)
+        if (!a.reuse_b && !both_kmajor && (e = cudaMemsetAsync(a.ws, 0, L.zero_b_bytes, a.st)) != cudaSuccess) return e;
+        record(0);
+        if (!a.reuse_b && both_kmajor) {
+            const KmajorOperand opb{a.B, a.max_b, qb, eb, L.N, a.stride_b}, none{nullptr, nullptr, nullptr, nullptr, 0, 0};
+            launch_kmajor<S>(opb, none, L.K, L.Kp, L.batch, clear_status, a.st);
+        } else if (!a.reuse_b) {
+            launch_split<S>(a.B, a.trans_b, a.max_b, max_b, qb, eb, L.N, L.K, L.Kp, L.batch, a.stride_b, status, a.st);
+        }
+        record(1);
     } else if (a.reuse_b) {
         // B's planes and exponents are those of the previous call on this workspace (same N, K, S): only A is split
         if (a.trans_a && (e = cudaMemsetAsync(a.ws + L.max_a, 0, L.zero_a_bytes, a.st)) != cudaSuccess) return e;
@@ -527,9 +541,7 @@ cudaError_t run(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
         record(0);
         const KmajorOperand opa{a.A, a.max_a, qa, ea, L.M, a.stride_a};
         const KmajorOperand opb{a.B, a.max_b, qb, eb, L.N, a.stride_b};
-        const KmajorOperand none{nullptr, nullptr, nullptr, nullptr, 0, 0};
-        if (a.reuse_a) launch_kmajor<S>(opb, none, L.K, L.Kp, L.batch, status, a.st);
-        else launch_kmajor<S>(opa, opb, L.K, L.Kp, L.batch, status, a.st);
+        launch_kmajor<S>(opa, opb, L.K, L.Kp, L.batch, clear_status, a.st);
         record(1);
     } else {
         if ((e = cudaMemsetAsync(a.ws, 0, L.zero_b_bytes, a.st)) != cudaSuccess) return e;   // status word + column maxima of B
@@ -645,21 +657,37 @@ cudaError_t dispatch(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
 }  // namespace
 
 // The product with an epilogue, for the entry points of rgb200_train.h (declared in rgb200_gemm.h).
-cudaError_t gemm_with_epilogue(const float* A, const float* B, float* C, int M, int N, int K, const rgb200_config& cfg, int epi,
-                               const EpilogueParams& E, bool reuse_a, bool reuse_b, void* ws, size_t ws_bytes, cudaStream_t st) {
-    Layout L;
+static cudaError_t epilogue_layout(int M, int N, int K, const rgb200_config& cfg, int epi, Layout& L) {
     const bool any_ranges = epi == EPI_NONE || epi == EPI_LINEAR;
     cudaError_t e = plan_layout(M, N, K, K, 1, cfg, false, L, 4611686018427387904.0, any_ranges);
     if (e != cudaSuccess) return e;
+    return !any_ranges && L.split != 1 ? cudaErrorNotSupported : cudaSuccess;
+}
+
+cudaError_t plane_slots(int M, int N, int K, const rgb200_config& cfg, void* ws, PlaneSlots* out) {
+    Layout L;
+    cudaError_t e = epilogue_layout(M, N, K, cfg, EPI_NONE, L);        // A's place does not depend on the K ranges
+    if (e != cudaSuccess) return e;
+    char* base = static_cast<char*>(ws);
+    *out = PlaneSlots{reinterpret_cast<signed char*>(base + L.qa), reinterpret_cast<int*>(base + L.ea), L.Kp};
+    return cudaSuccess;
+}
+
+cudaError_t gemm_with_epilogue(const float* A, const float* B, float* C, int M, int N, int K, const rgb200_config& cfg, int epi,
+                               const EpilogueParams& E, Prepared prepared, void* ws, size_t ws_bytes, cudaStream_t st) {
+    Layout L;
+    cudaError_t e = epilogue_layout(M, N, K, cfg, epi, L);
+    if (e != cudaSuccess) return e;
     const DeviceInfo* dev = nullptr;
     if ((e = check_device(L.algo, &dev)) != cudaSuccess) return e;
-    if (L.algo != RGB200_ALGO_TENSORCORE || (!any_ranges && L.split != 1)) return cudaErrorNotSupported;
+    if (L.algo != RGB200_ALGO_TENSORCORE) return cudaErrorNotSupported;
     if (!ws || ws_bytes < L.total) return cudaErrorInvalidValue;
     RunArgs a{A, B, C, nullptr, nullptr, nullptr, 0, 0, 0, cfg.trans_a != 0, cfg.trans_b != 0, static_cast<char*>(ws), st, nullptr};
     a.epi = epi;
     a.epi_params = &E;
-    a.reuse_a = reuse_a;
-    a.reuse_b = reuse_b;
+    a.reuse_a = prepared.a;
+    a.reuse_b = prepared.b;
+    if (prepared.status) { a.status = prepared.status; a.zero_status = prepared.zero_status; }
     return dispatch(L, a, *dev);
 }
 

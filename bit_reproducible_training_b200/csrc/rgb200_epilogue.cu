@@ -78,7 +78,7 @@ extern "C" int rgb200_gemm_epilogue_fp32_ws(const float* A, const float* B, floa
     if (!A || !B || !C || !cfg || !epilogue || epilogue->activation < 0 || epilogue->activation >= ACT_COUNT) return cudaErrorInvalidValue;
     EpilogueParams E = {};
     E.bias = epilogue->bias; E.residual = epilogue->residual; E.pre = epilogue->pre_activation; E.act = epilogue->activation;
-    return gemm_with_epilogue(A, B, C, M, N, K, *cfg, EPI_LINEAR, E, false, false, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+    return gemm_with_epilogue(A, B, C, M, N, K, *cfg, EPI_LINEAR, E, Prepared(), workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t rgb200_activation_backward_workspace(int M, int N) {
@@ -87,6 +87,57 @@ extern "C" size_t rgb200_activation_backward_workspace(int M, int N) {
     return n < 256 ? 256 : n;
 }
 
+namespace {
+
+// dZ (when P.dz), the columns' sums (db, with P.parts for the ranges') and, when P.row_max is set, dZ's maxima.
+cudaError_t run_activation_backward(ActBackwardParams P, float* db, cudaStream_t st) {
+    const int ranges = backward_ranges(P.M, P.N);
+    auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+    P.wide = aligned(P.dy) && aligned(P.z) && aligned(P.dz);
+    dim3 grid((P.N + ACTB_COLS - 1) / ACTB_COLS, 0);
+    if (P.M > 0) {
+        P.rows_per_range = (P.M + ranges - 1) / ranges;
+        grid.y = (P.M + P.rows_per_range - 1) / P.rows_per_range;
+        if (P.N % 4 == 0) activation_backward_kernel<4><<<grid, 32 * ACTB_WARPS, 0, st>>>(P);
+        else activation_backward_kernel<1><<<grid, 32 * ACTB_WARPS, 0, st>>>(P);
+        cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+    }
+    if (db) range_sums_kernel<<<(P.N + 31) / 32, 256, 0, st>>>(P.parts, (int)grid.y, P.N, db);
+    return cudaGetLastError();
+}
+
+constexpr size_t LB_ALIGN = 256;
+size_t lb_round(size_t x) { return (x + LB_ALIGN - 1) / LB_ALIGN * LB_ALIGN; }
+
+rgb200_config backward_config(int slices, bool ta) {
+    rgb200_config c;
+    rgb200_default_config(&c);
+    c.slices = slices; c.trans_a = ta;
+    return c;
+}
+
+// Workspace of the linear layer's backward pass: dZ (with an activation), its maxima, the ranges' column sums, and each product's own.
+struct LinearBackwardLayout { size_t status, maxima, dz, parts, dx, dw, total, dx_bytes, dw_bytes; };
+bool linear_backward_layout(int M, int N, int K, int act, int S, LinearBackwardLayout& L) {
+    if (M < 1 || N < 1 || K < 1 || S < 1 || S > 3 || act < 0 || act >= ACT_COUNT) return false;
+    const rgb200_config cx = backward_config(S, false), cw = backward_config(S, true);
+    rgb200_layout_info ix, iw;
+    if (rgb200_layout(M, K, N, 1, &cx, &ix) != cudaSuccess || rgb200_layout(N, K, M, 1, &cw, &iw) != cudaSuccess) return false;
+    L.dx_bytes = lb_round(ix.workspace_bytes);
+    L.dw_bytes = lb_round(iw.workspace_bytes);
+    L.status = 0;                            // one word, directly in front of the maxima: cleared together
+    L.maxima = 4;
+    L.dz = lb_round(L.maxima + (size_t)M * 4 + (size_t)N * 4);
+    L.parts = L.dz + (act == ACT_NONE ? 0 : lb_round((size_t)M * N * 4));
+    L.dx = L.parts + lb_round((size_t)backward_ranges(M, N) * N * 4);
+    L.dw = L.dx + L.dx_bytes;
+    L.total = L.dw + L.dw_bytes;
+    return true;
+}
+
+}  // namespace
+
 extern "C" int rgb200_activation_backward(const float* dY, const float* Z, float* dZ, float* db, int M, int N, int activation, void* workspace,
                                           size_t workspace_bytes, void* stream) {
     if (M < 0 || N < 1 || activation < 0 || activation >= ACT_COUNT || (!dZ && !db)) return cudaErrorInvalidValue;
@@ -94,23 +145,52 @@ extern "C" int rgb200_activation_backward(const float* dY, const float* Z, float
     if (db && (!workspace || workspace_bytes < rgb200_activation_backward_workspace(M, N))) return cudaErrorInvalidValue;
     cudaError_t e = check_b200();
     if (e != cudaSuccess) return e;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int ranges = backward_ranges(M, N);
-    ActBackwardParams P;
+    ActBackwardParams P = {};
     P.dy = dY; P.z = Z; P.dz = dZ;
     P.parts = db ? static_cast<float*>(workspace) : nullptr;
     P.M = M; P.N = N; P.act = activation;
-    auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-    P.wide = aligned(dY) && aligned(Z) && aligned(dZ);
-    if (M > 0) {
-        P.rows_per_range = (M + ranges - 1) / ranges;
-        const dim3 grid((N + ACTB_COLS - 1) / ACTB_COLS, (M + P.rows_per_range - 1) / P.rows_per_range);
-        if (N % 4 == 0) activation_backward_kernel<4><<<grid, 32 * ACTB_WARPS, 0, st>>>(P);
-        else activation_backward_kernel<1><<<grid, 32 * ACTB_WARPS, 0, st>>>(P);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
-        if (db) range_sums_kernel<<<(N + 31) / 32, 256, 0, st>>>(P.parts, (int)grid.y, N, db);
-    } else if (db) {
-        range_sums_kernel<<<(N + 31) / 32, 256, 0, st>>>(P.parts, 0, N, db);
+    return run_activation_backward(P, db, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t rgb200_linear_backward_workspace(int M, int N, int K, int activation, int slices) {
+    LinearBackwardLayout L;
+    return linear_backward_layout(M, N, K, activation, slices, L) ? L.total : 0;
+}
+
+extern "C" int rgb200_linear_backward(const float* dY, const float* Z, const float* X, const float* W, float* dX, float* dW, float* db, int M, int N, int K,
+                                      int activation, int slices, void* workspace, size_t workspace_bytes, void* stream) {
+    LinearBackwardLayout L;
+    if (!linear_backward_layout(M, N, K, activation, slices, L) || !dY || (activation != ACT_NONE && !Z) || (!dX && !dW && !db)) return cudaErrorInvalidValue;
+    if ((dX && !W) || (dW && !X)) return cudaErrorInvalidValue;
+    if (!workspace || workspace_bytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & (LB_ALIGN - 1)) != 0) return cudaErrorInvalidValue;
+    cudaError_t e = check_b200();
+    if (e != cudaSuccess) return e;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    char* ws = static_cast<char*>(workspace);
+    const bool both = dX && dW;
+    ActBackwardParams P = {};
+    P.dy = dY; P.z = Z;
+    P.dz = activation != ACT_NONE && (dX || dW) ? reinterpret_cast<float*>(ws + L.dz) : nullptr;
+    P.parts = db ? reinterpret_cast<float*>(ws + L.parts) : nullptr;
+    P.M = M; P.N = N; P.act = activation;
+    if (both) {
+        P.row_max = reinterpret_cast<unsigned*>(ws + L.maxima);
+        P.col_max = P.row_max + M;
     }
-    return cudaGetLastError();
+    if ((e = cudaMemsetAsync(ws + L.status, 0, L.maxima + (both ? (size_t)M * 4 + (size_t)N * 4 : 0), st)) != cudaSuccess) return e;
+    if ((P.dz || db || both) && (e = run_activation_backward(P, db, st)) != cudaSuccess) return e;
+    const float* dz = P.dz ? P.dz : dY;
+    const rgb200_config cx = backward_config(slices, false), cw = backward_config(slices, true);
+    Prepared prepared;
+    prepared.status = reinterpret_cast<int*>(ws + L.status);
+    if (both) {
+        PlaneSlots rows, cols;
+        if ((e = plane_slots(M, K, N, cx, ws + L.dx, &rows)) != cudaSuccess || (e = plane_slots(N, K, M, cw, ws + L.dw, &cols)) != cudaSuccess) return e;
+        if ((e = launch_split_both(slices, dz, M, N, P.row_max, P.col_max, rows, cols, st)) != cudaSuccess) return e;
+        prepared.a = true;
+    }
+    const EpilogueParams none = {};
+    if (dX && (e = gemm_with_epilogue(dz, W, dX, M, K, N, cx, EPI_NONE, none, prepared, ws + L.dx, L.dx_bytes, st)) != cudaSuccess) return e;
+    if (dW && (e = gemm_with_epilogue(dz, X, dW, N, K, M, cw, EPI_NONE, none, prepared, ws + L.dw, L.dw_bytes, st)) != cudaSuccess) return e;
+    return cudaSuccess;
 }

@@ -95,7 +95,8 @@ struct EpilogueRow<EPI_LINEAR, CPT> {
     }
 
     template <class Values>
-    __device__ __forceinline__ void finish(const GemmParams& P, int row, int col0, int, const float* slot, Values values) {
+    __device__ __forceinline__ void finish(const GemmParams& P, int row, bool row_ok, int col0, int, const float* slot, Values values) {
+        if (!row_ok) return;
         const size_t at = (size_t)row * P.N + col0;
         with_activation(P.epi.act, [&](auto act) {
 #pragma unroll
@@ -139,7 +140,8 @@ struct EpilogueRow<EPI_LSE, CPT> {
     }
 
     template <class Values>
-    __device__ __forceinline__ void finish(const GemmParams& P, int row, int col0, int part, const float*, Values values) {
+    __device__ __forceinline__ void finish(const GemmParams& P, int row, bool row_ok, int col0, int part, const float*, Values values) {
+        if (!row_ok) return;
         float v[CPT], top = -INFINITY, sum = 0.0f, hit = 0.0f;
 #pragma unroll
         for (int j = 0; j < CPT; j += 8) {
@@ -171,22 +173,39 @@ struct EpilogueRow<EPI_PROB, CPT> {
     }
 
     template <class Values>
-    __device__ __forceinline__ void finish(const GemmParams& P, int row, int col0, int, const float*, Values values) {
+    __device__ __forceinline__ void finish(const GemmParams& P, int row, bool row_ok, int col0, int, const float*, Values values) {
         float* dst = P.C + (size_t)row * P.N + col0;
-        const bool sectors = (reinterpret_cast<uintptr_t>(dst) & 31) == 0 && col0 + CPT <= P.N;
+        const bool sectors = row_ok && (reinterpret_cast<uintptr_t>(dst) & 31) == 0 && col0 + CPT <= P.N;
+        float row_top = 0.0f;
+        unsigned col_top = 0;
+        static_assert(CPT <= 32, "one column a lane");
 #pragma unroll
         for (int j = 0; j < CPT; j += 8) {
             float p[8];
             values(j, p);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)            // a row without a weight takes no part, whatever its logits are
-                p[i] = j + i == target || scale == 0.0f ? 0.0f : expf(p[i] - lse) * scale;
+            for (int i = 0; i < 8; ++i) {          // a row without a weight takes no part, whatever its logits are
+                p[i] = j + i == target || scale == 0.0f || col0 + j + i >= P.N ? 0.0f : expf(p[i] - lse) * scale;
+                row_top = fmaxf(row_top, fabsf(p[i]));
+            }
+            if (P.epi.col_max) {                   // rows that do not exist have no weight and join as zeros
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const unsigned top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(fmaxf(0.0f, fabsf(p[i]))));
+                    if ((threadIdx.x & 31) == j + i) col_top = top;
+                }
+            }
             if (sectors) st_global_256(dst + j, p);
-            else {
+            else if (row_ok) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if (col0 + j + i < P.N) dst[j + i] = p[i];
             }
+        }
+        if (P.epi.row_max && row_ok) atomicMax(P.epi.row_max + row, __float_as_uint(row_top));
+        if (P.epi.col_max) {
+            const int c = threadIdx.x & 31;
+            if (c < CPT && col0 + c < P.N) atomicMax(P.epi.col_max + col0 + c, col_top);
         }
     }
 };
@@ -245,6 +264,7 @@ struct ActBackwardParams {
     const float *dy, *z;
     float *dz;                  // null: only the column sums
     float *parts;               // [ranges][N], or null without a bias gradient
+    unsigned *row_max, *col_max;        // [M], [N]: the bits of dZ's largest magnitudes are joined in (zeroed by the caller), or null
     int M, N, act, rows_per_range, wide;
 };
 
@@ -259,7 +279,7 @@ activation_backward_kernel(const ActBackwardParams P) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) col[j] = blockIdx.x * ACTB_COLS + (V == 4 ? lane * 4 + j : j * 32 + lane);
     const bool wide = V == 4 && P.wide;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, top[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     with_activation(P.act, [&](auto act) {
         constexpr int ACT = decltype(act)::value;
 #pragma unroll 4
@@ -287,6 +307,12 @@ activation_backward_kernel(const ActBackwardParams P) {
             for (int j = 0; j < 4; ++j) {
                 if (ACT != ACT_NONE) d[j] = d[j] * activation_slope<ACT>(z[j]);
                 s[j] += d[j];
+                top[j] = fmaxf(top[j], fabsf(d[j]));
+            }
+            if (P.row_max) {
+                const float m = fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fmaxf(fabsf(d[3]), 0.0f)));
+                const unsigned all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m));
+                if (lane == 0) atomicMax(P.row_max + row, all);
             }
             if (P.dz) {
                 if (wide) {
@@ -299,6 +325,19 @@ activation_backward_kernel(const ActBackwardParams P) {
             }
         }
     });
+    if (P.col_max) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sums[warp][col[j] - blockIdx.x * ACTB_COLS] = top[j];
+        __syncthreads();
+        const int c = threadIdx.x, out = blockIdx.x * ACTB_COLS + c;
+        if (c < ACTB_COLS && out < P.N) {
+            float m = sums[0][c];
+#pragma unroll
+            for (int k = 1; k < ACTB_WARPS; ++k) m = fmaxf(m, sums[k][c]);
+            atomicMax(P.col_max + out, __float_as_uint(m));
+        }
+        __syncthreads();
+    }
     if (!P.parts) return;
 #pragma unroll
     for (int j = 0; j < 4; ++j) sums[warp][col[j] - blockIdx.x * ACTB_COLS] = s[j];

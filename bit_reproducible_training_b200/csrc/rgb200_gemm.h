@@ -7,11 +7,33 @@ namespace rgb200 {
 
 struct EpilogueParams;
 
+// What gemm_with_epilogue may take as prepared in its workspace.
+struct Prepared {
+    // op(A)'s digit planes and exponents are in place: from a call with the same M, N, K, slices and transposition, or written
+    // through plane_slots
+    bool a = false;
+    // op(B)'s are, from the previous call on this workspace with the same N, K, slices and transposition
+    bool b = false;
+    // Where the kernels report an expired wait, in place of the workspace's own word: an operation of several products keeps one
+    // word, so that a later product does not clear an earlier one's report.  It is zeroed by the first call (zero_status, needs
+    // both operands k-contiguous) or by the caller.
+    int* status = nullptr;
+    bool zero_status = false;
+};
+
+// Where a product's workspace holds op(A): planes [slices][M][k_padded] and exponents [M].
+struct PlaneSlots { signed char* planes; int* expo; int k_padded; };
+cudaError_t plane_slots(int M, int N, int K, const rgb200_config& cfg, void* ws, PlaneSlots* out);
+
 // C = epilogue(op(A) op(B)): rgb200_gemm_fp32_ws with an epilogue (EPI_*).  The workspace is the one rgb200_make_plan asks for.
 // EPI_NONE is the plain product; the cross-entropy epilogues need the whole K in one pass (K within one INT32 accumulation).
-// reuse_b: the workspace still holds B's digit planes from the previous call on it with the same N, K, slices and transposition;
-// reuse_a: A's, from a call with the same M, N, K, slices, both operands k-contiguous (C = A B^T).
+// A may be null where it is prepared.
 cudaError_t gemm_with_epilogue(const float* A, const float* B, float* C, int M, int N, int K, const rgb200_config& cfg, int epi,
-                               const EpilogueParams& E, bool reuse_a, bool reuse_b, void* ws, size_t ws_bytes, cudaStream_t st);
+                               const EpilogueParams& E, Prepared prepared, void* ws, size_t ws_bytes, cudaStream_t st);
+
+// Digit planes of src [R][C] as the row-scaled operand (k along the columns) and as the column-scaled one (k along the rows),
+// from the bits of its rows' and columns' largest magnitudes (rgb200_dual.cuh).
+cudaError_t launch_split_both(int slices, const float* src, int R, int C, const unsigned* row_max, const unsigned* col_max, const PlaneSlots& rows,
+                              const PlaneSlots& cols, cudaStream_t st);
 
 }  // namespace rgb200

@@ -53,19 +53,21 @@ int backward_words(int rows, int vocab) {
     return piece_words(vocab, limit);
 }
 
-struct ForwardLayout { int words; size_t product, parts, running, total; };
+struct ForwardLayout { int words; size_t status, product, product_bytes, parts, running, total; };
 bool forward_layout(int N, int V, int D, int S, ForwardLayout& L) {
     L.words = forward_words(V);
     size_t bytes;
     if (!product_bytes(N, L.words, D, S, false, true, &bytes)) return false;
-    L.product = 0;
-    L.parts = bytes;
+    L.status = 0;
+    L.product = XENT_ALIGN;
+    L.product_bytes = bytes;
+    L.parts = L.product + bytes;
     L.running = L.parts + round_up((size_t)2 * ((L.words + EPI_TILE_N - 1) / EPI_TILE_N) * N * sizeof(float2));
     L.total = L.running + round_up((size_t)N * sizeof(float2));
     return true;
 }
 
-struct BackwardLayout { int words; size_t weight, coefficient, inv_count, first, last, p, logits, dx, dw, total, logits_bytes, dx_bytes, dw_bytes; };
+struct BackwardLayout { int words; size_t status, maxima, weight, coefficient, inv_count, first, last, p, logits, dx, dw, total, logits_bytes, dx_bytes, dw_bytes; };
 bool backward_layout(int N, int V, int D, int S, BackwardLayout& L) {
     L.words = backward_words(N, V);
     if (!product_bytes(N, L.words, D, S, false, true, &L.logits_bytes) || !product_bytes(N, D, L.words, S, false, false, &L.dx_bytes) ||
@@ -78,7 +80,9 @@ bool backward_layout(int N, int V, int D, int S, BackwardLayout& L) {
     if (b > L.dx_bytes) L.dx_bytes = b;
     if (!product_bytes(rest, D, N, S, true, false, &b)) return false;
     if (b > L.dw_bytes) L.dw_bytes = b;
-    L.weight = 0;
+    L.status = 0;
+    L.maxima = XENT_ALIGN;
+    L.weight = L.maxima + round_up((size_t)N * 4 + (size_t)L.words * 4);
     L.coefficient = L.weight + round_up((size_t)N * 4);
     L.inv_count = L.coefficient + round_up((size_t)N * 4);
     L.first = L.inv_count + XENT_ALIGN;
@@ -129,7 +133,9 @@ extern "C" int rgb200_linear_xent_forward(const float* X, const float* W, const 
         const int words = V - at < L.words ? V - at : L.words;
         E.first_word = at;
         // C is not written; the product's other operand checks want an address
-        if ((e = gemm_with_epilogue(X, W + (size_t)at * D, nll, N, words, D, cfg, EPI_LSE, E, at > 0 && words == L.words, false, ws + L.product, L.parts, st)) != cudaSuccess)
+        if ((e = gemm_with_epilogue(X, W + (size_t)at * D, nll, N, words, D, cfg, EPI_LSE, E,
+                                    Prepared{at > 0 && words == L.words, false, reinterpret_cast<int*>(ws + L.status), at == 0}, ws + L.product,
+                                    L.product_bytes, st)) != cudaSuccess)
             return e;
         // the last half tile of a piece has a part only if it has columns
         const int parts = (words + EPI_TILE_N / 2 - 1) / (EPI_TILE_N / 2);
@@ -174,18 +180,31 @@ extern "C" int rgb200_linear_xent_backward(const float* X, const float* W, const
     E.target = target; E.lse = lse; E.row_scale = weight;
     EpilogueParams add = {};
     add.residual = dX;
+    const bool both = dX && dW;
+    int* status = reinterpret_cast<int*>(ws + L.status);
     for (int at = 0; at < V; at += L.words) {
         const int words = V - at < L.words ? V - at : L.words;
         const float* Wp = W + (size_t)at * D;
         E.first_word = at;
-        if ((e = gemm_with_epilogue(X, Wp, P, N, words, D, product_config(slices, false, true), EPI_PROB, E, at > 0 && words == L.words, false, ws + L.logits,
-                                    L.logits_bytes, st)) != cudaSuccess)
+        if (both) {
+            E.row_max = reinterpret_cast<unsigned*>(ws + L.maxima);
+            E.col_max = E.row_max + N;
+            if ((e = cudaMemsetAsync(E.row_max, 0, (size_t)N * 4 + (size_t)words * 4, st)) != cudaSuccess) return e;
+        }
+        if ((e = gemm_with_epilogue(X, Wp, P, N, words, D, product_config(slices, false, true), EPI_PROB, E,
+                                    Prepared{at > 0 && words == L.words, false, status, at == 0}, ws + L.logits, L.logits_bytes, st)) != cudaSuccess)
             return e;
-        if (dX && (e = gemm_with_epilogue(P, Wp, dX, N, D, words, product_config(slices, false, false), EPI_LINEAR, add, false, false, ws + L.dx, L.dx_bytes,
-                                          st)) != cudaSuccess)
+        const rgb200_config cx = product_config(slices, false, false), cw = product_config(slices, true, false);
+        if (both) {                                  // P once for both products
+            PlaneSlots rows, cols;
+            if ((e = plane_slots(N, D, words, cx, ws + L.dx, &rows)) != cudaSuccess || (e = plane_slots(words, D, N, cw, ws + L.dw, &cols)) != cudaSuccess)
+                return e;
+            if ((e = launch_split_both(slices, P, N, words, E.row_max, E.col_max, rows, cols, st)) != cudaSuccess) return e;
+        }
+        if (dX && (e = gemm_with_epilogue(P, Wp, dX, N, D, words, cx, EPI_LINEAR, add, Prepared{both, false, status}, ws + L.dx, L.dx_bytes, st)) != cudaSuccess)
             return e;
-        if (dW && (e = gemm_with_epilogue(P, X, dW + (size_t)at * D, words, D, N, product_config(slices, true, false), EPI_NONE, add, false, at > 0, ws + L.dw,
-                                          L.dw_bytes, st)) != cudaSuccess)
+        if (dW && (e = gemm_with_epilogue(P, X, dW + (size_t)at * D, words, D, N, cw, EPI_NONE, add, Prepared{both, at > 0, status}, ws + L.dw, L.dw_bytes, st)) !=
+                      cudaSuccess)
             return e;
     }
     if (dW)

@@ -93,6 +93,8 @@ struct EpilogueParams {
     float* target_logit;        // [M]
     const float* lse;           // [M]
     const float* row_scale;     // [M]
+    unsigned* row_max;          // [M], [N]: the bits of the stored values' largest magnitudes are joined in (EPI_PROB; zeroed by the
+    unsigned* col_max;          // caller, or null)
 };
 
 struct GemmParams {
@@ -538,11 +540,11 @@ gemm_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             mbar_arrive(tmem_empty_bar);
             // phase 2: one rounding per output (or the raw sums), overlapped with the next tile's MMAs
             if constexpr (EPI != EPI_NONE) {
-                if (!row_ok || col0 >= P.N) continue;
+                if (col0 >= P.N) continue;                 // uniform over the warp
                 const int e_row = ea + P.e0;
                 const float row_scale = plain_range ? pow2f(e_row) : 0.0f;
                 // outputs j .. j + 7 of the row, each rounded once to FP32
-                epi_row.finish(P, row, col0, tc.n_blk * 2 + half, col_slots + (warp - 2) * CPT, [&](int j, float (&v)[8]) {
+                epi_row.finish(P, row, row_ok, col0, tc.n_blk * 2 + half, col_slots + (warp - 2) * CPT, [&](int j, float (&v)[8]) {
                     if (plain_range) {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(__fmul_rn(sum_to_float(T[j + i]), row_scale), scale_s[j + i]);

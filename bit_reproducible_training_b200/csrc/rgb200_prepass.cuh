@@ -275,7 +275,7 @@ split_kmajor_short_kernel(const KmajorOperand first, const KmajorOperand second,
 constexpr int COLMAX_K_PER_CTA = 64;
 constexpr int COLMAX_MAX_GRID_Y = 65535;       // hardware limit on gridDim.y; longer K is walked by the CTAs
 
-__global__ void __launch_bounds__(PREPASS_THREADS)
+static __global__ void __launch_bounds__(PREPASS_THREADS)
 colmax_kstrided_kernel(const float* __restrict__ src, uint32_t* __restrict__ maxbits, int R, int K,
                        long long src_batch_stride) {
     __shared__ float red[8][128 + 4];
@@ -332,7 +332,7 @@ colmax_kstrided_kernel(const float* __restrict__ src, uint32_t* __restrict__ max
 
 // Row maxima of a k-contiguous operand, written as floats (the K-sharded path's first step).
 // One warp per row; 16-byte loads, four in flight per lane, when the rows are 16-byte aligned.  grid = ceil(R / 8).
-__global__ void __launch_bounds__(PREPASS_THREADS)
+static __global__ void __launch_bounds__(PREPASS_THREADS)
 rowmax_kmajor_kernel(const float* __restrict__ src, float* __restrict__ out, int R, int K) {
     const int row = blockIdx.x * (PREPASS_THREADS / 32) + (threadIdx.x >> 5);
     if (row >= R) return;
@@ -448,7 +448,7 @@ split_kstrided_kernel(const float* __restrict__ src, const uint32_t* __restrict_
 }
 
 // Turns float maxima (as exchanged between ranks) into the bit form split_kstrided_kernel reads.
-__global__ void maxima_to_bits_kernel(const float* __restrict__ in, uint32_t* __restrict__ out, int n) {
+static __global__ void maxima_to_bits_kernel(const float* __restrict__ in, uint32_t* __restrict__ out, int n) {
     int i = blockIdx.x * blockDim.x + threadIdx.x;
     if (i < n) out[i] = f32_bits(fmaxf(in[i], 0.0f));
 }

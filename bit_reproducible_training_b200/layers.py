@@ -89,14 +89,8 @@ class _FusedLinearFn(torch.autograd.Function):
         k, n = weight.shape[1], weight.shape[0]
         m = x.numel() // k
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dx = dw = dz = db = None
-        if need_x or need_w or need_b:
-            dz, db = rg.activation_backward(dy, z, m, n, ctx.activation, need_x or need_w, need_b)
-        if need_x:
-            dx = rg.gemm(dz, weight, m, k, n, False, False, ctx.slices).view(x.shape)
-        if need_w:
-            dw = rg.gemm(dz, x, n, k, m, True, False, ctx.slices)
-        return dx, dw, db, (dy if need_r else None), None
+        dx, dw, db = rg.linear_backward(dy, z, x, weight, m, n, k, ctx.activation, ctx.slices, need_x, need_w, need_b)
+        return None if dx is None else dx.view(x.shape), dw, db, (dy if need_r else None), None
 
 
 def linear(x, weight, bias=None, activation=None, residual=None):

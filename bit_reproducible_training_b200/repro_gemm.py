@@ -305,6 +305,35 @@ def activation_backward(dY, Z, M, N, activation=None, want_dz=True, want_db=Fals
     return (dZ.view(M, N) if want_dz else None), db
 
 
+def linear_backward(dY, Z, X, W, M, N, K, activation=None, slices=3, want_dx=True, want_dw=True, want_db=False):
+    """(dX, dW, db) of Y = act(X W^T + bias): with dZ = dY * act'(Z), dX [M, K] = dZ W, dW [N, K] = dZ^T X, db [N] = column sums
+    of dZ (see activation_backward); None where not wanted.  The products have the bits of ``gemm`` on dZ."""
+    act = _activation(activation)
+    dY, X, W = _check(dY, M * N, "dY"), _check(X, M * K, "X"), _check(W, N * K, "W")
+    if act and Z is None:
+        raise ValueError("the activation's gradient needs Z")
+    Z = _check(Z, M * N, "Z") if act else None
+    if any(t is not None and t.device != dY.device for t in (Z, X, W)):
+        raise ValueError("all tensors must be on one device")
+    if not (want_dx or want_dw or want_db):
+        return None, None, None
+    L = _lib.lib()
+    nbytes = L.rgb200_linear_backward_workspace(M, N, K, act, slices)
+    if nbytes == 0:
+        raise ReproGemmError(cudaErrorInvalidValue, "linear_backward_workspace")
+    with _on(dY.device):
+        dX = torch.empty((M, K), dtype=torch.float32, device=dY.device) if want_dx else None
+        dW = torch.empty((N, K), dtype=torch.float32, device=dY.device) if want_dw else None
+        db = torch.empty(N, dtype=torch.float32, device=dY.device) if want_db else None
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dY.device)
+        rc = L.rgb200_linear_backward(_addr(dY), _addr(Z), _addr(X), _addr(W), _addr(dX), _addr(dW), _addr(db), M, N, K, act, slices, _addr(ws), nbytes,
+                                      _raw_stream(dY.device))
+    if rc != cudaSuccess:
+        raise ReproGemmError(rc, "linear_backward")
+    _raise_if_incomplete(ws, "linear_backward")
+    return dX, dW, db
+
+
 def gemm_batched(A, B, batch, M, N, K, trans_a=False, trans_b=False, slices=3):
     """`batch` independent products of densely stacked matrices: A [batch, M*K], B [batch, K*N]."""
     A = _check(A, batch * M * K, "A")

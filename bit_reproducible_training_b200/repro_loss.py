@@ -7,7 +7,7 @@ backward pass forms the probabilities of one piece of words at a time.  ``layers
 import torch
 
 from . import _lib
-from .repro_gemm import ReproGemmError, _addr, _check, _on, _raw_stream, cudaSuccess
+from .repro_gemm import ReproGemmError, _addr, _check, _on, _raise_if_incomplete, _raw_stream, cudaSuccess
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
@@ -52,6 +52,7 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean",
                                                    _addr(nll), _addr(lse), _addr(target_logit), _addr(ws), ws.numel(), _raw_stream(x.device))
     if rc != cudaSuccess:
         raise ReproGemmError(rc, "linear_xent_forward")
+    _raise_if_incomplete(ws, "linear_cross_entropy")
     return (nll.view(shape) if loss is None else loss), lse, target_logit
 
 
@@ -74,4 +75,5 @@ def linear_cross_entropy_backward(dloss, x, weight, target, lse, target_logit, i
                                                     _addr(target_logit), _addr(dloss), _addr(dx), _addr(dw), _addr(ws), ws.numel(), _raw_stream(x.device))
     if rc != cudaSuccess:
         raise ReproGemmError(rc, "linear_xent_backward")
+    _raise_if_incomplete(ws, "linear_cross_entropy_backward")
     return dx, dw

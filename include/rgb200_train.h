@@ -3,7 +3,8 @@
  *
  * Same conventions as rgb200.h: plain device pointers and sizes, all work enqueued on the stream that is passed in (a
  * cudaStream_t cast to void*), nothing allocated, nothing kept between calls, cudaError_t codes as int
- * (0 = success, 1 = cudaErrorInvalidValue, 801 = cudaErrorNotSupported).  Sums of floats are taken in an order that depends
+ * (0 = success, 1 = cudaErrorInvalidValue, 801 = cudaErrorNotSupported).  Calls that contain products report an expired bounded
+ * wait through their workspace: rgb200_workspace_status reads it.  Sums of floats are taken in an order that depends
  * on the sizes alone, so the output bits depend on the inputs and the sizes, not on the stream, the call or the GPU.
  */
 #ifndef RGB200_TRAIN_H
@@ -40,6 +41,12 @@ int rgb200_gemm_epilogue_fp32_ws(const float* A, const float* B, float* C, int M
 size_t rgb200_activation_backward_workspace(int M, int N);
 int rgb200_activation_backward(const float* dY, const float* Z, float* dZ, float* db, int M, int N, int activation, void* workspace,
                                size_t workspace_bytes, void* stream);
+/* The whole backward pass of Y = act(X W^T + bias) (+ residual, whose gradient is dY): with dZ = dY act'(Z), dX [M, K] = dZ W,
+ * dW [N, K] = dZ^T X and db [N] = column sums of dZ; each of the three may be NULL.  The products are those of rgb200_gemm_fp32_ws
+ * on dZ, bit for bit; dZ's digits for both come from one pass over it.  Workspace: 256-byte aligned; 0 bytes: sizes not supported. */
+size_t rgb200_linear_backward_workspace(int M, int N, int K, int activation, int slices);
+int rgb200_linear_backward(const float* dY, const float* Z, const float* X, const float* W, float* dX, float* dW, float* db, int M, int N, int K,
+                           int activation, int slices, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Cross entropy of the logits X W^T against targets, in pieces of the vocabulary: the [N, V] logits are never stored.

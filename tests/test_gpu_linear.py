@@ -190,6 +190,39 @@ def test_layer_gradients(act, bias, residual):
         assert torch.equal(grads[id(r)], dy)
 
 
+@pytest.mark.parametrize("slices", [1, 2, 3])
+@pytest.mark.parametrize("act", [None, "gelu"])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (3, 5, 7), (64, 64, 64), (100, 33, 48), (127, 130, 65), (128, 128, 200), (129, 260, 70), (300, 1001, 33), (1000, 64, 1500),
+                                   (40, 3000, 50), (5000, 40, 60)])
+def test_whole_backward_pass(m, n, k, act, slices):
+    """dX and dW have the bits of the plain products on dZ, whichever of the three gradients are asked for."""
+    x, w, _, z, dy = operands(m, n, k)
+    dz, db = rg.activation_backward(dy, z, m, n, act, True, True)
+    want = rg.gemm(dz, w, m, k, n, False, False, slices), rg.gemm(dz, x, n, k, m, True, False, slices), db
+    for asked in ((True, True, True), (True, True, False), (True, False, True), (False, True, False), (False, False, True)):
+        got = rg.linear_backward(dy, z, x, w, m, n, k, act, slices, *asked)
+        for g, t, a in zip(got, want, asked):
+            assert (g is None) != a and (not a or torch.equal(g, t)), asked
+    flat = torch.empty(m * n + 1, device="cuda")
+    flat[1:] = dy.view(-1)
+    for g, t in zip(rg.linear_backward(flat[1:], z, x, w, m, n, k, act, slices, True, True, True), want):
+        assert torch.equal(g, t)
+
+
+def test_backward_of_wide_range_gradients():
+    """Rows and columns of very different magnitudes, zeros, subnormals: the exponents of the one-pass split are the plain ones."""
+    m, n, k = 150, 200, 40
+    g = fx.Rng(7)
+    dy = torch.from_numpy(g.wide(m * n, -100, 60)).cuda().view(m, n)
+    dy[3] = 0
+    dy[:, 5] = 0
+    dy[7] *= 1e-30
+    dy[:, 11] = 1e-42
+    x, w, _, _, _ = operands(m, n, k)
+    dx, dw, _ = rg.linear_backward(dy, None, x, w, m, n, k)
+    assert torch.equal(dx, rg.gemm(dy, w, m, k, n)) and torch.equal(dw, rg.gemm(dy, x, n, k, m, True, False))
+
+
 def test_gradients_against_differences():
     """The derivative along a direction by the 64-bit formula's central difference.  dX and dW are S = 3 products: each operand is off
     by at most 2^-21 of its row's largest magnitude, so a product of length L is off by at most L 2^-20 of the two largest magnitudes."""
@@ -244,6 +277,13 @@ def test_refusals():
         rg.gemm_epilogue(x, w, 8, 16, 24, False, True, out=torch.empty(8, 15, device="cuda"))
 
 
+def test_status_is_read_after_the_calls(monkeypatch):
+    monkeypatch.setenv("RGB200_CHECK_STATUS", "1")
+    x, w, b, r, dy = operands(50, 60, 70)
+    rg.gemm_epilogue(x, w, 50, 60, 70, False, True, bias=b)
+    rg.linear_backward(dy, r, x, w, 50, 60, 70, "silu", want_db=True)
+
+
 def test_two_graphs_at_once_and_other_streams():
     m, n, k = 300, 200, 400
     x, w, b, r, dy = operands(m, n, k)
@@ -251,7 +291,7 @@ def test_two_graphs_at_once_and_other_streams():
     def once():
         y, z = rg.gemm_epilogue(x, w, m, n, k, False, True, bias=b, activation="gelu", residual=r, keep_pre=True)
         dz, db = rg.activation_backward(dy, z, m, n, "gelu", True, True)
-        return y, z, dz, db, rg.gemm(dz, x, n, k, m, True, False)
+        return (y, z, dz, db) + rg.linear_backward(dy, z, x, w, m, n, k, "gelu", 3, True, True, True)
 
     want = once()
     torch.cuda.synchronize()

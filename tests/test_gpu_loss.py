@@ -219,6 +219,12 @@ def test_other_slice_counts():
         layers.set_slices(3)
 
 
+def test_status_is_read_after_the_calls(monkeypatch):
+    monkeypatch.setenv("RGB200_CHECK_STATUS", "1")
+    x, w, t = case(100, 32, 20000)
+    torch.autograd.grad(layers.linear_cross_entropy(x, w, t), [x, w])
+
+
 def test_runs_repeat_on_streams_and_in_graphs_at_once():
     x, w, t = case(600, 96, 5000)
     x, w = x.detach(), w.detach()
