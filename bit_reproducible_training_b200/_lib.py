@@ -105,8 +105,8 @@ def lib():
     L.rgb200_linear_backward.argtypes = [fp, fp, fp, fp, fp, fp, fp, i, i, i, i, i, vp, C.c_size_t, vp]
     L.rgb200_linear_xent_workspace.argtypes = [i, i, i, i, i]
     L.rgb200_linear_xent_workspace.restype = C.c_size_t
-    L.rgb200_linear_xent_forward.argtypes = [fp, fp, vp, ll, i, i, i, i, i, fp, fp, fp, fp, vp, C.c_size_t, vp]
-    L.rgb200_linear_xent_backward.argtypes = [fp, fp, vp, ll, i, i, i, i, i, fp, fp, fp, fp, fp, vp, C.c_size_t, vp]
+    L.rgb200_linear_xent_forward.argtypes = [fp, fp, vp, ll, i, i, i, i, i, fp, fp, fp, fp, fp, vp, C.c_size_t, vp]
+    L.rgb200_linear_xent_backward.argtypes = [fp, fp, vp, ll, i, i, i, i, i, fp, fp, fp, fp, fp, fp, vp, C.c_size_t, vp]
     L.rgb200_block_norm_forward.argtypes = [C.POINTER(BlockNorm), vp]
     L.rgb200_block_norm_backward_workspace.argtypes = [i, i, i]
     L.rgb200_block_norm_backward_workspace.restype = C.c_size_t

@@ -10,6 +10,7 @@ import os
 import re
 import shutil
 import subprocess
+import time
 from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -46,8 +47,16 @@ def _newer(target, inputs):
     return not os.path.exists(target) or any(os.path.getmtime(f) > os.path.getmtime(target) for f in inputs)
 
 
+def _object(src):
+    return os.path.join(OBJ, src[:-3] + ".o")
+
+
 def stale():
-    return any(_newer(LIB, _inputs(os.path.join(CSRC, src))) for src in SOURCES)
+    for src in SOURCES:
+        inputs, obj = _inputs(os.path.join(CSRC, src)), _object(src)
+        if _newer(LIB, inputs) or (os.path.exists(obj) and _newer(obj, inputs)):
+            return True
+    return False
 
 
 def build(force=False, verbose=False):
@@ -66,9 +75,11 @@ def build(force=False, verbose=False):
             print(res.stderr)
 
     def compile_one(src):
-        obj = os.path.join(OBJ, src[:-3] + ".o")
+        obj = _object(src)
         if force or _newer(obj, _inputs(os.path.join(CSRC, src))):
+            began = time.time()
             run([nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-c", "-o", obj, src])
+            os.utime(obj, (began, began))       # an input edited while the compiler ran makes the object old
         return obj
 
     with ThreadPoolExecutor(len(SOURCES)) as pool:

@@ -29,7 +29,7 @@ cudaError_t launch(int grid, const CUtensorMap& a, const CUtensorMap& b, const G
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     std::call_once(once[dev], [&] { err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, epilogue_smem<S>()); });
     if (err[dev] != cudaSuccess) return err[dev];
-    kernel<<<grid, GEMM_THREADS, epilogue_smem<S>(), st>>>(a, b, P);
+    kernel<<<grid, gemm_threads(EPI), epilogue_smem<S>(), st>>>(a, b, P);
     return cudaGetLastError();
 }
 

@@ -20,6 +20,13 @@ constexpr int ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_T
 // 2 sqrt(2 / pi), and that times 0.044715; gelu_tanh(z) = z / (1 + exp(-(G1 z + G3 z^3))), which is 0.5 z (1 + tanh(half of it)) without
 // the cancellation of 1 + tanh on the negative side.
 constexpr float GELU_G1 = 1.5957691216057308f, GELU_G3 = 0.0713548162726009f;
+// The same for a power of two, log2(e) folded into the constants: exp(-t) = 2^(-t log2 e), one multiplication and rounding less.
+constexpr float GELU_L1 = 2.302208198f, GELU_L3 = 0.102943240f;
+__device__ __forceinline__ float exp2_fast(float x) {           // within 2 ulp
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 constexpr float SQRT_HALF = 0.7071067811865476f, INV_SQRT_2PI = 0.3989422804014327f;
 
 template <int ACT>
@@ -27,7 +34,7 @@ __device__ __forceinline__ float activation(float z) {
     if (ACT == ACT_RELU) return z <= 0.0f ? 0.0f : z;
     if (ACT == ACT_SILU) return z / (1.0f + expf(-z));
     if (ACT == ACT_GELU) return 0.5f * z * (1.0f + erff(z * SQRT_HALF));
-    if (ACT == ACT_GELU_TANH) return z / (1.0f + expf(-z * (GELU_G1 + GELU_G3 * (z * z))));
+    if (ACT == ACT_GELU_TANH) return z / (1.0f + exp2_fast(-z * (GELU_L1 + GELU_L3 * (z * z))));
     return z;
 }
 
@@ -41,7 +48,7 @@ __device__ __forceinline__ float activation_slope(float z) {
     }
     if (ACT == ACT_GELU) return 0.5f * (1.0f + erff(z * SQRT_HALF)) + z * (expf(-0.5f * (z * z)) * INV_SQRT_2PI);
     if (ACT == ACT_GELU_TANH) {
-        const float q = z * z, p = 1.0f / (1.0f + expf(-z * (GELU_G1 + GELU_G3 * q)));
+        const float q = z * z, p = 1.0f / (1.0f + exp2_fast(-z * (GELU_L1 + GELU_L3 * q)));
         return p + (p * (1.0f - p)) * (z * (GELU_G1 + 3.0f * GELU_G3 * q));
     }
     return 1.0f;
@@ -185,7 +192,7 @@ struct EpilogueRow<EPI_PROB, CPT> {
             values(j, p);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {          // a row without a weight takes no part, whatever its logits are
-                p[i] = j + i == target || scale == 0.0f || col0 + j + i >= P.N ? 0.0f : expf(p[i] - lse) * scale;
+                p[i] = j + i == target || scale == 0.0f || col0 + j + i >= P.N ? 0.0f : __expf(p[i] - lse) * scale;
                 row_top = fmaxf(row_top, fabsf(p[i]));
             }
             if (P.epi.col_max) {                   // rows that do not exist have no weight and join as zeros
@@ -282,45 +289,58 @@ activation_backward_kernel(const ActBackwardParams P) {
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, top[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     with_activation(P.act, [&](auto act) {
         constexpr int ACT = decltype(act)::value;
-#pragma unroll 4
-        for (int row = first + warp; row < end; row += ACTB_WARPS) {
-            const size_t at = (size_t)row * P.N;
-            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f}, z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (wide) {
-                if (col[0] < P.N) {
-                    const float4 q = *reinterpret_cast<const float4*>(P.dy + at + col[0]);
-                    d[0] = q.x; d[1] = q.y; d[2] = q.z; d[3] = q.w;
-                    if (ACT != ACT_NONE) {
-                        const float4 t = *reinterpret_cast<const float4*>(P.z + at + col[0]);
-                        z[0] = t.x; z[1] = t.y; z[2] = t.z; z[3] = t.w;
-                    }
-                }
-            } else {
+        constexpr int BATCH = 4;            // rows whose loads are in flight together (dZ may be dY, so none moves over a store)
+        for (int row0 = first + warp; row0 < end; row0 += BATCH * ACTB_WARPS) {
+            float d[BATCH][4], z[BATCH][4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (col[j] < P.N) {
-                        d[j] = P.dy[at + col[j]];
-                        if (ACT != ACT_NONE) z[j] = P.z[at + col[j]];
-                    }
-            }
+            for (int i = 0; i < BATCH; ++i) {
+                const int row = row0 + i * ACTB_WARPS;
+                const size_t at = (size_t)row * P.N;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (ACT != ACT_NONE) d[j] = d[j] * activation_slope<ACT>(z[j]);
-                s[j] += d[j];
-                top[j] = fmaxf(top[j], fabsf(d[j]));
-            }
-            if (P.row_max) {
-                const float m = fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fmaxf(fabsf(d[3]), 0.0f)));
-                const unsigned all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m));
-                if (lane == 0) atomicMax(P.row_max + row, all);
-            }
-            if (P.dz) {
+                for (int j = 0; j < 4; ++j) d[i][j] = z[i][j] = 0.0f;
+                if (row >= end) continue;
                 if (wide) {
-                    if (col[0] < P.N) *reinterpret_cast<float4*>(P.dz + at + col[0]) = make_float4(d[0], d[1], d[2], d[3]);
+                    if (col[0] < P.N) {
+                        const float4 q = *reinterpret_cast<const float4*>(P.dy + at + col[0]);
+                        d[i][0] = q.x; d[i][1] = q.y; d[i][2] = q.z; d[i][3] = q.w;
+                        if (ACT != ACT_NONE) {
+                            const float4 t = *reinterpret_cast<const float4*>(P.z + at + col[0]);
+                            z[i][0] = t.x; z[i][1] = t.y; z[i][2] = t.z; z[i][3] = t.w;
+                        }
+                    }
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        if (col[j] < P.N) P.dz[at + col[j]] = d[j];
+                        if (col[j] < P.N) {
+                            d[i][j] = P.dy[at + col[j]];
+                            if (ACT != ACT_NONE) z[i][j] = P.z[at + col[j]];
+                        }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const int row = row0 + i * ACTB_WARPS;
+                if (row >= end) break;                              // uniform over the warp
+                const size_t at = (size_t)row * P.N;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (ACT != ACT_NONE) d[i][j] = d[i][j] * activation_slope<ACT>(z[i][j]);
+                    s[j] += d[i][j];
+                    top[j] = fmaxf(top[j], fabsf(d[i][j]));
+                }
+                if (P.dz) {
+                    if (wide) {
+                        if (col[0] < P.N) *reinterpret_cast<float4*>(P.dz + at + col[0]) = make_float4(d[i][0], d[i][1], d[i][2], d[i][3]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (col[j] < P.N) P.dz[at + col[j]] = d[i][j];
+                    }
+                }
+                if (P.row_max) {
+                    const float m = fmaxf(fmaxf(fabsf(d[i][0]), fabsf(d[i][1])), fmaxf(fabsf(d[i][2]), fmaxf(fabsf(d[i][3]), 0.0f)));
+                    const unsigned all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m));
+                    if (lane == 0) atomicMax(P.row_max + row, all);
                 }
             }
         }

@@ -46,11 +46,27 @@ int piece_words(int vocab, int limit) {
     return w < vocab ? w : vocab;
 }
 int forward_words(int vocab) { return piece_words(vocab, 16384); }
-// P of one piece holds at most 2^26 values (256 MB) while pieces of 1024 words allow it.
-int backward_words(int rows, int vocab) {
+// Words per piece of the backward pass, a multiple of 128 (or the whole vocabulary).  P of one piece holds at most 2^26 values (256 MB)
+// while pieces of 1024 words allow it; below that the width is the one whose products fill the SMs' rounds best.  Cost in k blocks of
+// one SM's tensor pipe: rounds of tiles times k blocks for the three products, and for each piece the time of its other
+// kernels (about 30 us, 85 blocks).
+int backward_words(int rows, int vocab, int dim) {
     int limit = 8192;
     while (limit > 1024 && (long long)limit * rows > (1ll << 26)) limit /= 2;
-    return piece_words(vocab, limit);
+    if (vocab <= limit) return vocab;
+    auto up = [](long long a, long long b) { return (a + b - 1) / b; };
+    const long long row_tiles = up(rows, 128), dim_tiles = up(dim, EPI_TILE_N), row_blocks = up(rows, 128), dim_blocks = up(dim, 128);
+    auto cost = [&](long long words) {
+        return up(row_tiles * up(words, EPI_TILE_N), 148) * dim_blocks + up(row_tiles * dim_tiles, 148) * up(words, 128) +
+               up(up(words, 128) * dim_tiles, 148) * row_blocks + 85;
+    };
+    int best = limit;
+    long long best_cost = -1;
+    for (int w = limit; w >= 1024; w -= 128) {
+        const long long pieces = vocab / w, rest = vocab % w, c = pieces * cost(w) + (rest ? cost(rest) : 0);
+        if (best_cost < 0 || c < best_cost) { best = w; best_cost = c; }
+    }
+    return best;
 }
 
 struct ForwardLayout { int words; size_t status, product, product_bytes, parts, running, total; };
@@ -67,9 +83,9 @@ bool forward_layout(int N, int V, int D, int S, ForwardLayout& L) {
     return true;
 }
 
-struct BackwardLayout { int words; size_t status, maxima, weight, coefficient, inv_count, first, last, p, logits, dx, dw, total, logits_bytes, dx_bytes, dw_bytes; };
+struct BackwardLayout { int words; size_t status, listed, maxima, weight, coefficient, list, first, not_last, p, logits, dx, dw, total, logits_bytes, dx_bytes, dw_bytes; };
 bool backward_layout(int N, int V, int D, int S, BackwardLayout& L) {
-    L.words = backward_words(N, V);
+    L.words = backward_words(N, V, D);
     if (!product_bytes(N, L.words, D, S, false, true, &L.logits_bytes) || !product_bytes(N, D, L.words, S, false, false, &L.dx_bytes) ||
         !product_bytes(L.words, D, N, S, true, false, &L.dw_bytes))
         return false;
@@ -80,14 +96,15 @@ bool backward_layout(int N, int V, int D, int S, BackwardLayout& L) {
     if (b > L.dx_bytes) L.dx_bytes = b;
     if (!product_bytes(rest, D, N, S, true, false, &b)) return false;
     if (b > L.dw_bytes) L.dw_bytes = b;
-    L.status = 0;
-    L.maxima = XENT_ALIGN;
-    L.weight = L.maxima + round_up((size_t)N * 4 + (size_t)L.words * 4);
+    L.status = 0;                            // status, listed and the first piece's maxima are cleared together
+    L.listed = 4;
+    L.maxima = 8;
+    L.weight = round_up(L.maxima + (size_t)N * 4 + (size_t)L.words * 4);
     L.coefficient = L.weight + round_up((size_t)N * 4);
-    L.inv_count = L.coefficient + round_up((size_t)N * 4);
-    L.first = L.inv_count + XENT_ALIGN;
-    L.last = L.first + round_up((size_t)V * 4);
-    L.p = L.last + round_up((size_t)V * 4);
+    L.list = L.coefficient + round_up((size_t)N * 4);
+    L.first = L.list + round_up((size_t)N * 4);
+    L.not_last = L.first + (size_t)V * 4;
+    L.p = L.first + round_up((size_t)V * 8);
     L.logits = L.p + round_up((size_t)N * L.words * 4);
     L.dx = L.logits + L.logits_bytes;
     L.dw = L.dx + L.dx_bytes;
@@ -113,10 +130,10 @@ extern "C" size_t rgb200_linear_xent_workspace(int N, int V, int D, int slices, 
 }
 
 extern "C" int rgb200_linear_xent_forward(const float* X, const float* W, const long long* target, long long ignore_index, int reduction, int N, int V,
-                                          int D, int slices, float* loss, float* nll, float* lse, float* target_logit, void* workspace,
-                                          size_t workspace_bytes, void* stream) {
+                                          int D, int slices, float* loss, float* nll, float* lse, float* target_logit, float* inv_count,
+                                          void* workspace, size_t workspace_bytes, void* stream) {
     if (!good_sizes(N, V, D, slices) || !X || !W || !target || !nll || !lse || !target_logit || !workspace) return cudaErrorInvalidValue;
-    if (reduction < RGB200_REDUCE_NONE || reduction > RGB200_REDUCE_SUM || (reduction != RGB200_REDUCE_NONE && !loss)) return cudaErrorInvalidValue;
+    if (reduction < RGB200_REDUCE_NONE || reduction > RGB200_REDUCE_SUM || (reduction != RGB200_REDUCE_NONE && (!loss || !inv_count))) return cudaErrorInvalidValue;
     ForwardLayout L;
     if (!forward_layout(N, V, D, slices, L)) return cudaErrorInvalidValue;
     if (workspace_bytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & (XENT_ALIGN - 1)) != 0) return cudaErrorInvalidValue;
@@ -144,15 +161,15 @@ extern "C" int rgb200_linear_xent_forward(const float* X, const float* W, const 
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }
     if (reduction != RGB200_REDUCE_NONE)
-        xent_reduce_kernel<<<1, 1024, 0, st>>>(nll, target, ignore_index, N, reduction == RGB200_REDUCE_MEAN, loss, nullptr);
+        xent_reduce_kernel<<<1, 1024, 0, st>>>(nll, target, ignore_index, N, reduction == RGB200_REDUCE_MEAN, loss, inv_count);
     return cudaGetLastError();
 }
 
 extern "C" int rgb200_linear_xent_backward(const float* X, const float* W, const long long* target, long long ignore_index, int reduction, int N, int V,
-                                           int D, int slices, const float* lse, const float* target_logit, const float* dloss, float* dX, float* dW,
-                                           void* workspace, size_t workspace_bytes, void* stream) {
+                                           int D, int slices, const float* lse, const float* target_logit, const float* inv_count, const float* dloss,
+                                           float* dX, float* dW, void* workspace, size_t workspace_bytes, void* stream) {
     if (!good_sizes(N, V, D, slices) || !X || !W || !target || !lse || !target_logit || !dloss || (!dX && !dW) || !workspace) return cudaErrorInvalidValue;
-    if (reduction < RGB200_REDUCE_NONE || reduction > RGB200_REDUCE_SUM) return cudaErrorInvalidValue;
+    if (reduction < RGB200_REDUCE_NONE || reduction > RGB200_REDUCE_SUM || (reduction != RGB200_REDUCE_NONE && !inv_count)) return cudaErrorInvalidValue;
     BackwardLayout L;
     if (!backward_layout(N, V, D, slices, L)) return cudaErrorInvalidValue;
     if (workspace_bytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & (XENT_ALIGN - 1)) != 0) return cudaErrorInvalidValue;
@@ -162,17 +179,18 @@ extern "C" int rgb200_linear_xent_backward(const float* X, const float* W, const
     char* ws = static_cast<char*>(workspace);
     float* weight = reinterpret_cast<float*>(ws + L.weight);
     float* coefficient = reinterpret_cast<float*>(ws + L.coefficient);
-    float* inv_count = reinterpret_cast<float*>(ws + L.inv_count);
+    int* list = reinterpret_cast<int*>(ws + L.list);
+    int* listed = reinterpret_cast<int*>(ws + L.listed);
     int* first = reinterpret_cast<int*>(ws + L.first);
-    int* last = reinterpret_cast<int*>(ws + L.last);
+    int* not_last = reinterpret_cast<int*>(ws + L.not_last);
+    const bool both = dX && dW;
+    const size_t maxima_bytes = (size_t)N * 4 + (size_t)L.words * 4;
     float* P = reinterpret_cast<float*>(ws + L.p);
 
-    if ((e = cudaMemsetAsync(first, 0x7F, (size_t)V * 4, st)) != cudaSuccess) return e;      // above every row
-    if ((e = cudaMemsetAsync(last, 0xFF, (size_t)V * 4, st)) != cudaSuccess) return e;       // -1
-    if (reduction != RGB200_REDUCE_NONE)
-        xent_reduce_kernel<<<1, 1024, 0, st>>>(nullptr, target, ignore_index, N, reduction == RGB200_REDUCE_MEAN, nullptr, inv_count);
+    if ((e = cudaMemsetAsync(ws, 0, L.maxima + (both ? maxima_bytes : 0), st)) != cudaSuccess) return e;
+    if ((e = cudaMemsetAsync(first, 0x7F, (size_t)V * 8, st)) != cudaSuccess) return e;          // above every row and every complement of one
     xent_rows_kernel<<<(N + 255) / 256, 256, 0, st>>>(target, ignore_index, N, V, lse, target_logit, dloss, reduction == RGB200_REDUCE_NONE, inv_count, weight,
-                                                     coefficient, first, last);
+                                                     coefficient, first, not_last);
     if (dX) xent_target_dx_kernel<<<N, 256, 0, st>>>(target, coefficient, W, D, dX);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
 
@@ -180,7 +198,6 @@ extern "C" int rgb200_linear_xent_backward(const float* X, const float* W, const
     E.target = target; E.lse = lse; E.row_scale = weight;
     EpilogueParams add = {};
     add.residual = dX;
-    const bool both = dX && dW;
     int* status = reinterpret_cast<int*>(ws + L.status);
     for (int at = 0; at < V; at += L.words) {
         const int words = V - at < L.words ? V - at : L.words;
@@ -189,10 +206,10 @@ extern "C" int rgb200_linear_xent_backward(const float* X, const float* W, const
         if (both) {
             E.row_max = reinterpret_cast<unsigned*>(ws + L.maxima);
             E.col_max = E.row_max + N;
-            if ((e = cudaMemsetAsync(E.row_max, 0, (size_t)N * 4 + (size_t)words * 4, st)) != cudaSuccess) return e;
+            if (at > 0 && (e = cudaMemsetAsync(E.row_max, 0, maxima_bytes, st)) != cudaSuccess) return e;
         }
         if ((e = gemm_with_epilogue(X, Wp, P, N, words, D, product_config(slices, false, true), EPI_PROB, E,
-                                    Prepared{at > 0 && words == L.words, false, status, at == 0}, ws + L.logits, L.logits_bytes, st)) != cudaSuccess)
+                                    Prepared{at > 0 && words == L.words, false, status}, ws + L.logits, L.logits_bytes, st)) != cudaSuccess)
             return e;
         const rgb200_config cx = product_config(slices, false, false), cw = product_config(slices, true, false);
         if (both) {                                  // P once for both products
@@ -207,7 +224,11 @@ extern "C" int rgb200_linear_xent_backward(const float* X, const float* W, const
                       cudaSuccess)
             return e;
     }
-    if (dW)
-        xent_target_dw_kernel<<<dim3(N, (D + XENT_DW_COLS - 1) / XENT_DW_COLS), 256, 0, st>>>(target, coefficient, X, first, last, N, V, D, dW);
+    if (dW) {
+        xent_single_dw_kernel<<<(N + 7) / 8, 256, 0, st>>>(target, coefficient, X, first, not_last, N, V, D, dW, list, listed);
+        // at most N / 2 words are listed; the CTAs walk over them
+        const long long most = ((long long)N / 2) * ((D + XENT_DW_COLS - 1) / XENT_DW_COLS);
+        if (most > 0) xent_repeated_dw_kernel<<<(int)(most < 148 * 8 ? most : 148 * 8), 256, 0, st>>>(target, coefficient, X, not_last, D, dW, list, listed);
+    }
     return cudaGetLastError();
 }

@@ -42,7 +42,7 @@ xent_join_kernel(const float2* __restrict__ parts, int count, float2* running, i
 }
 
 // Sum of the rows' losses (in double, thread t adding rows t, t + 1024, ..., then a tree) over the number of rows that count.
-// loss may be null; inv_count receives 1 / max(1, rows that count) for the mean, 1 for the sum.
+// inv_count receives 1 / max(1, rows that count) for the mean, 1 for the sum.
 static __global__ void __launch_bounds__(1024)
 xent_reduce_kernel(const float* __restrict__ nll, const long long* __restrict__ target, long long ignore, int rows, bool mean, float* loss, float* inv_count) {
     __shared__ double sums[1024];
@@ -50,7 +50,7 @@ xent_reduce_kernel(const float* __restrict__ nll, const long long* __restrict__ 
     double s = 0.0;
     int n = 0;
     for (int i = threadIdx.x; i < rows; i += 1024) {
-        if (nll) s += (double)nll[i];
+        s += (double)nll[i];
         n += target[i] != ignore;
     }
     sums[threadIdx.x] = s;
@@ -65,16 +65,17 @@ xent_reduce_kernel(const float* __restrict__ nll, const long long* __restrict__ 
     }
     if (threadIdx.x != 0) return;
     const double many = mean ? (double)(counts[0] > 1 ? counts[0] : 1) : 1.0;
-    if (loss) *loss = (float)(sums[0] / many);
-    if (inv_count) *inv_count = (float)(1.0 / many);
+    *loss = (float)(sums[0] / many);
+    *inv_count = (float)(1.0 / many);
 }
 
 // Per row: weight g (the loss's gradient, over the number of rows for the mean; 0 for rows that do not count) and the target's
-// coefficient (p - 1) g; and for each word that is a target its first and last row (integer minimum and maximum: any order).
+// coefficient (p - 1) g; and for each word that is a target its first row and the complement of its last one (integer minima of words
+// that start at 0x7F7F7F7F: any order).
 static __global__ void __launch_bounds__(256)
 xent_rows_kernel(const long long* __restrict__ target, long long ignore, int rows, int vocab, const float* __restrict__ lse,
                  const float* __restrict__ target_logit, const float* __restrict__ dloss, bool per_row, const float* __restrict__ inv_count, float* weight,
-                 float* coefficient, int* first, int* last) {
+                 float* coefficient, int* first, int* not_last) {
     const int i = blockIdx.x * 256 + threadIdx.x;
     if (i >= rows) return;
     const long long t = target[i];
@@ -84,7 +85,7 @@ xent_rows_kernel(const long long* __restrict__ target, long long ignore, int row
     coefficient[i] = counts ? (expf(target_logit[i] - lse[i]) - 1.0f) * g : 0.0f;
     if (counts) {
         atomicMin(first + t, i);
-        atomicMax(last + t, i);
+        atomicMin(not_last + t, ~i);
     }
 }
 
@@ -97,43 +98,76 @@ xent_target_dx_kernel(const long long* __restrict__ target, const float* __restr
     for (int k = threadIdx.x; k < dim; k += 256) dX[(size_t)row * dim + k] = c != 0.0f ? c * w[k] : 0.0f;
 }
 
-// dW[t] += sum over the rows with target t of coefficient * x.  One CTA for each row that is its target's first, and 128 columns; its
-// eight warps take the range from the first to the last such row in eight equal stretches, each adding its rows in order, then the
-// warps' sums are added in order: the order depends on the targets alone.
-constexpr int XENT_DW_COLS = 128;
+// dW[t] += sum over the rows with target t of coefficient * x, in two kernels.  The first gives a warp to each row: it adds the row itself
+// where no other has its target, and lists it where it is the first of several (in any order: the listed words are independent).
 static __global__ void __launch_bounds__(256)
-xent_target_dw_kernel(const long long* __restrict__ target, const float* __restrict__ coefficient, const float* __restrict__ X, const int* __restrict__ first,
-                      const int* __restrict__ last, int rows, int vocab, int dim, float* dW) {
-    __shared__ float sums[8][XENT_DW_COLS];
-    const int row = blockIdx.x;
+xent_single_dw_kernel(const long long* __restrict__ target, const float* __restrict__ coefficient, const float* __restrict__ X, const int* __restrict__ first,
+                      const int* __restrict__ not_last, int rows, int vocab, int dim, float* dW, int* list, int* listed) {
+    const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= rows) return;
     const long long t = target[row];
     if (t < 0 || t >= vocab || first[t] != row) return;                     // ignored rows were never entered in first
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int stretch = (last[t] - row) / 8 + 1, begin = row + warp * stretch;
-    const int end = begin + stretch < last[t] + 1 ? begin + stretch : last[t] + 1;
-    const int col0 = blockIdx.y * XENT_DW_COLS + lane;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int base = begin; base < end; base += 32) {
-        const int i = base + lane;
-        unsigned hits = __ballot_sync(0xFFFFFFFFu, i < end && target[i] == t);
-        while (hits) {
-            const int k = base + __ffs(hits) - 1;
-            hits &= hits - 1;
-            const float c = coefficient[k];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (col0 + 32 * j < dim) s[j] += c * X[(size_t)k * dim + col0 + 32 * j];
-        }
+    if (~not_last[t] != row) {
+        if (lane == 0) list[atomicAdd(listed, 1)] = row;
+        return;
     }
+    const float c = coefficient[row];
+    const float* x = X + (size_t)row * dim;
+    float* w = dW + (size_t)t * dim;
+#pragma unroll 4
+    for (int k = lane; k < dim; k += 32) w[k] += c * x[k];
+}
+
+// The second takes the listed words, 128 columns at a time.  Its eight warps take the range from the word's first to its last row in eight
+// equal stretches, each adding its rows in order, then the warps' sums are added in order: the order depends on the targets alone.
+constexpr int XENT_DW_COLS = 128;
+static __global__ void __launch_bounds__(256)
+xent_repeated_dw_kernel(const long long* __restrict__ target, const float* __restrict__ coefficient, const float* __restrict__ X,
+                        const int* __restrict__ not_last, int dim, float* dW, const int* __restrict__ list, const int* __restrict__ listed) {
+    __shared__ float sums[8][XENT_DW_COLS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, strips = (dim + XENT_DW_COLS - 1) / XENT_DW_COLS;
+    const long long items = (long long)*listed * strips;
+    for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+        const int row = list[item / strips], strip = (int)(item % strips);
+        const long long t = target[row];
+        const int last = ~not_last[t];
+        const int stretch = (last - row) / 8 + 1, begin = row + warp * stretch;
+        const int end = begin + stretch < last + 1 ? begin + stretch : last + 1;
+        const int col0 = strip * XENT_DW_COLS + lane;
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int base = begin; base < end; base += 32) {
+            const int i = base + lane;
+            unsigned hits = __ballot_sync(0xFFFFFFFFu, i < end && target[i] == t);
+            while (hits) {                                   // four rows' loads in flight, added in order
+                float c[4], x[4][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sums[warp][lane + 32 * j] = s[j];
-    __syncthreads();
-    const int c = threadIdx.x, col = blockIdx.y * XENT_DW_COLS + c;
-    if (c >= XENT_DW_COLS || col >= dim) return;
-    float total = sums[0][c];
+                for (int i = 0; i < 4; ++i) {
+                    const bool some = hits != 0;
+                    const int k = some ? base + __ffs(hits) - 1 : row;
+                    hits &= hits - 1;
+                    c[i] = some ? coefficient[k] : 0.0f;
 #pragma unroll
-    for (int k = 1; k < 8; ++k) total += sums[k][c];
-    dW[(size_t)t * dim + col] += total;
+                    for (int j = 0; j < 4; ++j) x[i][j] = some && col0 + 32 * j < dim ? X[(size_t)k * dim + col0 + 32 * j] : 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[j] += c[i] * x[i][j];
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sums[warp][lane + 32 * j] = s[j];
+        __syncthreads();
+        const int c = threadIdx.x, col = strip * XENT_DW_COLS + c;
+        if (c < XENT_DW_COLS && col < dim) {
+            float total = sums[0][c];
+#pragma unroll
+            for (int k = 1; k < 8; ++k) total += sums[k][c];
+            dW[(size_t)t * dim + col] += total;
+        }
+        __syncthreads();
+    }
 }
 
 }  // namespace rgb200

@@ -41,6 +41,11 @@ constexpr int BLOCK_K = 128;         // bytes = int8 elements per pipeline stage
 constexpr int UMMA_K = 32;           // k extent of one kind::i8 MMA
 constexpr int EPI_WARPS = 8;         // two warps per TMEM lane quarter, each taking half of the tile's columns
 constexpr int EPI_THREADS = EPI_WARPS * 32;
+// The kernel with bias, activation and residual has sixteen epilogue warps: its loads and activations make a tile's epilogue longer than
+// the MMAs of a short K, and twice the warps halve each thread's chain (8192 x 4096 x 1024 with gelu: 245 -> 233 us).  The
+// plain kernel and the cross-entropy kernels gain nothing from them (8192 x 50257 x 768: 2.11 ms with eight, 2.21 with sixteen).
+RGB_HD constexpr int epilogue_warps(int epi) { return epi == 1 /* EPI_LINEAR */ ? 16 : EPI_WARPS; }
+RGB_HD constexpr int gemm_threads(int epi) { return 64 + 32 * epilogue_warps(epi); }
 constexpr int GEMM_THREADS = 64 + EPI_THREADS;   // warp 0: TMA producer, warp 1: MMA issuer + TMEM owner, then the epilogue
 constexpr long long WAIT_LIMIT_CLOCKS = 4000000000ll;   // about two seconds
 
@@ -89,7 +94,7 @@ struct EpilogueParams {
     // cross entropy: columns are words first_word .. first_word + N - 1 of the vocabulary
     const long long* target;    // [M]
     long long first_word;
-    float2* lse_parts;          // [2 * n_tiles][M]: maximum, sum of exp(value - maximum)
+    float2* lse_parts;          // [N / 32 rounded up][M]: maximum, sum of exp(value - maximum)
     float* target_logit;        // [M]
     const float* lse;           // [M]
     const float* row_scale;     // [M]
@@ -208,10 +213,15 @@ __device__ __forceinline__ void umma_commit(uint32_t bar) {
 }
 
 // 32 lanes x 16 consecutive 32-bit columns: thread i of the warp receives row (lane base + i).
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&r)[16]) {
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, int (&r)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
                    "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, int (&r)[8]) {          // eight columns
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -364,7 +374,7 @@ struct EpilogueRow;
 // [image][column][place], see GemmParams::c_image_rows; only the FP32 store of the epilogue differs.
 // EPI: see Epilogue; the kernels with one have no INT64 output.
 template <int S, int NT, bool IMAGE_MAJOR_C = false, int EPI = EPI_NONE>
-__global__ void __launch_bounds__(GEMM_THREADS, 1)
+__global__ void __launch_bounds__(gemm_threads(EPI), 1)
 gemm_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                        const GemmParams P) {
     using Tr = GemmTraits<S, NT>;
@@ -393,7 +403,7 @@ gemm_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
         mbar_init(tmem_full_bar, 1);
-        mbar_init(tmem_empty_bar, EPI_THREADS);
+        mbar_init(tmem_empty_bar, 32 * epilogue_warps(EPI));
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -469,14 +479,16 @@ gemm_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             }
         }
     } else {
-        // ---------------------------------------------------------------- epilogue (warps 2..9)
-        constexpr int CPT = NT / 2;                    // columns per thread
-        static_assert(CPT % 16 == 0, "epilogue reads TMEM sixteen columns at a time");
+        // ---------------------------------------------------------------- epilogue (warps 2..9, or 2..17)
+        constexpr int SHARES = epilogue_warps(EPI) / 4;              // warps that share the columns of 32 rows
+        constexpr int CPT = NT / SHARES;                             // columns per thread
+        constexpr int LD = SHARES == 2 ? 16 : 8;                     // columns per TMEM read
+        static_assert(CPT % LD == 0, "epilogue reads TMEM LD columns at a time");
         // exact sums kept in registers between the TMEM drain and the rounding: one level (S = 1) fits INT32
         using TAcc = typename std::conditional<S == 1, int, long long>::type;
         static_assert(CPT * (S == 1 ? 1 : 2) <= 128, "the tile's sums must fit the register file");
         const int quarter = warp & 3;                  // TMEM lanes this warp may read: 32*quarter .. +31
-        const int half = (warp - 2) >> 2;              // which half of the tile's columns
+        const int half = (warp - 2) >> 2;              // which half (quarter) of the tile's columns
         const int row_in_tile = quarter * 32 + lane;
         uint32_t tile_it = 0;
         bool ok = true;
@@ -522,13 +534,13 @@ gemm_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * CPT;
             TAcc T[CPT];
 #pragma unroll
-            for (int c0 = 0; c0 < CPT; c0 += 16) {
-                int lv[Tr::LEVELS][16];
+            for (int c0 = 0; c0 < CPT; c0 += LD) {
+                int lv[Tr::LEVELS][LD];
 #pragma unroll
-                for (int L = 0; L < Tr::LEVELS; ++L) tmem_ld16(t_row + L * NT + c0, lv[L]);
+                for (int L = 0; L < Tr::LEVELS; ++L) tmem_ld(t_row + L * NT + c0, lv[L]);
                 tmem_ld_wait();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
+                for (int j = 0; j < LD; ++j) {
                     long long t = lv[Tr::LEVELS - 1][j];
 #pragma unroll
                     for (int L = Tr::LEVELS - 2; L >= 0; --L)
@@ -544,7 +556,7 @@ gemm_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                 const int e_row = ea + P.e0;
                 const float row_scale = plain_range ? pow2f(e_row) : 0.0f;
                 // outputs j .. j + 7 of the row, each rounded once to FP32
-                epi_row.finish(P, row, row_ok, col0, tc.n_blk * 2 + half, col_slots + (warp - 2) * CPT, [&](int j, float (&v)[8]) {
+                epi_row.finish(P, row, row_ok, col0, tc.n_blk * SHARES + half, col_slots + (warp - 2) * CPT, [&](int j, float (&v)[8]) {
                     if (plain_range) {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(__fmul_rn(sum_to_float(T[j + i]), row_scale), scale_s[j + i]);

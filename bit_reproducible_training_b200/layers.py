@@ -231,16 +231,16 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction):
-        loss, lse, target_logit = rl.linear_cross_entropy(x, weight, target, ignore_index, reduction, _slices)
-        ctx.save_for_backward(x, weight, target, lse, target_logit)
+        loss, stats = rl.linear_cross_entropy(x, weight, target, ignore_index, reduction, _slices)
+        ctx.save_for_backward(x, weight, target, stats)
         ctx.how = (ignore_index, reduction, _slices)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
-        x, weight, target, lse, target_logit = ctx.saved_tensors
-        dx, dw = rl.linear_cross_entropy_backward(dloss, x, weight, target, lse, target_logit, *ctx.how, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        x, weight, target, stats = ctx.saved_tensors
+        dx, dw = rl.linear_cross_entropy_backward(dloss, x, weight, target, stats, *ctx.how, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
         return dx, dw, None, None, None
 
 

@@ -36,43 +36,46 @@ def _workspace(n, v, d, slices, backward, device):
 
 
 def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean", slices=3):
-    """(loss, lse, target_logit).  x [..., dim], weight [vocabulary, dim], target [...] int64.
+    """(loss, stats).  x [..., dim], weight [vocabulary, dim], target [...] int64.
 
     loss: a scalar ("mean" over the rows whose target is not ignore_index, at least 1; or "sum"), or with "none" the rows'
-    losses: 0 where the target is ignore_index and NaN, without a gradient, where it is outside the vocabulary otherwise."""
+    losses: 0 where the target is ignore_index and NaN, without a gradient, where it is outside the vocabulary otherwise.
+    stats: float32 [2 n + 1] for the backward call, the rows' log-sum-exp and target logits and the weight of a row."""
     n, v, d = _sizes(x, weight, target, reduction, slices)
     shape = target.shape
     x, weight, target = _check(x, n * d, "x"), _check(weight, v * d, "weight"), target.contiguous()
-    out = torch.empty((3, n), dtype=torch.float32, device=x.device)
-    nll, lse, target_logit = out[0], out[1], out[2]
+    stats = torch.empty(2 * n + 1, dtype=torch.float32, device=x.device)
+    nll = torch.empty(shape, dtype=torch.float32, device=x.device)
     loss = torch.empty((), dtype=torch.float32, device=x.device) if reduction != "none" else None
+    at = stats.data_ptr()
     with _on(x.device):
         ws = _workspace(n, v, d, slices, 0, x.device)
         rc = _lib.lib().rgb200_linear_xent_forward(_addr(x), _addr(weight), _addr(target), ignore_index, REDUCTIONS[reduction], n, v, d, slices, _addr(loss),
-                                                   _addr(nll), _addr(lse), _addr(target_logit), _addr(ws), ws.numel(), _raw_stream(x.device))
+                                                   _addr(nll), at, at + 4 * n, at + 8 * n, _addr(ws), ws.numel(), _raw_stream(x.device))
     if rc != cudaSuccess:
         raise ReproGemmError(rc, "linear_xent_forward")
     _raise_if_incomplete(ws, "linear_cross_entropy")
-    return (nll.view(shape) if loss is None else loss), lse, target_logit
+    return (nll if loss is None else loss), stats
 
 
-def linear_cross_entropy_backward(dloss, x, weight, target, lse, target_logit, ignore_index=-100, reduction="mean", slices=3, want_dx=True, want_dw=True):
-    """(dx, dweight) from the loss's gradient (a scalar, or one value a row with reduction "none") and what the forward call returned."""
+def linear_cross_entropy_backward(dloss, x, weight, target, stats, ignore_index=-100, reduction="mean", slices=3, want_dx=True, want_dw=True):
+    """(dx, dweight) from the loss's gradient (a scalar, or one value a row with reduction "none") and the forward call's stats."""
     n, v, d = _sizes(x, weight, target, reduction, slices)
     shape = x.shape
     x, weight, target = _check(x, n * d, "x"), _check(weight, v * d, "weight"), target.contiguous()
-    lse, target_logit = _check(lse, n, "lse"), _check(target_logit, n, "target_logit")
+    stats = _check(stats, 2 * n + 1, "stats")
     dloss = _check(dloss, n if reduction == "none" else 1, "dloss")
-    if any(t.device != x.device for t in (dloss, lse, target_logit)):
+    if dloss.device != x.device or stats.device != x.device:
         raise ValueError("all tensors must be on one device")
-    dx = torch.empty(shape, dtype=torch.float32, device=x.device) if want_dx else None
-    dw = torch.empty((v, d), dtype=torch.float32, device=x.device) if want_dw else None
     if not (want_dx or want_dw):
         return None, None
+    dx = torch.empty(shape, dtype=torch.float32, device=x.device) if want_dx else None
+    dw = torch.empty((v, d), dtype=torch.float32, device=x.device) if want_dw else None
+    at = stats.data_ptr()
     with _on(x.device):
         ws = _workspace(n, v, d, slices, 1, x.device)
-        rc = _lib.lib().rgb200_linear_xent_backward(_addr(x), _addr(weight), _addr(target), ignore_index, REDUCTIONS[reduction], n, v, d, slices, _addr(lse),
-                                                    _addr(target_logit), _addr(dloss), _addr(dx), _addr(dw), _addr(ws), ws.numel(), _raw_stream(x.device))
+        rc = _lib.lib().rgb200_linear_xent_backward(_addr(x), _addr(weight), _addr(target), ignore_index, REDUCTIONS[reduction], n, v, d, slices, at, at + 4 * n,
+                                                    at + 8 * n, _addr(dloss), _addr(dx), _addr(dw), _addr(ws), ws.numel(), _raw_stream(x.device))
     if rc != cudaSuccess:
         raise ReproGemmError(rc, "linear_xent_backward")
     _raise_if_incomplete(ws, "linear_cross_entropy_backward")

@@ -231,8 +231,8 @@ def test_runs_repeat_on_streams_and_in_graphs_at_once():
     up = torch.tensor(1.0, device="cuda")
 
     def once():
-        loss, lse, tl = repro_loss.linear_cross_entropy(x, w, t)
-        return (loss, lse) + repro_loss.linear_cross_entropy_backward(up, x, w, t, lse, tl)
+        loss, stats = repro_loss.linear_cross_entropy(x, w, t)
+        return (loss,) + repro_loss.linear_cross_entropy_backward(up, x, w, t, stats)
 
     want = once()
     torch.cuda.synchronize()

@@ -12,20 +12,20 @@ HERE = 1 << 20            # an address that is never followed: every call here i
 
 
 def forward(**kw):
-    a = dict(X=HERE, W=HERE, target=HERE, ignore=-100, reduction=1, N=4, V=10, D=8, S=3, loss=HERE, nll=HERE, lse=HERE, tl=HERE, ws=HERE, size=1 << 40)
+    a = dict(X=HERE, W=HERE, target=HERE, ignore=-100, reduction=1, N=4, V=10, D=8, S=3, loss=HERE, nll=HERE, lse=HERE, tl=HERE, inv=HERE, ws=HERE, size=1 << 40)
     a.update(kw)
     return _lib.lib().rgb200_linear_xent_forward(*a.values(), None)
 
 
 def backward(**kw):
-    a = dict(X=HERE, W=HERE, target=HERE, ignore=-100, reduction=1, N=4, V=10, D=8, S=3, lse=HERE, tl=HERE, dloss=HERE, dX=HERE, dW=HERE, ws=HERE, size=1 << 40)
+    a = dict(X=HERE, W=HERE, target=HERE, ignore=-100, reduction=1, N=4, V=10, D=8, S=3, lse=HERE, tl=HERE, inv=HERE, dloss=HERE, dX=HERE, dW=HERE, ws=HERE, size=1 << 40)
     a.update(kw)
     return _lib.lib().rgb200_linear_xent_backward(*a.values(), None)
 
 
 @needs_lib
 @pytest.mark.parametrize("bad", [dict(X=None), dict(W=None), dict(target=None), dict(N=0), dict(V=0), dict(D=0), dict(S=0), dict(S=4), dict(D=200000), dict(reduction=3),
-                                 dict(reduction=-1), dict(ws=None), dict(ws=HERE + 16), dict(size=100), dict(lse=None), dict(tl=None)], ids=str)
+                                 dict(reduction=-1), dict(ws=None), dict(ws=HERE + 16), dict(size=100), dict(lse=None), dict(tl=None), dict(inv=None)], ids=str)
 def test_both_calls_refuse(bad):
     assert forward(**bad) == 1 and backward(**bad) == 1
 
