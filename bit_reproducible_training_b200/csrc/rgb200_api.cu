@@ -398,7 +398,8 @@ void launch_kmajor(const KmajorOperand& first, const KmajorOperand& second, int 
 // One operand through the pre-pass.  k_major: element (r, k) at src[r*K + k].
 template <int S>
 void launch_split(const float* src, bool k_major, const float* given_max, uint32_t* maxbits, int8_t* planes, int* expo,
-                  int R, int K, int Kp, int batch, long long batch_stride, int* status, cudaStream_t st, bool overlap = false) {
+                  int R, int K, int Kp, int batch, long long batch_stride, int* status, cudaStream_t st, bool overlap = false,
+                  bool zero_maxima = false /* maxbits has not been zeroed: done here if it is needed */) {
     if (k_major) {
         const KmajorOperand op{src, given_max, planes, expo, R, batch_stride};
         const KmajorOperand none{nullptr, nullptr, nullptr, nullptr, 0, 0};
@@ -406,6 +407,7 @@ void launch_split(const float* src, bool k_major, const float* given_max, uint32
     } else if (try_cluster_split<S>(src, given_max, planes, expo, R, K, Kp, batch, batch_stride, status, overlap, st)) {
         // one read of the operand; the zeroed maxima words stay unused
     } else {
+        if (zero_maxima && !given_max) (void)cudaMemsetAsync(maxbits, 0, (size_t)batch * R * sizeof(uint32_t), st);   // an error shows at the launches' check
         if (given_max)
             maxima_to_bits_kernel<<<ceil_div(batch * R, 256), 256, 0, st>>>(given_max, maxbits, batch * R);
         else
@@ -521,14 +523,14 @@ cudaError_t run(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
         if ((e = a.hook->launch(a.hook->ctx, L, max_a, max_b, qa, qb, ea, eb, a.st)) != cudaSuccess) return e;
         record(1);
     } else if (a.reuse_a) {
-        // A's planes are in place; B's may be too (the status word then keeps the value of the call that left them)
-        if (!a.reuse_b && !both_kmajor && (e = cudaMemsetAsync(a.ws, 0, L.zero_b_bytes, a.st)) != cudaSuccess) return e;
+        // A's planes are in place; B's may be too.  The status word is the caller's, or is cleared with B's split.
+        if (!a.status && !a.reuse_b && !both_kmajor && (e = cudaMemsetAsync(status, 0, sizeof(int), a.st)) != cudaSuccess) return e;
         record(0);
         if (!a.reuse_b && both_kmajor) {
             const KmajorOperand opb{a.B, a.max_b, qb, eb, L.N, a.stride_b}, none{nullptr, nullptr, nullptr, nullptr, 0, 0};
             launch_kmajor<S>(opb, none, L.K, L.Kp, L.batch, clear_status, a.st);
         } else if (!a.reuse_b) {
-            launch_split<S>(a.B, a.trans_b, a.max_b, max_b, qb, eb, L.N, L.K, L.Kp, L.batch, a.stride_b, status, a.st);
+            launch_split<S>(a.B, a.trans_b, a.max_b, max_b, qb, eb, L.N, L.K, L.Kp, L.batch, a.stride_b, status, a.st, false, true);
         }
         record(1);
     } else if (a.reuse_b) {

@@ -45,14 +45,24 @@ int piece_words(int vocab, int limit) {
     const int w = ((vocab + pieces - 1) / pieces + 63) / 64 * 64;
     return w < vocab ? w : vocab;
 }
-int forward_words(int vocab) { return piece_words(vocab, 16384); }
-// Words per piece of the backward pass, a multiple of 128 (or the whole vocabulary).  P of one piece holds at most 2^26 values (256 MB)
-// while pieces of 1024 words allow it; below that the width is the one whose products fill the SMs' rounds best.  Cost in k blocks of
-// one SM's tensor pipe: rounds of tiles times k blocks for the three products, and for each piece the time of its other
-// kernels (about 30 us, 85 blocks).
+// Few launches and bounded buffers: a piece's digit planes of W stay near 100 MB a copy (2^25 values), the forward pass's statistics below
+// 64 MB (2^28 values of logits).
+int bounded_words(long long most, int dim) {
+    long long w = (1ll << 25) / dim;
+    if (w > most) w = most;
+    if (w > 65536) w = 65536;
+    return w < 1024 ? 1024 : (int)(w / 128 * 128);
+}
+int forward_words(int rows, int vocab, int dim) { return piece_words(vocab, bounded_words((1ll << 28) / rows, dim)); }
+// Words per piece of the backward pass, a multiple of 128 (or the whole vocabulary).  P of one piece holds at most 2^25 values, or up to
+// 2^26 in pieces of up to 8192 words, while pieces of 1024 words allow it; below that the width is the one whose products fill the
+// SMs' rounds best.  Cost in k blocks of one SM's tensor pipe: rounds of tiles times k blocks for the three products, and for each
+// piece the time of its other kernels (about 30 us, 85 blocks).  8 rows of 256 against 50000 words: 568 us in pieces of at most
+// 8192 words, most of it launches, 251 us in one.
 int backward_words(int rows, int vocab, int dim) {
-    int limit = 8192;
-    while (limit > 1024 && (long long)limit * rows > (1ll << 26)) limit /= 2;
+    long long most = (1ll << 26) / rows;
+    if (most > 8192) most = (1ll << 25) / rows > 8192 ? (1ll << 25) / rows : 8192;
+    const int limit = bounded_words(most, dim);
     if (vocab <= limit) return vocab;
     auto up = [](long long a, long long b) { return (a + b - 1) / b; };
     const long long row_tiles = up(rows, 128), dim_tiles = up(dim, EPI_TILE_N), row_blocks = up(rows, 128), dim_blocks = up(dim, 128);
@@ -62,7 +72,7 @@ int backward_words(int rows, int vocab, int dim) {
     };
     int best = limit;
     long long best_cost = -1;
-    for (int w = limit; w >= 1024; w -= 128) {
+    for (int w = limit; w >= limit / 2 && w >= 1024; w -= 128) {
         const long long pieces = vocab / w, rest = vocab % w, c = pieces * cost(w) + (rest ? cost(rest) : 0);
         if (best_cost < 0 || c < best_cost) { best = w; best_cost = c; }
     }
@@ -71,7 +81,7 @@ int backward_words(int rows, int vocab, int dim) {
 
 struct ForwardLayout { int words; size_t status, product, product_bytes, parts, running, total; };
 bool forward_layout(int N, int V, int D, int S, ForwardLayout& L) {
-    L.words = forward_words(V);
+    L.words = forward_words(N, V, D);
     size_t bytes;
     if (!product_bytes(N, L.words, D, S, false, true, &bytes)) return false;
     L.status = 0;
@@ -189,9 +199,8 @@ extern "C" int rgb200_linear_xent_backward(const float* X, const float* W, const
 
     if ((e = cudaMemsetAsync(ws, 0, L.maxima + (both ? maxima_bytes : 0), st)) != cudaSuccess) return e;
     if ((e = cudaMemsetAsync(first, 0x7F, (size_t)V * 8, st)) != cudaSuccess) return e;          // above every row and every complement of one
-    xent_rows_kernel<<<(N + 255) / 256, 256, 0, st>>>(target, ignore_index, N, V, lse, target_logit, dloss, reduction == RGB200_REDUCE_NONE, inv_count, weight,
-                                                     coefficient, first, not_last);
-    if (dX) xent_target_dx_kernel<<<N, 256, 0, st>>>(target, coefficient, W, D, dX);
+    xent_rows_kernel<<<N, 128, 0, st>>>(target, ignore_index, V, D, lse, target_logit, dloss, reduction == RGB200_REDUCE_NONE, inv_count, W, weight, coefficient,
+                                        first, not_last, dX);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
 
     EpilogueParams E = {};

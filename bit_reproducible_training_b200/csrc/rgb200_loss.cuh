@@ -69,33 +69,30 @@ xent_reduce_kernel(const float* __restrict__ nll, const long long* __restrict__ 
     *inv_count = (float)(1.0 / many);
 }
 
-// Per row: weight g (the loss's gradient, over the number of rows for the mean; 0 for rows that do not count) and the target's
-// coefficient (p - 1) g; and for each word that is a target its first row and the complement of its last one (integer minima of words
-// that start at 0x7F7F7F7F: any order).
-static __global__ void __launch_bounds__(256)
-xent_rows_kernel(const long long* __restrict__ target, long long ignore, int rows, int vocab, const float* __restrict__ lse,
-                 const float* __restrict__ target_logit, const float* __restrict__ dloss, bool per_row, const float* __restrict__ inv_count, float* weight,
-                 float* coefficient, int* first, int* not_last) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows) return;
+// One CTA a row: the row's weight g (the loss's gradient, over the number of rows for the mean; 0 for rows that do not count) and its
+// target's coefficient (p - 1) g; for the target word its first row and the complement of its last one (integer minima of words
+// that start at 0x7F7F7F7F: any order); and dX's start, coefficient times the target's row of W, to which the pieces' products are added.
+static __global__ void __launch_bounds__(128)
+xent_rows_kernel(const long long* __restrict__ target, long long ignore, int vocab, int dim, const float* __restrict__ lse,
+                 const float* __restrict__ target_logit, const float* __restrict__ dloss, bool per_row, const float* __restrict__ inv_count,
+                 const float* __restrict__ W, float* weight, float* coefficient, int* first, int* not_last, float* dX) {
+    const int i = blockIdx.x;
     const long long t = target[i];
     const bool counts = t != ignore && t >= 0 && t < vocab;
     const float g = counts ? (per_row ? dloss[i] : dloss[0] * *inv_count) : 0.0f;
-    weight[i] = g;
-    coefficient[i] = counts ? (expf(target_logit[i] - lse[i]) - 1.0f) * g : 0.0f;
-    if (counts) {
-        atomicMin(first + t, i);
-        atomicMin(not_last + t, ~i);
+    const float c = counts ? (expf(target_logit[i] - lse[i]) - 1.0f) * g : 0.0f;
+    if (threadIdx.x == 0) {
+        weight[i] = g;
+        coefficient[i] = c;
+        if (counts) {
+            atomicMin(first + t, i);
+            atomicMin(not_last + t, ~i);
+        }
     }
-}
-
-// dX's start: coefficient times the target's row of W (0 for rows that do not count); the pieces' products are added to it.
-static __global__ void __launch_bounds__(256)
-xent_target_dx_kernel(const long long* __restrict__ target, const float* __restrict__ coefficient, const float* __restrict__ W, int dim, float* dX) {
-    const int row = blockIdx.x;
-    const float c = coefficient[row];
-    const float* w = W + (size_t)(c != 0.0f ? target[row] : 0) * dim;      // a non-zero coefficient has a target inside the vocabulary
-    for (int k = threadIdx.x; k < dim; k += 256) dX[(size_t)row * dim + k] = c != 0.0f ? c * w[k] : 0.0f;
+    if (!dX) return;
+    const float* w = W + (size_t)(counts ? t : 0) * dim;
+#pragma unroll 4
+    for (int k = threadIdx.x; k < dim; k += 128) dX[(size_t)i * dim + k] = c != 0.0f ? c * w[k] : 0.0f;
 }
 
 // dW[t] += sum over the rows with target t of coefficient * x, in two kernels.  The first gives a warp to each row: it adds the row itself

@@ -98,23 +98,25 @@ def linear(x, weight, bias=None, activation=None, residual=None):
 
     x [..., in], weight [out, in], bias [out], residual [..., out]; activation None, "relu", "silu", "gelu" (erf) or
     "gelu_tanh".  The bias gradient is summed in an order that depends on the sizes alone (no set_bias_grad is needed)."""
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+    xs, ws = x.shape, weight.shape
+    if len(ws) != 2 or len(xs) < 1 or xs[-1] != ws[1]:
         raise ValueError("x must be [..., in] and weight [out, in]")
-    k, n = weight.shape[1], weight.shape[0]
+    n, k = ws
+    shape = (*xs[:-1], n)
     if bias is not None and bias.shape != (n,):
         raise ValueError("bias must be [%d]" % n)
-    shape = (*x.shape[:-1], n)
     if residual is not None and residual.shape != shape:
         raise ValueError("residual must have the output's shape")
-    if min(k, n) == 0:
+    if k == 0 or n == 0:
         raise ValueError("weight must not be empty")
     rg._activation(activation)
     if x.numel() == 0:                                   # no tokens: nothing to launch, gradients of zeros
         return torch.nn.functional.linear(x, weight, bias) + (0 if residual is None else residual)
-    tensors = (x, weight, bias, residual)
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
-        return rg.gemm_epilogue(x, weight, x.numel() // k, n, k, False, True, _slices, bias, activation, residual).view(shape)
-    return _FusedLinearFn.apply(*tensors, activation)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
+                                    (residual is not None and residual.requires_grad)):
+        return _FusedLinearFn.apply(x, weight, bias, residual, activation)
+    y = rg.gemm_epilogue(x, weight, x.numel() // k, n, k, False, True, _slices, bias, activation, residual)
+    return y if len(xs) == 2 else y.view(shape)
 
 
 class FusedLinear(torch.nn.Linear):

@@ -257,7 +257,9 @@ def gemm_epilogue(A, B, M, N, K, trans_a=False, trans_b=False, slices=3, bias=No
     B = _check(B, K * N, "B")
     bias = None if bias is None else _check(bias, N, "bias")
     residual = None if residual is None else _check(residual, M * N, "residual")
-    if any(t is not None and t.device != A.device for t in (B, bias, residual, out)):
+    device = A.device
+    if B.device != device or (bias is not None and bias.device != device) or (residual is not None and residual.device != device) or \
+            (out is not None and out.device != device):
         raise ValueError("all tensors must be on one device")
     if out is not None and (out.dtype != torch.float32 or out.numel() != M * N or not out.is_contiguous()):
         raise ValueError("out must be a contiguous float32 tensor of %d elements" % (M * N))
