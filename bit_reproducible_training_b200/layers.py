@@ -1,5 +1,7 @@
 """Linear and Conv2d layers on the reproducible GEMM and convolutions: the counterparts of ``_LinearFn`` /
-``Linear`` and ``_ConvFn`` / ``Conv2d`` in the reference's repro_torch/repro_torch/layers.py:70-135.
+``Linear`` and ``_ConvFn`` / ``Conv2d`` in the reference's repro_torch/repro_torch/layers.py:70-135; and the operators around them in a
+language-model training step: ``linear`` / ``FusedLinear`` (bias, activation and residual in the product's epilogue, with their own bias
+gradient), ``block_norm`` / ``BlockNorm``, ``linear_cross_entropy`` / ``LinearCrossEntropy``.  The optimizer is repro_optim.AdamW.
 
 Forward  Y  = X W^T     gemm(x,  W, m, n, k, trans_a=False, trans_b=True)     (layers.py:85)
 Backward dX = dY W      gemm(dy, W, m, k, n, False, False)                    (layers.py:89)
@@ -74,23 +76,25 @@ class _FusedLinearFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
-        m, k, n = x.numel() // x.shape[-1], weight.shape[1], weight.shape[0]
+        x, weight = x.contiguous(), weight.contiguous()      # the copies, where there are any, serve the backward pass too
+        n, k = weight.shape
+        m = x.numel() // k
         keep = activation is not None and any(ctx.needs_input_grad[:3])
         out = rg.gemm_epilogue(x, weight, m, n, k, False, True, _slices, bias, activation, residual, keep)
         y, z = out if keep else (out, None)
         ctx.save_for_backward(x, weight, z)
-        ctx.activation, ctx.slices = activation, _slices
-        return y.view(*x.shape[:-1], n)
+        ctx.how = (m, n, k, activation, _slices)
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, z = ctx.saved_tensors
-        k, n = weight.shape[1], weight.shape[0]
-        m = x.numel() // k
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dx, dw, db = rg.linear_backward(dy, z, x, weight, m, n, k, ctx.activation, ctx.slices, need_x, need_w, need_b)
-        return None if dx is None else dx.view(x.shape), dw, db, (dy if need_r else None), None
+        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+        dx, dw, db = rg.linear_backward(dy, z, x, weight, *ctx.how, need_x, need_w, need_b)
+        if dx is not None and x.dim() != 2:
+            dx = dx.view(x.shape)
+        return dx, dw, db, (dy if need_r else None), None
 
 
 def linear(x, weight, bias=None, activation=None, residual=None):
@@ -174,6 +178,7 @@ class _BlockNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, y, weight, bias, post_weight, gate, residual_scale, kind, eps):
+        y = None if y is None else y.contiguous()
         r, h, stats = rn.block_norm(x, y, weight=weight, bias=bias, post_weight=post_weight, gate=gate, residual_scale=residual_scale,
                                     kind=kind, eps=eps, keep_stats=True)
         ctx.save_for_backward(r, y, stats, weight, bias, post_weight, gate)
@@ -233,6 +238,7 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction):
+        x, weight, target = x.contiguous(), weight.contiguous(), target.contiguous()
         loss, stats = rl.linear_cross_entropy(x, weight, target, ignore_index, reduction, _slices)
         ctx.save_for_backward(x, weight, target, stats)
         ctx.how = (ignore_index, reduction, _slices)
