@@ -15,11 +15,11 @@ namespace rgb200 {
 constexpr int DUAL_ROWS = 128, DUAL_COLS = 64, DUAL_THREADS = 256;
 
 struct DualParams {
-    const float* src;               // [R][C]
+    const float* src;               // [R][C], rows ld apart
     const uint32_t *row_max, *col_max;      // bits of the largest magnitudes
     int8_t *row_planes, *col_planes;        // [S][R][Cp], [S][C][Rp]
     int *row_expo, *col_expo;
-    int R, C, Rp, Cp;
+    int R, C, ld, Rp, Cp;
 };
 
 template <int S>
@@ -28,22 +28,28 @@ __device__ __forceinline__ void dual_words(float a, float b, float c, float d, c
     else quad_words<S, false>(a, b, c, d, q, (float)q.lim, w);
 }
 
-// grid = (Cp / 64, Rp / 128)
+// grid = (Cp / 64) * (Rp / 128), column tiles fastest
 template <int S, bool VEC>
 __global__ void __launch_bounds__(DUAL_THREADS)
 split_both_kernel(const DualParams P) {
     __shared__ __align__(16) float tile[DUAL_ROWS * DUAL_COLS];
     __shared__ int row_e[DUAL_ROWS], col_e[DUAL_COLS];
     const int t = threadIdx.x, quad = t & 15, sub = t >> 4;           // sixteen threads along a row of the tile
-    const int r0 = blockIdx.y * DUAL_ROWS, c0 = blockIdx.x * DUAL_COLS;
+    const int col_tiles = P.Cp / DUAL_COLS, row_tile = blockIdx.x / col_tiles, col_tile = blockIdx.x - row_tile * col_tiles;
+    const int r0 = row_tile * DUAL_ROWS, c0 = col_tile * DUAL_COLS;
     float4 v[8];
     const int col = c0 + quad * 4;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int row = r0 + sub + 16 * i;
-        const float* s = P.src + (size_t)row * P.C + col;
-        if (VEC) {
+        const float* s = P.src + (size_t)row * P.ld + col;
+        if (VEC) {                                       // ld is a multiple of four: the quad exists, its values behind column C do not count
             v[i] = row < P.R && col < P.C ? *reinterpret_cast<const float4*>(s) : make_float4(0.f, 0.f, 0.f, 0.f);
+            if (col + 4 > P.C) {
+                v[i].y = col + 1 < P.C ? v[i].y : 0.f;
+                v[i].z = col + 2 < P.C ? v[i].z : 0.f;
+                v[i].w = 0.f;
+            }
         } else {
             const bool in = row < P.R;
             v[i] = make_float4(in && col < P.C ? s[0] : 0.f, in && col + 1 < P.C ? s[1] : 0.f, in && col + 2 < P.C ? s[2] : 0.f, in && col + 3 < P.C ? s[3] : 0.f);
@@ -52,11 +58,11 @@ split_both_kernel(const DualParams P) {
     if (t < DUAL_ROWS) {
         const int row = r0 + t, e = row < P.R ? scale_exponent(bits_f32(P.row_max[row])) : 0;
         row_e[t] = e;
-        if (row < P.R && blockIdx.x == 0) P.row_expo[row] = e;
+        if (row < P.R && col_tile == 0) P.row_expo[row] = e;
     } else if (t < DUAL_ROWS + DUAL_COLS) {
         const int j = t - DUAL_ROWS, c = c0 + j, e = c < P.C ? scale_exponent(bits_f32(P.col_max[c])) : 0;
         col_e[j] = e;
-        if (c < P.C && blockIdx.y == 0) P.col_expo[c] = e;
+        if (c < P.C && row_tile == 0) P.col_expo[c] = e;
     }
     __syncthreads();
     const size_t row_plane = (size_t)P.R * P.Cp, col_plane = (size_t)P.C * P.Rp;

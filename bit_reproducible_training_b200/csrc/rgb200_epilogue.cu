@@ -186,7 +186,7 @@ extern "C" int rgb200_linear_backward(const float* dY, const float* Z, const flo
     if (both) {
         PlaneSlots rows, cols;
         if ((e = plane_slots(M, K, N, cx, ws + L.dx, &rows)) != cudaSuccess || (e = plane_slots(N, K, M, cw, ws + L.dw, &cols)) != cudaSuccess) return e;
-        if ((e = launch_split_both(slices, dz, M, N, P.row_max, P.col_max, rows, cols, st)) != cudaSuccess) return e;
+        if ((e = launch_split_both(slices, dz, N, M, N, P.row_max, P.col_max, rows, cols, st)) != cudaSuccess) return e;
         prepared.a = true;
     }
     const EpilogueParams none = {};

@@ -181,8 +181,8 @@ struct EpilogueRow<EPI_PROB, CPT> {
 
     template <class Values>
     __device__ __forceinline__ void finish(const GemmParams& P, int row, bool row_ok, int col0, int, const float*, Values values) {
-        float* dst = P.C + (size_t)row * P.N + col0;
-        const bool sectors = row_ok && (reinterpret_cast<uintptr_t>(dst) & 31) == 0 && col0 + CPT <= P.N;
+        float* dst = P.C + (size_t)row * P.epi.ldc + col0;
+        const bool sectors = row_ok && (reinterpret_cast<uintptr_t>(dst) & 31) == 0 && col0 + CPT <= P.epi.ldc;      // zeros behind the last word
         float row_top = 0.0f;
         unsigned col_top = 0;
         static_assert(CPT <= 32, "one column a lane");

@@ -31,9 +31,9 @@ cudaError_t plane_slots(int M, int N, int K, const rgb200_config& cfg, void* ws,
 cudaError_t gemm_with_epilogue(const float* A, const float* B, float* C, int M, int N, int K, const rgb200_config& cfg, int epi,
                                const EpilogueParams& E, Prepared prepared, void* ws, size_t ws_bytes, cudaStream_t st);
 
-// Digit planes of src [R][C] as the row-scaled operand (k along the columns) and as the column-scaled one (k along the rows),
+// Digit planes of src [R][C] (rows ld elements apart) as the row-scaled operand (k along the columns) and as the column-scaled one (k along the rows),
 // from the bits of its rows' and columns' largest magnitudes (rgb200_dual.cuh).
-cudaError_t launch_split_both(int slices, const float* src, int R, int C, const unsigned* row_max, const unsigned* col_max, const PlaneSlots& rows,
+cudaError_t launch_split_both(int slices, const float* src, int ld, int R, int C, const unsigned* row_max, const unsigned* col_max, const PlaneSlots& rows,
                               const PlaneSlots& cols, cudaStream_t st);
 
 }  // namespace rgb200

@@ -98,6 +98,7 @@ struct EpilogueParams {
     float* target_logit;        // [M]
     const float* lse;           // [M]
     const float* row_scale;     // [M]
+    int ldc;                    // elements between C's rows, at least N (EPI_PROB)
     unsigned* row_max;          // [M], [N]: the bits of the stored values' largest magnitudes are joined in (EPI_PROB; zeroed by the
     unsigned* col_max;          // caller, or null)
 };

@@ -186,6 +186,18 @@ def _workspace(nbytes, device):
     return ws
 
 
+def _scratch(nbytes, device):
+    """Workspace of one call.  Calls of several kernels that two threads issue on one stream may interleave there, so each has a tensor
+    of its own; torch's allocator gives the memory to a later call on the stream only after this one is enqueued."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _extent(*sizes):
+    """The C ABI counts rows and columns in 32 bits."""
+    if max(sizes) > 0x7FFFFFFF:
+        raise ValueError("sizes of 2^31 and more are not supported")
+
+
 class ReproGemmIncomplete(RuntimeError):
     """A kernel gave up a bounded wait and left its output incomplete; ``status`` holds the code of the wait."""
 
@@ -253,6 +265,7 @@ def gemm_epilogue(A, B, M, N, K, trans_a=False, trans_b=False, slices=3, bias=No
 
     The product is the one ``gemm`` returns, bit for bit; bias [N], activation and residual [M, N] are applied in the kernel's
     epilogue, one FP32 operation each.  out: a contiguous [M, N] tensor to write (it may be the residual)."""
+    _extent(M, N, K)
     A = _check(A, M * K, "A")
     B = _check(B, K * N, "B")
     bias = None if bias is None else _check(bias, N, "bias")
@@ -270,7 +283,7 @@ def gemm_epilogue(A, B, M, N, K, trans_a=False, trans_b=False, slices=3, bias=No
         rc = L.rgb200_make_plan(M, N, K, C.byref(cfg), C.byref(plan))
         if rc != cudaSuccess:
             raise ReproGemmError(rc, "make_plan")
-        ws = _workspace(plan.workspace_bytes, A.device)
+        ws = _scratch(plan.workspace_bytes, A.device)
         if out is None:
             out = torch.empty((M, N), dtype=torch.float32, device=A.device)
         pre = torch.empty((M, N), dtype=torch.float32, device=A.device) if keep_pre else None
@@ -287,6 +300,7 @@ def activation_backward(dY, Z, M, N, activation=None, want_dz=True, want_db=Fals
     """(dZ, db): dZ = dY * act'(Z) as [M, N] and db = column sums of dZ, summed in an order that depends on (M, N) alone.
     Without an activation dZ is dY itself and Z is not needed."""
     act = _activation(activation)
+    _extent(M, N)
     dY = _check(dY, M * N, "dY")
     if act and Z is None:
         raise ValueError("the activation's gradient needs Z")
@@ -299,7 +313,7 @@ def activation_backward(dY, Z, M, N, activation=None, want_dz=True, want_db=Fals
         return (dZ.view(M, N) if want_dz else None), None
     L = _lib.lib()
     with _on(dY.device):
-        ws = _workspace(L.rgb200_activation_backward_workspace(M, N), dY.device) if want_db else None
+        ws = _scratch(L.rgb200_activation_backward_workspace(M, N), dY.device) if want_db else None
         rc = L.rgb200_activation_backward(_addr(dY), _addr(Z), _addr(dZ) if act else None, _addr(db), M, N, act, _addr(ws),
                                           0 if ws is None else ws.numel(), _raw_stream(dY.device))
     if rc != cudaSuccess:
@@ -311,6 +325,7 @@ def linear_backward(dY, Z, X, W, M, N, K, activation=None, slices=3, want_dx=Tru
     """(dX, dW, db) of Y = act(X W^T + bias): with dZ = dY * act'(Z), dX [M, K] = dZ W, dW [N, K] = dZ^T X, db [N] = column sums
     of dZ (see activation_backward); None where not wanted.  The products have the bits of ``gemm`` on dZ."""
     act = _activation(activation)
+    _extent(M, N, K)
     dY, X, W = _check(dY, M * N, "dY"), _check(X, M * K, "X"), _check(W, N * K, "W")
     if act and Z is None:
         raise ValueError("the activation's gradient needs Z")
@@ -327,7 +342,7 @@ def linear_backward(dY, Z, X, W, M, N, K, activation=None, slices=3, want_dx=Tru
         dX = torch.empty((M, K), dtype=torch.float32, device=dY.device) if want_dx else None
         dW = torch.empty((N, K), dtype=torch.float32, device=dY.device) if want_dw else None
         db = torch.empty(N, dtype=torch.float32, device=dY.device) if want_db else None
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dY.device)
+        ws = _scratch(nbytes, dY.device)
         rc = L.rgb200_linear_backward(_addr(dY), _addr(Z), _addr(X), _addr(W), _addr(dX), _addr(dW), _addr(db), M, N, K, act, slices, _addr(ws), nbytes,
                                       _raw_stream(dY.device))
     if rc != cudaSuccess:

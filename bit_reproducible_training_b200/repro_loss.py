@@ -7,7 +7,7 @@ backward pass forms the probabilities of one piece of words at a time.  ``layers
 import torch
 
 from . import _lib
-from .repro_gemm import ReproGemmError, _addr, _check, _on, _raise_if_incomplete, _raw_stream, cudaSuccess
+from .repro_gemm import ReproGemmError, _addr, _check, _extent, _on, _raise_if_incomplete, _raw_stream, _scratch, cudaSuccess
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
@@ -25,6 +25,7 @@ def _sizes(x, weight, target, reduction, slices):
         raise ValueError("target must have the shape of x without its last dimension")
     if not (x.device == weight.device == target.device):
         raise ValueError("all tensors must be on one device")
+    _extent(target.numel(), *weight.shape)
     return target.numel(), weight.shape[0], weight.shape[1]
 
 
@@ -32,7 +33,7 @@ def _workspace(n, v, d, slices, backward, device):
     nbytes = _lib.lib().rgb200_linear_xent_workspace(n, v, d, slices, backward)
     if nbytes == 0:
         raise ValueError("sizes not supported: %d tokens, %d words, %d values a token" % (n, v, d))
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return _scratch(nbytes, device)
 
 
 def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean", slices=3):

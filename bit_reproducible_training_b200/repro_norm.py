@@ -13,7 +13,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .repro_gemm import ReproGemmError, _addr, _check, _on, _raw_stream, _workspace, cudaSuccess
+from .repro_gemm import ReproGemmError, _addr, _check, _extent, _on, _raw_stream, _scratch, cudaSuccess
 
 KINDS = {"rms": 0, "layer": 1}
 MAX_DIM = 8192
@@ -50,6 +50,7 @@ def _sizes(x, y, weight, bias, post_weight, gate, kind, eps):
         raise ValueError("post_weight and gate need y")
     if y is not None and y.shape != x.shape:
         raise ValueError("y must have the shape of x")
+    _extent(rows)
     groups = 1
     if gate is not None:
         if gate.dim() not in (1, 2) or gate.shape[-1] != dim:
@@ -107,7 +108,7 @@ def block_norm_backward(dh, dr, r, y, stats, *, weight, bias=None, post_weight=N
                   out("post_weight", post_weight is not None, dim), out("gate", gate is not None, gate_shape))
     L = _lib.lib()
     with _on(r.device):
-        ws = _workspace(L.rgb200_block_norm_backward_workspace(rows, dim, groups), r.device)
+        ws = _scratch(L.rgb200_block_norm_backward_workspace(rows, dim, groups), r.device)
         n = _lib.BlockNorm(rows, dim, groups, KINDS[kind], residual_scale, eps, _addr(r), _addr(y), _addr(weight), None, _addr(post_weight), _addr(gate),
                            _addr(r), None, _addr(stats), _addr(dr), _addr(dh), _addr(g.x), _addr(g.y), _addr(g.weight), _addr(g.bias),
                            _addr(g.post_weight), _addr(g.gate))

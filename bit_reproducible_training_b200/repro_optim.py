@@ -33,7 +33,8 @@ class AdamW(torch.optim.Optimizer):
     ``state_bits``: 32, or 8 for codes with one scale per 256 values (2.03 instead of 8 bytes of state a parameter).
     ``capturable``: steps are counted on the device, so that ``step()`` can be captured into a CUDA graph and replayed; all
     parameters must then have gradients, and the captured learning rate and other hyper-parameters stay as they were.
-    Without it a step under capture is refused.  Parameters must not overlap in memory.
+    Without it a step under capture is refused.  Parameters must not overlap in memory.  The tensors in ``state`` are updated in
+    place; to put others in their place use ``adopt`` or ``load_state_dict``.
 
     ``state_dict()`` holds the moments' values in float32 whatever ``state_bits`` is, and ``load_state_dict`` takes such a
     dict into either width (values pass through the codes again, which returns the same codes)."""
@@ -65,6 +66,15 @@ class AdamW(torch.optim.Optimizer):
         except Exception:
             self.param_groups.pop()
             raise
+
+    def __getstate__(self):
+        for index, t in self._tables.items():
+            self._steps(t)
+        return {**super().__getstate__(), "state_bits": self.state_bits, "capturable": self.capturable}
+
+    def __setstate__(self, state):
+        self._tables = {}                            # addresses of the original's tensors do not travel
+        super().__setstate__(state)
 
     # -- states --------------------------------------------------------------------------------------------------
     def _state(self, p):
@@ -124,7 +134,8 @@ class AdamW(torch.optim.Optimizer):
                 if len(steps) > 1:
                     raise ValueError("capturable: all parameters of a group must have done the same number of steps")
                 device_step = torch.tensor([steps.pop()], dtype=torch.int64, device=group["params"][0].device)
-            t = self._tables[index] = dict(params=len(states), rows=rows, counts=counts, states=states, device_step=device_step)
+            # `kept`: the rows hold addresses, so the tensors behind them must live as long
+            t = self._tables[index] = dict(params=len(states), rows=rows, counts=counts, states=states, kept=[s[n] for s in states for n in self._names()], device_step=device_step)
         return t
 
     def _steps(self, t):

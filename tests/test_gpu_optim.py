@@ -307,3 +307,36 @@ def test_a_parameter_that_changed_its_size_is_refused():
     ps[0].data = torch.zeros(32, device="cuda")
     with pytest.raises(ValueError):
         opt.step()
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("state_bits", [32, 8])
+def test_a_copied_optimizer_has_states_of_its_own(state_bits, capturable):
+    ps, gs = make([300, 40], 15)
+    for p, g in zip(ps, gs):
+        p.grad = g
+    opt = repro_optim.AdamW(ps, state_bits=state_bits, capturable=capturable, **HYPER)
+    opt.step()
+    twin = copy.deepcopy(opt)
+    qs = twin.param_groups[0]["params"]
+    for p, q in zip(ps, qs):
+        assert q is not p
+        q.grad = p.grad.clone()
+    kept = [t.clone() for t in opt.state[ps[0]].values() if isinstance(t, torch.Tensor)]
+    twin.step()
+    assert all(torch.equal(a, b) for a, b in zip(kept, (t for t in opt.state[ps[0]].values() if isinstance(t, torch.Tensor))))
+    opt.step()
+    for p, q in zip(ps, qs):
+        assert np.array_equal(bits(p), bits(q))
+
+
+def test_replaced_state_tensors_do_not_leave_the_kernel_without_memory():
+    ps, gs = make([300], 16)
+    ps[0].grad = gs[0]
+    opt = repro_optim.AdamW(ps, **HYPER)
+    opt.step()
+    held = opt._tables[0]["kept"][0]
+    opt.state[ps[0]]["exp_avg"] = torch.zeros(300, device="cuda")
+    before = held.clone()
+    opt.step()
+    assert not torch.equal(held, before)             # the step's own tensor was updated; adopt() is the way to replace it

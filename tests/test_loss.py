@@ -24,7 +24,7 @@ def backward(**kw):
 
 
 @needs_lib
-@pytest.mark.parametrize("bad", [dict(X=None), dict(W=None), dict(target=None), dict(N=0), dict(V=0), dict(D=0), dict(S=0), dict(S=4), dict(D=200000), dict(reduction=3),
+@pytest.mark.parametrize("bad", [dict(X=None), dict(W=None), dict(target=None), dict(N=0), dict(V=0), dict(V=(1 << 30) + 1), dict(N=(1 << 30) + 1), dict(D=0), dict(S=0), dict(S=4), dict(D=200000), dict(reduction=3),
                                  dict(reduction=-1), dict(ws=None), dict(ws=HERE + 16), dict(size=100), dict(lse=None), dict(tl=None), dict(inv=None)], ids=str)
 def test_both_calls_refuse(bad):
     assert forward(**bad) == 1 and backward(**bad) == 1
