@@ -77,8 +77,11 @@ cudaError_t launch_backward(const NormParams& P, int grid, cudaStream_t st) {
 template <int TPR, int V>
 cudaError_t launch_norm(const NormParams& P, bool backward, cudaStream_t st) {
     constexpr int CTA = norm_cta(TPR), GROUPS = CTA / TPR;
-    const int items = backward ? P.parts_total : P.rows, grid = (items - 1) / GROUPS + 1;
+    const int items = backward ? P.parts_total : P.rows;
+    int grid = (items - 1) / GROUPS + 1;
     if (!backward) {
+        const int mode = !P.y ? NORM_ONLY : !P.pw ? NORM_RESIDUAL : NORM_POST, resident = 148 * (2048 / CTA);
+        if (norm_stays(TPR, mode) && grid > resident) grid = resident;
         if (!P.y) block_norm_kernel<TPR, V, NORM_ONLY><<<grid, CTA, 0, st>>>(P);
         else if (!P.pw) block_norm_kernel<TPR, V, NORM_RESIDUAL><<<grid, CTA, 0, st>>>(P);
         else block_norm_kernel<TPR, V, NORM_POST><<<grid, CTA, 0, st>>>(P);

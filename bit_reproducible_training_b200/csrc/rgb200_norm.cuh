@@ -142,24 +142,13 @@ enum NormMode : int { NORM_ONLY = 0, NORM_RESIDUAL = 1, NORM_POST = 2 };     // 
 
 RGB_HD constexpr int norm_cta(int tpr) { return tpr < 256 ? 256 : tpr; }
 
+// One row from its values r (of x) and u (of y): r, h and the row's statistics.
 template <int TPR, int V, int MODE>
-__global__ void __launch_bounds__(norm_cta(TPR))
-block_norm_kernel(const NormParams P) {
-    constexpr int GROUPS = norm_cta(TPR) / TPR;
-    __shared__ float slots_all[GROUPS * NORM_SLOTS];
-    const int group = threadIdx.x / TPR, lane = threadIdx.x & (TPR - 1);
-    float* slots = slots_all + group * NORM_SLOTS;
-    int turn = 0;
-    const int row = blockIdx.x * GROUPS + group;
-    if (row >= P.rows) return;                                           // whole warps, and whole rows of threads
-    const bool wide = P.wide != 0;
+__device__ __forceinline__ void norm_forward_row(const NormParams& P, int row, float (&r)[NORM_VALUES], float (&u)[NORM_VALUES], int lane, float* slots,
+                                                 int& turn, int group, bool wide) {
     const size_t at = (size_t)row * P.dim;
-    float r[NORM_VALUES];
-    float mean_y = 0.0f, rstd_y = 0.0f, mean, rstd;
-    norm_load<TPR, V>(P.x + at, P.dim, lane, wide, r);
+    float t[NORM_VALUES], mean_y = 0.0f, rstd_y = 0.0f, mean, rstd;
     if (MODE != NORM_ONLY) {
-        float u[NORM_VALUES], t[NORM_VALUES];
-        norm_load<TPR, V>(P.y + at, P.dim, lane, wide, u);
         if (MODE == NORM_POST) {
             norm_row<TPR, V>(u, P, lane, slots, turn, group, mean_y, rstd_y);
             norm_load<TPR, V>(P.pw, P.dim, lane, wide, t);
@@ -176,14 +165,13 @@ block_norm_kernel(const NormParams P) {
         norm_store<TPR, V>(P.r + at, P.dim, lane, wide, r);
     }
     norm_row<TPR, V>(r, P, lane, slots, turn, group, mean, rstd);
-    float w[NORM_VALUES];
-    norm_load<TPR, V>(P.w, P.dim, lane, wide, w);
+    norm_load<TPR, V>(P.w, P.dim, lane, wide, t);
 #pragma unroll
-    for (int j = 0; j < NORM_VALUES; ++j) r[j] *= w[j];
+    for (int j = 0; j < NORM_VALUES; ++j) r[j] *= t[j];
     if (P.b) {
-        norm_load<TPR, V>(P.b, P.dim, lane, wide, w);
+        norm_load<TPR, V>(P.b, P.dim, lane, wide, t);
 #pragma unroll
-        for (int j = 0; j < NORM_VALUES; ++j) r[j] += w[j];
+        for (int j = 0; j < NORM_VALUES; ++j) r[j] += t[j];
     }
     norm_store<TPR, V>(P.h + at, P.dim, lane, wide, r);
     if (P.stats && lane == 0) {
@@ -191,6 +179,48 @@ block_norm_kernel(const NormParams P) {
         P.stats[(size_t)P.rows + row] = rstd;
         P.stats[2 * (size_t)P.rows + row] = mean_y;
         P.stats[3 * (size_t)P.rows + row] = rstd_y;
+    }
+}
+
+// Forward: a row of threads for each row, the SM's other rows filling the pauses of its sums; or, where that leaves too little in flight,
+// CTAs that stay and load their next row before they work on the present one.  That pays where few CTAs fit an SM (rows of 1024
+// threads: 4096 x 8192 with post norm 109 us against 131, without 52 against 57) and for 64 and 128 threads without a block's output
+// (65536 x 512: 48 us against 55; 43690 x 768: 54 against 65; 32768 x 1024: 48 against 55); elsewhere the registers of a second row cost more than they give (8192 x 4096:
+// 134 us against 87 with post norm, 48 against 46 without; 16384 x 2048: 48 against 44; 131072 x 256: 47 against 44).
+RGB_HD constexpr bool norm_stays(int tpr, int mode) { return tpr == 1024 || ((tpr == 64 || tpr == 128) && mode == NORM_ONLY); }
+
+template <int TPR, int V, int MODE>
+__global__ void __launch_bounds__(norm_cta(TPR))
+block_norm_kernel(const NormParams P) {
+    constexpr int GROUPS = norm_cta(TPR) / TPR;
+    __shared__ float slots_all[GROUPS * NORM_SLOTS];
+    const int group = threadIdx.x / TPR, lane = threadIdx.x & (TPR - 1);
+    float* slots = slots_all + group * NORM_SLOTS;
+    int turn = 0;
+    const bool wide = P.wide != 0;
+    long long row = (long long)blockIdx.x * GROUPS + group;
+    if (row >= P.rows) return;                                           // whole warps, and whole rows of threads
+    float x[NORM_VALUES], y[NORM_VALUES];
+    norm_load<TPR, V>(P.x + (size_t)row * P.dim, P.dim, lane, wide, x);
+    if (MODE != NORM_ONLY) norm_load<TPR, V>(P.y + (size_t)row * P.dim, P.dim, lane, wide, y);
+    if constexpr (!norm_stays(TPR, MODE)) {
+        norm_forward_row<TPR, V, MODE>(P, (int)row, x, y, lane, slots, turn, group, wide);
+    } else {
+        const long long step = (long long)gridDim.x * GROUPS;
+        for (; row < P.rows; row += step) {
+            float r[NORM_VALUES], u[NORM_VALUES];
+#pragma unroll
+            for (int j = 0; j < NORM_VALUES; ++j) {
+                r[j] = x[j];
+                if (MODE != NORM_ONLY) u[j] = y[j];
+            }
+            if (row + step < P.rows) {
+                const size_t next = (size_t)(row + step) * P.dim;
+                norm_load<TPR, V>(P.x + next, P.dim, lane, wide, x);
+                if (MODE != NORM_ONLY) norm_load<TPR, V>(P.y + next, P.dim, lane, wide, y);
+            }
+            norm_forward_row<TPR, V, MODE>(P, (int)row, r, u, lane, slots, turn, group, wide);
+        }
     }
 }
 
