@@ -462,10 +462,10 @@ struct RunArgs {
     // B's digit planes and exponents already sit in the workspace from the previous call on it with the same
     // N, K, S and transposition (row blocks of one product): skip B's pre-pass.
     bool reuse_b = false;
-    // An epilogue behind the rounding (see Epilogue); such a product takes the general kernel whatever its shape.
     bool reuse_a = false;      // op(A)'s planes and exponents are in place (see Prepared in rgb200_gemm.h)
     int* status = nullptr;     // a word of the caller's in place of the workspace's (see Prepared)
     bool zero_status = true;
+    // An epilogue behind the rounding (see Epilogue); such a product takes the general kernel whatever its shape.
     int epi = EPI_NONE;
     const EpilogueParams* epi_params = nullptr;
 };
