@@ -6,6 +6,7 @@ the moments held in FP32 or in 8 bits.  Every value goes through the same fixed 
 CUDA float32 parameters only; there is no CPU path.
 """
 import ctypes as C
+import operator
 import sys
 
 import numpy as np
@@ -18,9 +19,16 @@ _torch_optimizer = sys.modules[torch.optim.Optimizer.__module__]        # torch.
 
 STATE_BLOCK = 256           # values of a tensor that share one scale (8-bit states)
 
+_nbytes = operator.attrgetter("nbytes")
+
 # one row of the C ABI's rgb200_adamw_tensor
 _ROW = np.dtype([(n, np.uint64) for n in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")] +
                 [("count", np.int64)])
+
+
+def _counter(n):
+    """A number of steps done, as a tensor that several states can share."""
+    return torch.tensor(int(n), dtype=torch.int64, device="cpu")
 
 
 def _blocks(n):
@@ -128,21 +136,27 @@ class AdamW(torch.optim.Optimizer):
                 rows[name] = [s[name].data_ptr() for s in states]
             counts = [s["exp_avg"].numel() for s in states]
             rows["count"] = counts
-            steps = {s["step"] for s in states}
-            device_step = None
-            if self.capturable and states:
-                if len(steps) > 1:
-                    raise ValueError("capturable: all parameters of a group must have done the same number of steps")
-                device_step = torch.tensor([steps.pop()], dtype=torch.int64, device=group["params"][0].device)
+            steps = {int(s["step"]) for s in states}
+            device_step = shared = None
+            if len(steps) == 1:                      # one counter for all parameters, until a missing gradient parts them
+                shared = _counter(steps.pop())
+                for s in states:
+                    s["step"] = shared
+                if self.capturable:
+                    device_step = shared.to(group["params"][0].device)
+            elif self.capturable and states:
+                raise ValueError("capturable: all parameters of a group must have done the same number of steps")
+            else:
+                for s in states:
+                    s["step"] = _counter(s["step"])
             # `kept`: the rows hold addresses, so the tensors behind them must live as long
-            t = self._tables[index] = dict(params=len(states), rows=rows, counts=counts, states=states, kept=[s[n] for s in states for n in self._names()], device_step=device_step)
+            t = self._tables[index] = dict(params=len(states), rows=rows, counts=counts, bytes=[4 * n for n in counts], states=states, step=shared,
+                                           kept=[s[n] for s in states for n in self._names()], device_step=device_step)
         return t
 
     def _steps(self, t):
         if t["device_step"] is not None:
-            n = int(t["device_step"].item())
-            for s in t["states"]:
-                s["step"] = n
+            t["step"].fill_(t["device_step"].item())
 
     # -- the step ------------------------------------------------------------------------------------------------
     def step(self, closure=None):
@@ -171,6 +185,33 @@ class AdamW(torch.optim.Optimizer):
         if not self.capturable and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW.step under CUDA graph capture needs capturable=True")
         t = self._table(index)
+        if t["step"] is None or not self._ready(t, group["params"]):
+            return self._step_checked(group, t)
+        torch.autograd.graph.increment_version(group["params"])
+        if t["device_step"] is not None:
+            self._launch(group, t["rows"], 0, t["device_step"].data_ptr())
+        else:
+            self._launch(group, t["rows"], int(t["step"].add_(1)), None)
+
+    @staticmethod
+    def _ready(t, params):
+        """Enters the addresses of the usual case, every parameter and gradient a contiguous float32 tensor of its size on the group's device;
+        False for anything else.  A few passes over the list in C: a step over many small tensors costs what the host spends on each."""
+        T, nbytes, dev = torch.Tensor, _nbytes, {t["kept"][0].get_device()}
+        try:
+            grads = [p.grad for p in params]
+            # of the floating types only float32 has four bytes
+            if not (list(map(nbytes, params)) == t["bytes"] == list(map(nbytes, grads)) and set(map(T.get_device, params)) == dev == set(map(T.get_device, grads)) and
+                    all(map(T.is_contiguous, params)) and all(map(T.is_contiguous, grads))):
+                return False
+            addresses = list(map(T.data_ptr, params)), list(map(T.data_ptr, grads))
+        except (AttributeError, TypeError, RuntimeError):        # a gradient that is None or not dense
+            return False
+        t["rows"]["param"], t["rows"]["grad"] = addresses
+        return True
+
+    def _step_checked(self, group, t):
+        """Missing gradients, gradients to be laid out, parameters that have done different numbers of steps; and the errors."""
         params, states, rows, counts = group["params"], t["states"], t["rows"], t["counts"]
         grads = [p.grad for p in params]
         live = [i for i, g in enumerate(grads) if g is not None]
@@ -181,8 +222,7 @@ class AdamW(torch.optim.Optimizer):
                 return
             params, states, grads = ([x[i] for i in live] for x in (params, states, grads))
             rows, counts = np.ascontiguousarray(rows[live]), [counts[i] for i in live]
-        T, dev = torch.Tensor, {params[0].get_device()}
-        # whole-list checks: a call's host time is what bounds a step over many small tensors
+        T, dev = torch.Tensor, {t["kept"][0].get_device()}
         if {g.dtype for g in grads} != {torch.float32} or {g.layout for g in grads} != {torch.strided} or set(map(T.get_device, grads)) != dev:
             raise TypeError("gradients must be dense float32 tensors on the parameter's device")
         if not all(map(T.is_contiguous, grads)):
@@ -197,12 +237,14 @@ class AdamW(torch.optim.Optimizer):
         if t["device_step"] is not None:
             self._launch(group, rows, 0, t["device_step"].data_ptr())
             return
-        steps = [s["step"] + 1 for s in states]
-        for s, n in zip(states, steps):
-            s["step"] = n
-        if min(steps) == max(steps):
-            self._launch(group, rows, steps[0], None)
+        if t["step"] is not None and len(live) == len(group["params"]):
+            self._launch(group, rows, int(t["step"].add_(1)), None)
             return
+        if t["step"] is not None:                    # from here on each parameter counts for itself
+            t["step"] = None
+            for s in t["states"]:
+                s["step"] = s["step"].clone()
+        steps = [int(s["step"].add_(1)) for s in states]
         for n in sorted(set(steps)):
             self._launch(group, np.ascontiguousarray(rows[[i for i, k in enumerate(steps) if k == n]]), n, None)
 
@@ -237,9 +279,10 @@ class AdamW(torch.optim.Optimizer):
             t = self._table(index)
             gm, gv, dev = ms[at:at + len(params)], vs[at:at + len(params)], params[0].device
             at += len(params)
-            for x, n in zip(list(gm) + list(gv), list(t["rows"]["count"]) * 2):
-                if x.dtype != torch.float32 or x.device != dev or x.numel() != n or not x.is_contiguous():
-                    raise ValueError("the moments' values are contiguous float32 tensors of the parameters' sizes on their device")
+            both, T = [*gm, *gv], torch.Tensor
+            if {x.dtype for x in both} != {torch.float32} or set(map(T.get_device, both)) != {dev.index} or list(map(T.numel, both)) != t["counts"] * 2 or \
+                    not all(map(T.is_contiguous, both)):
+                raise ValueError("the moments' values are contiguous float32 tensors of the parameters' sizes on their device")
             with _on(dev):
                 if self.state_bits == 32:
                     for s, m, v in zip(t["states"], gm, gv):
@@ -248,7 +291,7 @@ class AdamW(torch.optim.Optimizer):
                             (x.view(-1).copy_(own.view(-1)) if call.endswith("read") else own.view(-1).copy_(x.view(-1)))
                     continue
                 rows = t["rows"].copy()
-                rows["param"], rows["grad"] = [m.data_ptr() for m in gm], [v.data_ptr() for v in gv]
+                rows["param"], rows["grad"] = list(map(T.data_ptr, gm)), list(map(T.data_ptr, gv))
                 rc = getattr(_lib.lib(), call)(rows.ctypes.data, len(rows), _raw_stream(dev))
                 if rc != cudaSuccess:
                     raise ReproGemmError(rc, call[7:])
@@ -265,7 +308,7 @@ class AdamW(torch.optim.Optimizer):
             n = len(g["params"])
             groups.append({**{k: v for k, v in g.items() if k != "params"}, "params": list(range(at, at + n))})
             at += n
-        state = {i: dict(step=self.state[p]["step"], exp_avg=ms[i], exp_avg_sq=vs[i]) for i, p in enumerate(params)}
+        state = {i: dict(step=int(self.state[p]["step"]), exp_avg=ms[i], exp_avg_sq=vs[i]) for i, p in enumerate(params)}
         return {"state": state, "param_groups": groups}
 
     def load_state_dict(self, state_dict):
@@ -288,12 +331,20 @@ class AdamW(torch.optim.Optimizer):
             for name, to in (("exp_avg", ms), ("exp_avg_sq", vs)):
                 to.append(got[name].to(device=p.device, dtype=torch.float32).contiguous() if got else torch.zeros(p.shape, device=p.device))
         self.write_states(ms, vs)                    # into the tensors there are: a captured step stays valid
-        for index, t in list(self._tables.items()):
-            steps = {s["step"] for s in t["states"]}
-            if t["device_step"] is not None:
-                if len(steps) > 1:
+        for t in self._tables.values():
+            steps = {int(s["step"]) for s in t["states"]}
+            if len(steps) == 1:                      # one counter again, and the captured step's
+                t["step"] = _counter(steps.pop())
+                for s in t["states"]:
+                    s["step"] = t["step"]
+                if t["device_step"] is not None:
+                    t["device_step"].fill_(int(t["step"]))
+            else:
+                if t["device_step"] is not None:
                     raise ValueError("capturable: all parameters of a group must have done the same number of steps")
-                t["device_step"].fill_(steps.pop())
+                t["step"] = None
+                for s in t["states"]:
+                    s["step"] = _counter(s["step"])
 
 
 _hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)

@@ -340,3 +340,57 @@ def test_replaced_state_tensors_do_not_leave_the_kernel_without_memory():
     before = held.clone()
     opt.step()
     assert not torch.equal(held, before)             # the step's own tensor was updated; adopt() is the way to replace it
+
+
+def test_parameters_part_and_meet_again():
+    """Missing gradients part the parameters' counters; a loaded state joins them again; a table made from states that differ works too."""
+    ps, gs = make([300, 40, 5], 17)
+    opt = repro_optim.AdamW(ps, **HYPER)
+    for have in ((0, 1, 2), (0, 2), (1,), (), (0, 1, 2)):
+        for i, p in enumerate(ps):
+            p.grad = gs[i] if i in have else None
+        opt.step()
+    assert [int(opt.state[p]["step"]) for p in ps] == [3, 3, 3]
+    saved = copy.deepcopy(opt.state_dict())
+    saved["state"][1]["step"] = 7
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    twin = repro_optim.AdamW(qs, **HYPER)
+    twin.load_state_dict(saved)
+    for q, g in zip(qs, gs):
+        q.grad = g
+    twin.step()
+    assert [int(twin.state[q]["step"]) for q in qs] == [4, 8, 4]
+    want = adamw(host([ps[1]])[0], host([gs[1]])[0], *(saved["state"][1][k].cpu().numpy() for k in ("exp_avg", "exp_avg_sq")), HYPER["lr"], *HYPER["betas"],
+                 HYPER["eps"], HYPER["weight_decay"], 8)[0]
+    assert np.array_equal(bits(qs[1]), bits(want))
+    saved["state"][1]["step"] = 3
+    twin.load_state_dict(saved)
+    twin.step()
+    assert [int(twin.state[q]["step"]) for q in qs] == [4, 4, 4] and twin.state[qs[0]]["step"] is twin.state[qs[2]]["step"]
+    # the same sequence of steps on each parameter alone
+    for i, p in enumerate(ps):
+        lone = torch.nn.Parameter(make([300, 40, 5], 17)[0][i].detach().clone())
+        alone = repro_optim.AdamW([lone], **HYPER)
+        lone.grad = gs[i]
+        for _ in range(3):
+            alone.step()
+        assert np.array_equal(bits(p), bits(lone))
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float64])
+def test_swapped_gradient_data_is_refused(kind):
+    ps, gs = make([64, 8], 18)
+    for p, g in zip(ps, gs):
+        p.grad = g
+    opt = repro_optim.AdamW(ps, **HYPER)
+    opt.step()
+    before = host(ps)
+    ps[0].grad.data = ps[0].grad.data.to(kind)
+    with pytest.raises(TypeError):
+        opt.step()
+    ps[0].grad = None
+    ps[0].grad = gs[0].float()
+    ps[1].grad.data = ps[1].grad.data.cpu()
+    with pytest.raises(TypeError):
+        opt.step()
+    assert all(np.array_equal(bits(a), bits(b)) for a, b in zip(ps, before)) and int(opt.state[ps[0]]["step"]) == 1
