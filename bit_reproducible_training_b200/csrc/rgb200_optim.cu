@@ -74,8 +74,10 @@ cudaError_t adamw_call(const rgb200_adamw_tensor* t, int count, int bits, OptMod
     if (e != cudaSuccess || total == 0) return e;
     const int chunk = pick_chunk(total);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return count <= OPT_SMALL_TABLE ? run_adamw<OPT_SMALL_TABLE>(t, count, chunk, bits, mode, H, st)
-                                    : run_adamw<OPT_LARGE_TABLE>(t, count, chunk, bits, mode, H, st);
+    // the smallest table that takes them all: its bytes are copied twice on the way to the GPU
+    if (count <= OPT_SMALL_TABLE) return run_adamw<OPT_SMALL_TABLE>(t, count, chunk, bits, mode, H, st);
+    if (count <= OPT_MEDIUM_TABLE) return run_adamw<OPT_MEDIUM_TABLE>(t, count, chunk, bits, mode, H, st);
+    return run_adamw<OPT_LARGE_TABLE>(t, count, chunk, bits, mode, H, st);
 }
 
 }  // namespace

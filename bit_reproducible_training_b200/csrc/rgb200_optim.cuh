@@ -27,7 +27,7 @@ namespace rgb200 {
 constexpr int OPT_THREADS = 256;
 constexpr int OPT_BLOCK = 256;          // values that share a scale
 constexpr int OPT_MIN_CHUNK = 1024;     // values per CTA: a multiple of this
-constexpr int OPT_SMALL_TABLE = 48, OPT_LARGE_TABLE = 448;   // tensors a launch takes by value (448 x 60 bytes < 32 KB)
+constexpr int OPT_SMALL_TABLE = 48, OPT_MEDIUM_TABLE = 160, OPT_LARGE_TABLE = 448;   // tensors a launch takes by value (448 x 60 bytes < 32 KB)
 
 struct OptEntry {
     float* p;
