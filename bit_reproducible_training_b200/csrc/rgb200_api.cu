@@ -327,7 +327,7 @@ cudaError_t launch_cluster_split(const CUtensorMap& map, const float* given_max,
 // Whether a k-strided operand of R rows (16-byte aligned base and batch stride taken for granted) takes the cluster form.
 bool cluster_split_fits(int R, int Kp) {
     const int KC = ceil_div(ceil_div(Kp, KSC_CLUSTER), KSC_BOX_K) * KSC_BOX_K;
-    return R % 4 == 0 && (size_t)KC * 8 * 4 <= (size_t)KSC_MAX_SLAB_BYTES;
+    return R % 4 == 0 && (size_t)KC * 16 * 4 <= (size_t)KSC_MAX_SLAB_BYTES;
 }
 
 template <int S>
@@ -338,7 +338,9 @@ bool try_cluster_split(const float* src, const float* given_max, int8_t* planes,
     const int KC = ceil_div(ceil_div(Kp, KSC_CLUSTER), KSC_BOX_K) * KSC_BOX_K;
     int W = 32;
     while (W > 8 && (size_t)KC * W * 4 > (size_t)KSC_MAX_SLAB_BYTES) W >>= 1;
-    if ((size_t)KC * W * 4 > (size_t)KSC_MAX_SLAB_BYTES) return false;
+    // a slab that leaves room for panels of eight columns only (K beyond 24 576) reads half sectors: the two-kernel form is faster (32003 x
+    // 512: 37 us against 59; a 512 x 8192 x 30000 product 1.26 ms against 1.47)
+    if ((size_t)KC * W * 4 > (size_t)KSC_MAX_SLAB_BYTES || W < 16) return false;
     while (W > 8 && (long long)ceil_div(R, W) * KSC_CLUSTER * batch < PLAN_SM_COUNT) W >>= 1;   // few columns: narrower panels, more CTAs
     CUtensorMap map;
     if (encode_kstrided_map(&map, src, R, K, batch, batch_stride, W) != cudaSuccess) return false;
