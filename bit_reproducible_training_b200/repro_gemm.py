@@ -8,6 +8,7 @@ the reference's binding sends CPU tensors to its CPU implementation, this one re
 """
 import contextlib
 import ctypes as C
+import functools
 import os
 import enum
 from dataclasses import dataclass
@@ -230,20 +231,26 @@ def _check(t, n, name):
     return t.contiguous()
 
 
+@functools.lru_cache(maxsize=4096)
+def _planned(device, M, N, K, trans_a, trans_b, slices, split_k, algo):
+    """(code, configuration, workspace bytes) of a product of these sizes on this device; the configuration is only read."""
+    cfg, plan = _lib.Config(split_k, 16, 16, 32, algo, slices, trans_a, trans_b), _lib.Plan()
+    rc = _lib.lib().rgb200_make_plan(M, N, K, C.byref(cfg), C.byref(plan))
+    return rc, cfg, plan.workspace_bytes
+
+
 def gemm(A, B, M, N, K, trans_a=False, trans_b=False, slices=3, split_k=1, algo=Algo.Auto):
     """C[M,N] = op(A) op(B) on the current stream; the counterpart of ``_backend.gemm``
     (repro_torch/src/bindings.cpp:43-66).  Returns a new [M, N] float32 CUDA tensor."""
     A = _check(A, M * K, "A")
     B = _check(B, K * N, "B")
-    L = _lib.lib()
-    cfg, plan = _lib.Config(split_k, 16, 16, 32, int(algo), slices, int(trans_a), int(trans_b)), _lib.Plan()
     with _on(A.device):
-        rc = L.rgb200_make_plan(M, N, K, C.byref(cfg), C.byref(plan))
+        rc, cfg, nbytes = _planned(A.device.index, M, N, K, bool(trans_a), bool(trans_b), slices, split_k, int(algo))
         if rc != cudaSuccess:
             raise ReproGemmError(rc, "make_plan")
-        ws = _workspace(plan.workspace_bytes, A.device)
+        ws = _workspace(nbytes, A.device)
         out = torch.empty((M, N), dtype=torch.float32, device=A.device)
-        rc = L.rgb200_gemm_fp32_ws(_addr(A), _addr(B), _addr(out), M, N, K, C.byref(cfg), _addr(ws), ws.numel(), _raw_stream(A.device), None)
+        rc = _lib.lib().rgb200_gemm_fp32_ws(_addr(A), _addr(B), _addr(out), M, N, K, C.byref(cfg), _addr(ws), ws.numel(), _raw_stream(A.device), None)
     if rc != cudaSuccess:
         raise ReproGemmError(rc, "repro_gemm_fp32_ws")
     _raise_if_incomplete(ws, "gemm")
@@ -277,19 +284,17 @@ def gemm_epilogue(A, B, M, N, K, trans_a=False, trans_b=False, slices=3, bias=No
     if out is not None and (out.dtype != torch.float32 or out.numel() != M * N or not out.is_contiguous()):
         raise ValueError("out must be a contiguous float32 tensor of %d elements" % (M * N))
     act = _activation(activation)
-    L = _lib.lib()
-    cfg, plan = _lib.Config(1, 16, 16, 32, 0, slices, int(trans_a), int(trans_b)), _lib.Plan()
-    with _on(A.device):
-        rc = L.rgb200_make_plan(M, N, K, C.byref(cfg), C.byref(plan))
+    with _on(device):
+        rc, cfg, nbytes = _planned(device.index, M, N, K, bool(trans_a), bool(trans_b), slices, 1, 0)
         if rc != cudaSuccess:
             raise ReproGemmError(rc, "make_plan")
-        ws = _scratch(plan.workspace_bytes, A.device)
+        ws = _scratch(nbytes, device)
         if out is None:
             out = torch.empty((M, N), dtype=torch.float32, device=A.device)
         pre = torch.empty((M, N), dtype=torch.float32, device=A.device) if keep_pre else None
         e = _lib.Epilogue(_addr(bias), _addr(residual), _addr(pre), act)
-        rc = L.rgb200_gemm_epilogue_fp32_ws(_addr(A), _addr(B), _addr(out), M, N, K, C.byref(cfg), C.byref(e), _addr(ws), ws.numel(),
-                                            _raw_stream(A.device))
+        rc = _lib.lib().rgb200_gemm_epilogue_fp32_ws(_addr(A), _addr(B), _addr(out), M, N, K, C.byref(cfg), C.byref(e), _addr(ws), nbytes,
+                                                     _raw_stream(device))
     if rc != cudaSuccess:
         raise ReproGemmError(rc, "gemm_epilogue_fp32_ws")
     _raise_if_incomplete(ws, "gemm_epilogue")
