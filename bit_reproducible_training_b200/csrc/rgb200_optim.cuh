@@ -17,6 +17,10 @@
 // A value that is not finite makes its block's scale NaN, so that the block reads as NaN (FP32 states keep a NaN too).
 //
 // Bound: HBM.  28 bytes a value in FP32 (p, m, v read and written, g read), 16 + 16/256 with 8-bit states.
+// Measured, 124 M values in 111 tensors: FP32 states 511 us (6.8 TB/s, the copy rate); 8-bit states 451 us (4.5 TB/s), where the issue of
+// about 90 instructions a value (the definition's root and quotient a third of them) takes longer than the memory: five CTAs an SM
+// (48 registers) against four: 9 % faster, six: 2 % faster still with more spills; read-out of the values 226 us (5.5 TB/s).
+// Split: a CTA takes a chunk of one tensor, found by bisection in the launch's table.
 #pragma once
 #include <cuda_runtime.h>
 #include <cstdint>
