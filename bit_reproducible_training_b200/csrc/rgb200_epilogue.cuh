@@ -8,7 +8,7 @@
 // fixed order, so the bits do not depend on the tiling (EPI_LSE: on the tile width alone).
 //
 // Why here: an output costs 4 bytes of HBM written by the product and 8 more for every elementwise pass behind it.  In
-// the kernel the extra work of a thread (32 columns of one row) overlaps the next tile's MMAs, which take about 1150 clocks for each
+// the kernel the extra work of a thread (16 or 32 columns of one row) overlaps the next tile's MMAs, which take about 1150 clocks for each
 // 128 values of k; the residual and the bias are requested before the wait for the accumulators.
 #pragma once
 #include "rgb200_mma.cuh"
