@@ -27,6 +27,8 @@ extern "C" {
  * bias [N], residual [M, N] (may be C itself) and pre_activation [M, N] (receives Z) may be NULL.  Activations: gelu is
  * z/2 (1 + erf(z / sqrt 2)), gelu_tanh z/2 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))), silu z / (1 + exp(-z)).
  * Plan and workspace are those of rgb200_make_plan.  1: as rgb200_gemm_fp32_ws, or an unknown activation; 801: RGB200_ALGO_REFERENCE.
+ * Slopes are those of the computed Z: relu's is 0 for Z <= 0, so a Z within the product's rounding of zero may pass or stop a gradient that
+ * another product, rounded otherwise, would not.
  * rgb200_activation_backward: dZ = dY act'(Z) (dZ may be NULL, or dY itself) and db = column sums of dZ (may be NULL; the
  * workspace, of rgb200_activation_backward_workspace bytes, is needed for db alone).  Z may be NULL without an activation. */
 enum { RGB200_ACT_NONE = 0, RGB200_ACT_RELU = 1, RGB200_ACT_SILU = 2, RGB200_ACT_GELU = 3, RGB200_ACT_GELU_TANH = 4 };
