@@ -87,7 +87,7 @@ cudaError_t launch_norm(const NormParams& P, bool backward, cudaStream_t st) {
         else block_norm_kernel<TPR, V, NORM_POST><<<grid, CTA, 0, st>>>(P);
         return cudaGetLastError();
     }
-    if (!P.y) return launch_backward<TPR, V, NORM_ONLY>(P, grid, st);
+    if (!P.y && !P.dr) return launch_backward<TPR, V, NORM_ONLY>(P, grid, st);
     if (!P.pw) return launch_backward<TPR, V, NORM_RESIDUAL>(P, grid, st);
     return launch_backward<TPR, V, NORM_POST>(P, grid, st);
 }
@@ -136,6 +136,10 @@ extern "C" int rgb200_block_norm_backward(const rgb200_block_norm* n, void* work
     const NormParts parts = norm_parts(n->rows, n->dim, n->groups);
     P.parts = static_cast<float*>(workspace);
     P.rows_per_part = parts.rows; P.parts_per_group = parts.per_group; P.parts_total = parts.total;
+    if (!P.y) {                              // r is x itself, with a weight of one in the stream's gradient
+        P.r = const_cast<float*>(P.x);       // only read
+        P.scale = 1.0f;
+    }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (n->rows > 0) {
         e = P.dim % 4 == 0 ? dispatch_norm<4>(P, true, st) : dispatch_norm<1>(P, true, st);

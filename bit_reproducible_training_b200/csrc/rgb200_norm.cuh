@@ -8,7 +8,7 @@
 //
 // Backward, with R = gradient of r from the residual stream, H = gradient of h, t^ the normed rows and
 // N'(t^, rstd, q) = rstd (q - t^ mean(q t^) - mean(q)) (the RMS kind without the last term):
-//   D  = R + N'(r^, rstd, w H)         dx = s D
+//   D  = R + N'(r^, rstd, w H)         dx = s D  (D when there is no y)
 //   dy = N'(y^, rstd', w' g D)         (or g D without a post norm)
 //   dw = sum_rows H r^,  db = sum_rows H,  and with Q = sum_rows D y^ (D y without a post norm) over the rows of a group,
 //   dw' = sum_groups g Q,  dg = w' Q.
@@ -138,7 +138,8 @@ __device__ __forceinline__ void norm_row(float (&v)[NORM_VALUES], const NormPara
     for (int j = 0; j < NORM_VALUES; ++j) v[j] *= rstd;
 }
 
-enum NormMode : int { NORM_ONLY = 0, NORM_RESIDUAL = 1, NORM_POST = 2 };     // no y; y as it is; y through its own norm
+// no y; y as it is; y through its own norm.  Backward: no y and no dr; y as it is, or no y but a dr (r is x, nothing is read of y); y through its own norm
+enum NormMode : int { NORM_ONLY = 0, NORM_RESIDUAL = 1, NORM_POST = 2 };
 
 RGB_HD constexpr int norm_cta(int tpr) { return tpr < 256 ? 256 : tpr; }
 

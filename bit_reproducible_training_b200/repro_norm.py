@@ -89,7 +89,7 @@ def block_norm(x, y=None, *, weight, bias=None, post_weight=None, gate=None, res
 
 def block_norm_backward(dh, dr, r, y, stats, *, weight, bias=None, post_weight=None, gate=None, residual_scale=1.0, kind="rms", eps=1e-5,
                         wanted=("x", "y", "weight", "bias", "post_weight", "gate")):
-    """Gradients of block_norm from dh and dr (the gradient that reaches r from the residual stream; may be None).
+    """Gradients of block_norm from dh and dr (the gradient that reaches r, without y x itself, from the residual stream; may be None).
     r, y, stats: what the forward call returned and took.  `wanted` names the gradients to form."""
     rows, dim, groups = _sizes(r, y, weight, bias, post_weight, gate, kind, eps)
     _same_device((r, dh, dr, stats))

@@ -116,7 +116,8 @@ int rgb200_adamw_states_write(const rgb200_adamw_tensor* tensors, int count, voi
  * groups 1 it is one value a channel.
  * stats (float[4 * rows]; forward: may be NULL) carries the rows' means and reciprocal deviations to the backward call, which
  * takes the gradients dr (of r from elsewhere; may be NULL) and dh, and writes those outputs that are not NULL: dx[rows, dim],
- * dy, dweight[dim], dbias[dim], dpost_weight[dim], dgate[groups, dim].  r may be the forward call's x when y is NULL.
+ * dy, dweight[dim], dbias[dim], dpost_weight[dim], dgate[groups, dim].  Without y, r is x: r is not read, and dr (of x from the
+ * residual stream) is added to dx as it is.
  * Sums are taken in an order that depends on (rows, dim, groups) alone.  Asynchronous and allocation-free; dim at most 8192.
  * The workspace (16-byte aligned) may be reused by any later call on the same stream.
  * 1 (invalid value): sizes outside those limits, rows not a multiple of groups, negative or NaN eps, post_weight or gate or
