@@ -1,7 +1,7 @@
 // Epilogues of the tcgen05 GEMM kernel (rgb200_mma.cuh) and of the rounding kernel behind K ranges:
 //
 //   EPI_LINEAR   y = act(c + bias[col]) + residual[row][col], with c + bias stored beside it on request.
-//   EPI_LSE      per row: m = max over the tile's columns, s = sum exp(c - m); c itself is not stored.
+//   EPI_LSE      per row: m = max over the tile's columns, s = sum exp(c - m) over all but the row's target word; of c only the target's is stored.
 //   EPI_PROB     row_scale[row] * exp(c - lse[row]), zero at the row's target word.
 //
 // c is the product rounded once to FP32, as the plain entry points return it; every step after it is one FP32 operation in a
@@ -158,7 +158,10 @@ struct EpilogueRow<EPI_LSE, CPT> {
             for (int i = 0; i < 8; ++i) {
                 v[j + i] = col0 + j + i < P.N ? c[i] : -INFINITY;          // the first column is always inside, so top is finite
                 top = fmaxf(top, v[j + i]);
-                if (j + i == target) hit = v[j + i];
+                if (j + i == target) {                                     // kept apart from the sum: see xent_join_kernel
+                    hit = c[i];
+                    v[j + i] = -INFINITY;
+                }
             }
         }
 #pragma unroll

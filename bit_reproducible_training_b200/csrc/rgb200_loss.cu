@@ -1,7 +1,7 @@
 // Cross entropy of logits X W^T against targets in pieces of the vocabulary, without the logits (include/rgb200_train.h).
 //
 // Forward, for each piece of words: the product X W_piece^T runs with an epilogue that keeps, of each row and each 32 columns, the
-// maximum and the sum of exponentials (8 bytes instead of 128), and the target's logit; a small kernel joins them into the
+// maximum and the sum of exponentials without the target's (8 bytes instead of 128), and the target's logit; a small kernel joins them into the
 // rows' running statistics.  Backward, for each piece: the product again, now leaving P = g softmax without the targets' own
 // entries in FP32 (one piece at a time), then dX += P W_piece (the running dX is the epilogue's residual) and
 // dW_piece = P^T X.  The targets' entries (p - 1) g are kept apart: beside them the rest of a row is small, and in one matrix
@@ -146,9 +146,9 @@ extern "C" size_t rgb200_linear_xent_workspace(int N, int V, int D, int slices, 
 }
 
 extern "C" int rgb200_linear_xent_forward(const float* X, const float* W, const long long* target, long long ignore_index, int reduction, int N, int V,
-                                          int D, int slices, float* loss, float* nll, float* lse, float* target_logit, float* inv_count,
+                                          int D, int slices, float* loss, float* nll, float* lse, float* target_rest, float* inv_count,
                                           void* workspace, size_t workspace_bytes, void* stream) {
-    if (!good_sizes(N, V, D, slices) || !X || !W || !target || !nll || !lse || !target_logit || !workspace) return cudaErrorInvalidValue;
+    if (!good_sizes(N, V, D, slices) || !X || !W || !target || !nll || !lse || !target_rest || !workspace) return cudaErrorInvalidValue;
     if (reduction < RGB200_REDUCE_NONE || reduction > RGB200_REDUCE_SUM || (reduction != RGB200_REDUCE_NONE && (!loss || !inv_count))) return cudaErrorInvalidValue;
     ForwardLayout L;
     if (!forward_layout(N, V, D, slices, L)) return cudaErrorInvalidValue;
@@ -161,7 +161,7 @@ extern "C" int rgb200_linear_xent_forward(const float* X, const float* W, const 
     EpilogueParams E = {};
     E.target = target;
     E.lse_parts = reinterpret_cast<float2*>(ws + L.parts);
-    E.target_logit = target_logit;
+    E.target_logit = target_rest;            // the logits, until the last join leaves the others' probability in their place
     for (int at = 0; at < V; at += L.words) {
         const int words = V - at < L.words ? V - at : L.words;
         E.first_word = at;
@@ -173,7 +173,7 @@ extern "C" int rgb200_linear_xent_forward(const float* X, const float* W, const 
         // the last half tile of a piece has a part only if it has columns
         const int parts = (words + EPI_TILE_N / 2 - 1) / (EPI_TILE_N / 2);
         xent_join_kernel<<<(N + XENT_ROWS - 1) / XENT_ROWS, 32 * XENT_WARPS, 0, st>>>(
-            E.lse_parts, parts, reinterpret_cast<float2*>(ws + L.running), N, at == 0, at + words == V, target, ignore_index, V, target_logit, lse, nll);
+            E.lse_parts, parts, reinterpret_cast<float2*>(ws + L.running), N, at == 0, at + words == V, target, ignore_index, V, target_rest, lse, nll);
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }
     if (reduction != RGB200_REDUCE_NONE)
@@ -182,9 +182,9 @@ extern "C" int rgb200_linear_xent_forward(const float* X, const float* W, const 
 }
 
 extern "C" int rgb200_linear_xent_backward(const float* X, const float* W, const long long* target, long long ignore_index, int reduction, int N, int V,
-                                           int D, int slices, const float* lse, const float* target_logit, const float* inv_count, const float* dloss,
+                                           int D, int slices, const float* lse, const float* target_rest, const float* inv_count, const float* dloss,
                                            float* dX, float* dW, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!good_sizes(N, V, D, slices) || !X || !W || !target || !lse || !target_logit || !dloss || (!dX && !dW) || !workspace) return cudaErrorInvalidValue;
+    if (!good_sizes(N, V, D, slices) || !X || !W || !target || !lse || !target_rest || !dloss || (!dX && !dW) || !workspace) return cudaErrorInvalidValue;
     if (reduction < RGB200_REDUCE_NONE || reduction > RGB200_REDUCE_SUM || (reduction != RGB200_REDUCE_NONE && !inv_count)) return cudaErrorInvalidValue;
     BackwardLayout L;
     if (!backward_layout(N, V, D, slices, L)) return cudaErrorInvalidValue;
@@ -205,7 +205,7 @@ extern "C" int rgb200_linear_xent_backward(const float* X, const float* W, const
 
     if ((e = cudaMemsetAsync(ws, 0, L.maxima + (both ? maxima_bytes : 0), st)) != cudaSuccess) return e;
     if ((e = cudaMemsetAsync(first, 0x7F, (size_t)V * 8, st)) != cudaSuccess) return e;          // above every row and every complement of one
-    xent_rows_kernel<<<N, 128, 0, st>>>(target, ignore_index, V, D, lse, target_logit, dloss, reduction == RGB200_REDUCE_NONE, inv_count, W, weight, coefficient,
+    xent_rows_kernel<<<N, 128, 0, st>>>(target, ignore_index, V, D, target_rest, dloss, reduction == RGB200_REDUCE_NONE, inv_count, W, weight, coefficient,
                                         first, not_last, dX);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
 

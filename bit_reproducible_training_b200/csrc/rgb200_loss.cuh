@@ -16,10 +16,15 @@ __device__ __forceinline__ float2 lse_join(float2 a, float2 b) {
 }
 
 // One vocabulary piece's partial statistics [parts][rows] joined into the rows' running ones: a CTA owns 32 rows (lanes), warp k joins
-// parts k, k + 16, ... in order, then the warps' results in order.  last: also log-sum-exp and loss of each row.
+// parts k, k + 16, ... in order, then the warps' results in order.  last: also log-sum-exp and loss of each row, and in place of its target's logit
+// the probability of all words but the target.
+//
+// The maximum m is over all words, the sum over all but the target.  A confident row's loss and its target's gradient are as small as
+// the others' probability 1 - p; from p or from the log-sum-exp they would come out as a difference of numbers near 1 or near the logits: with logits
+// near 60 and 1 - p = 1e-5 a fifth of the value would be rounding, near 300 all of it.  As a sum of the others nothing cancels.
 static __global__ void __launch_bounds__(32 * XENT_WARPS)
 xent_join_kernel(const float2* __restrict__ parts, int count, float2* running, int rows, bool first, bool last, const long long* __restrict__ target,
-                 long long ignore, int vocab, const float* __restrict__ target_logit, float* lse, float* nll) {
+                 long long ignore, int vocab, float* target_rest, float* lse, float* nll) {
     __shared__ float2 joined[XENT_WARPS][XENT_ROWS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * XENT_ROWS + lane;
     float2 s = make_float2(-INFINITY, 0.0f);
@@ -34,11 +39,14 @@ xent_join_kernel(const float2* __restrict__ parts, int count, float2* running, i
     if (!first) s = lse_join(running[row], s);
     running[row] = s;
     if (!last) return;
-    const float l = s.x + logf(s.y);
-    lse[row] = l;
     const long long t = target[row];
-    // a target outside the vocabulary makes the row's loss NaN; an ignored one leaves it 0
-    nll[row] = t == ignore ? 0.0f : t < 0 || t >= vocab ? __int_as_float(0x7FC00000) : l - target_logit[row];
+    const bool word = t >= 0 && t < vocab;
+    const float z = word ? target_rest[row] : 0.0f, total = word ? s.y + expf(z - s.x) : s.y;
+    lse[row] = s.x + logf(total);
+    target_rest[row] = s.y / total;
+    // a target outside the vocabulary makes the row's loss NaN; an ignored one leaves it 0.  Where the target is the largest, total is 1 + s.y;
+    // elsewhere it is above 1, and all terms are positive
+    nll[row] = t == ignore ? 0.0f : !word ? __int_as_float(0x7FC00000) : (s.x - z) + (z == s.x ? log1pf(s.y) : logf(total));
 }
 
 // Sum of the rows' losses (in double, thread t adding rows t, t + 1024, ..., then a tree) over the number of rows that count.
@@ -70,17 +78,16 @@ xent_reduce_kernel(const float* __restrict__ nll, const long long* __restrict__ 
 }
 
 // One CTA a row: the row's weight g (the loss's gradient, over the number of rows for the mean; 0 for rows that do not count) and its
-// target's coefficient (p - 1) g; for the target word its first row and the complement of its last one (integer minima of words
+// target's coefficient (p - 1) g, from the sum of the others' probabilities; for the target word its first row and the complement of its last one (integer minima of words
 // that start at 0x7F7F7F7F: any order); and dX's start, coefficient times the target's row of W, to which the pieces' products are added.
 static __global__ void __launch_bounds__(128)
-xent_rows_kernel(const long long* __restrict__ target, long long ignore, int vocab, int dim, const float* __restrict__ lse,
-                 const float* __restrict__ target_logit, const float* __restrict__ dloss, bool per_row, const float* __restrict__ inv_count,
+xent_rows_kernel(const long long* __restrict__ target, long long ignore, int vocab, int dim, const float* __restrict__ target_rest, const float* __restrict__ dloss, bool per_row, const float* __restrict__ inv_count,
                  const float* __restrict__ W, float* weight, float* coefficient, int* first, int* not_last, float* dX) {
     const int i = blockIdx.x;
     const long long t = target[i];
     const bool counts = t != ignore && t >= 0 && t < vocab;
     const float g = counts ? (per_row ? dloss[i] : dloss[0] * *inv_count) : 0.0f;
-    const float c = counts ? (expf(target_logit[i] - lse[i]) - 1.0f) * g : 0.0f;
+    const float c = counts ? -target_rest[i] * g : 0.0f;
     if (threadIdx.x == 0) {
         weight[i] = g;
         coefficient[i] = c;

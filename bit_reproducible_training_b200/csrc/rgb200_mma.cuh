@@ -83,7 +83,7 @@ struct GemmTraits {
 enum Epilogue : int {
     EPI_NONE = 0,
     EPI_LINEAR = 1,     // bias, activation, residual
-    EPI_LSE = 2,        // nothing is stored but each row's maximum and sum of exponentials over the tile's columns
+    EPI_LSE = 2,        // nothing is stored but each row's target logit, maximum and sum of exponentials over the tile's columns
     EPI_PROB = 3        // softmax probabilities from the rows' log-sum-exp, scaled by row, zero at the row's target
 };
 struct EpilogueParams {
@@ -94,7 +94,7 @@ struct EpilogueParams {
     // cross entropy: columns are words first_word .. first_word + N - 1 of the vocabulary
     const long long* target;    // [M]
     long long first_word;
-    float2* lse_parts;          // [N / 32 rounded up][M]: maximum, sum of exp(value - maximum)
+    float2* lse_parts;          // [N / 32 rounded up][M]: maximum, sum of exp(value - maximum) without the target's
     float* target_logit;        // [M]
     const float* lse;           // [M]
     const float* row_scale;     // [M]

@@ -1,6 +1,6 @@
 """Cross entropy of the logits x @ weight.T against targets in pieces of the vocabulary, on the C ABI.
 
-The [tokens, vocabulary] logits are never stored: the forward pass keeps each row's log-sum-exp and target logit, the
+The [tokens, vocabulary] logits are never stored: the forward pass keeps each row's log-sum-exp and the others' share beside its target, the
 backward pass forms the probabilities of one piece of words at a time.  ``layers.linear_cross_entropy`` and
 ``layers.LinearCrossEntropy`` are the differentiable forms.  CUDA float32 only; there is no CPU path.
 """
@@ -41,7 +41,8 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean",
 
     loss: a scalar ("mean" over the rows whose target is not ignore_index, at least 1; or "sum"), or with "none" the rows'
     losses: 0 where the target is ignore_index and NaN, without a gradient, where it is outside the vocabulary otherwise.
-    stats: float32 [2 n + 1] for the backward call, the rows' log-sum-exp and target logits and the weight of a row."""
+    stats: float32 [2 n + 1] for the backward call, the rows' log-sum-exp, the probability of all words
+    but their target, and the weight of a row."""
     n, v, d = _sizes(x, weight, target, reduction, slices)
     shape = target.shape
     x, weight, target = _check(x, n * d, "x"), _check(weight, v * d, "weight"), target.contiguous()

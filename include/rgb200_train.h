@@ -53,21 +53,22 @@ int rgb200_linear_backward(const float* dY, const float* Z, const float* X, cons
 /* ------------------------------------------------------------------------------------------------
  * Cross entropy of the logits X W^T against targets, in pieces of the vocabulary: the [N, V] logits are never stored.
  * (The reference's cross entropy, repro_math_cuda/repro_softmax.cuh:8-49, takes stored logits.)
- * X [N, D], W [V, D], target [N] (int64).  Per row: lse = log sum exp(logits), nll = lse - logit of the target; 0 where the target is
+ * X [N, D], W [V, D], target [N] (int64).  Per row: lse = log sum exp(logits), target_rest = the probability of all words but the target
+ * (summed over them, so that it keeps its digits in a confident row), nll = lse - logit of the target; 0 where the target is
  * ignore_index; NaN, and no gradient, where it is any other value outside 0 .. V - 1.  Reductions: NONE leaves nll, SUM and
  * MEAN write *loss (MEAN divides by the number of rows that are not ignored, at least 1).
  * SUM and MEAN also write *inv_count, what the rows' weights are multiplied by (MEAN: the reciprocal count; SUM: 1).
- * Backward: dloss points to one value (SUM, MEAN) or N of them (NONE); lse, target_logit and inv_count are the forward call's.
+ * Backward: dloss points to one value (SUM, MEAN) or N of them (NONE); lse, target_rest and inv_count are the forward call's.
  *   dX = sum_j g p_j W_j - g W_target,  dW = sum_i g_i (p_i - onehot_i) x_i,  g the row's weight; either may be NULL.
  * The logits are the library's products (S = `slices`); sums are taken in an order that depends on the sizes and targets
  * alone.  D at most 105472 (S = 3).  Workspaces: 256-byte aligned, rgb200_linear_xent_workspace bytes (0: sizes not supported). */
 enum { RGB200_REDUCE_NONE = 0, RGB200_REDUCE_MEAN = 1, RGB200_REDUCE_SUM = 2 };
 size_t rgb200_linear_xent_workspace(int N, int V, int D, int slices, int backward);
 int rgb200_linear_xent_forward(const float* X, const float* W, const long long* target, long long ignore_index, int reduction, int N, int V,
-                               int D, int slices, float* loss, float* nll, float* lse, float* target_logit, float* inv_count,
+                               int D, int slices, float* loss, float* nll, float* lse, float* target_rest, float* inv_count,
                                void* workspace, size_t workspace_bytes, void* stream);
 int rgb200_linear_xent_backward(const float* X, const float* W, const long long* target, long long ignore_index, int reduction, int N, int V,
-                                int D, int slices, const float* lse, const float* target_logit, const float* inv_count, const float* dloss,
+                                int D, int slices, const float* lse, const float* target_rest, const float* inv_count, const float* dloss,
                                 float* dX, float* dW, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
