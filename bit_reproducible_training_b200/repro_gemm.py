@@ -332,13 +332,13 @@ def linear_backward(dY, Z, X, W, M, N, K, activation=None, slices=3, want_dx=Tru
     act = _activation(activation)
     _extent(M, N, K)
     dY, X, W = _check(dY, M * N, "dY"), _check(X, M * K, "X"), _check(W, N * K, "W")
+    if not (want_dx or want_dw or want_db):              # Z may be missing: the forward call keeps it for these three alone
+        return None, None, None
     if act and Z is None:
         raise ValueError("the activation's gradient needs Z")
     Z = _check(Z, M * N, "Z") if act else None
     if any(t is not None and t.device != dY.device for t in (Z, X, W)):
         raise ValueError("all tensors must be on one device")
-    if not (want_dx or want_dw or want_db):
-        return None, None, None
     L = _lib.lib()
     nbytes = L.rgb200_linear_backward_workspace(M, N, K, act, slices)
     if nbytes == 0:
