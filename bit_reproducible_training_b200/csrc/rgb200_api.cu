@@ -310,7 +310,7 @@ cudaError_t encode_c_store_map(CUtensorMap* map, float* C, int M, int N, int bat
 // not depend on - is still draining; the next ordinary launch of the stream waits for both, as stream order demands.
 template <int S, int W>
 cudaError_t launch_cluster_split(const CUtensorMap& map, const float* given_max, int8_t* planes, int* expo, int R, int K, int Kp,
-                                 int KC, int batch, int* status, bool overlap, cudaStream_t st) {
+                                 int KC, int batch, int* status, bool overlap, int nonfinite, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(KSC_CLUSTER * ceil_div(R, W), batch);
     cfg.blockDim = dim3(PREPASS_THREADS);
@@ -321,7 +321,7 @@ cudaError_t launch_cluster_split(const CUtensorMap& map, const float* given_max,
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = overlap ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, split_kstrided_cluster_kernel<S, W>, map, given_max, planes, expo, R, K, Kp, KC, status);
+    return cudaLaunchKernelEx(&cfg, split_kstrided_cluster_kernel<S, W>, map, given_max, planes, expo, R, K, Kp, KC, status, nonfinite);
 }
 
 // Whether a k-strided operand of R rows (16-byte aligned base and batch stride taken for granted) takes the cluster form.
@@ -332,7 +332,7 @@ bool cluster_split_fits(int R, int Kp) {
 
 template <int S>
 bool try_cluster_split(const float* src, const float* given_max, int8_t* planes, int* expo, int R, int K, int Kp, int batch,
-                       long long batch_stride, int* status, bool overlap, cudaStream_t st) {
+                       long long batch_stride, int* status, bool overlap, int nonfinite, cudaStream_t st) {
     if (R % 4 != 0 || (reinterpret_cast<uintptr_t>(src) & 15) != 0 || (batch > 1 && batch_stride % 4 != 0)) return false;
     if (!ensure_encode()) return false;
     const int KC = ceil_div(ceil_div(Kp, KSC_CLUSTER), KSC_BOX_K) * KSC_BOX_K;
@@ -345,9 +345,9 @@ bool try_cluster_split(const float* src, const float* given_max, int8_t* planes,
     CUtensorMap map;
     if (encode_kstrided_map(&map, src, R, K, batch, batch_stride, W) != cudaSuccess) return false;
     cudaError_t e;
-    if (W == 32) e = launch_cluster_split<S, 32>(map, given_max, planes, expo, R, K, Kp, KC, batch, status, overlap, st);
-    else if (W == 16) e = launch_cluster_split<S, 16>(map, given_max, planes, expo, R, K, Kp, KC, batch, status, overlap, st);
-    else e = launch_cluster_split<S, 8>(map, given_max, planes, expo, R, K, Kp, KC, batch, status, overlap, st);
+    if (W == 32) e = launch_cluster_split<S, 32>(map, given_max, planes, expo, R, K, Kp, KC, batch, status, overlap, nonfinite, st);
+    else if (W == 16) e = launch_cluster_split<S, 16>(map, given_max, planes, expo, R, K, Kp, KC, batch, status, overlap, nonfinite, st);
+    else e = launch_cluster_split<S, 8>(map, given_max, planes, expo, R, K, Kp, KC, batch, status, overlap, nonfinite, st);
     if (e != cudaSuccess) (void)cudaGetLastError();      // not launched: the caller falls back to the two-kernel form
     return e == cudaSuccess;
 }
@@ -357,9 +357,9 @@ bool try_cluster_split(const float* src, const float* given_max, int8_t* planes,
 // ------------------------------------------------------------------------------------------
 // Launches the k-contiguous split for one operand (second.src == nullptr) or for two operands of the same
 // row length in one grid.
-template <int S>
-void launch_kmajor(const KmajorOperand& first, const KmajorOperand& second, int K, int Kp, int batch, int* zero_word,
-                   cudaStream_t st) {
+template <int S, bool MARK>
+void launch_kmajor_as(const KmajorOperand& first, const KmajorOperand& second, int K, int Kp, int batch, int* zero_word,
+                      cudaStream_t st) {
     const bool two = second.src != nullptr;
     auto aligned_op = [&](const KmajorOperand& o) {
         return (K % 4 == 0) && ((reinterpret_cast<uintptr_t>(o.src) & 15) == 0) && (o.batch_stride % 4 == 0);
@@ -370,15 +370,15 @@ void launch_kmajor(const KmajorOperand& first, const KmajorOperand& second, int 
     do {                                                                                                      \
         const int rpc = PREPASS_THREADS / TPR;                                                                \
         const int b1 = ceil_div(first.R, rpc), b2 = two ? ceil_div(second.R, rpc) : 0;                        \
-        split_kmajor_kernel<S, TPR, CH, VEC><<<dim3(b1 + b2, batch), PREPASS_THREADS, 0, st>>>(               \
+        split_kmajor_kernel<S, TPR, CH, VEC, MARK><<<dim3(b1 + b2, batch), PREPASS_THREADS, 0, st>>>(               \
             first, second, b1, K, Kp, zero_word);                                                             \
     } while (0)
     if (aligned && Kp == 128) {                          // short rows: a small grid of warps, each walking over many rows
         const long long rows = (long long)first.R + (two ? second.R : 0);
         const long long want = (rows + 63) / 64;         // eight rows per warp at least
         const int ctas = (int)(want < 1 ? 1 : (want > PLAN_SM_COUNT * 8 ? PLAN_SM_COUNT * 8 : want));
-        if (K <= 64) split_kmajor_short_kernel<S, true><<<dim3(ctas, batch), PREPASS_THREADS, 0, st>>>(first, second, K, zero_word);
-        else split_kmajor_short_kernel<S, false><<<dim3(ctas, batch), PREPASS_THREADS, 0, st>>>(first, second, K, zero_word);
+        if (K <= 64) split_kmajor_short_kernel<S, true, MARK><<<dim3(ctas, batch), PREPASS_THREADS, 0, st>>>(first, second, K, zero_word);
+        else split_kmajor_short_kernel<S, false, MARK><<<dim3(ctas, batch), PREPASS_THREADS, 0, st>>>(first, second, K, zero_word);
         return;
     }
     if (!aligned || nq > 256 * KMAJOR_MAX_CHUNKS) {      // general path: any K, any alignment; row group sized to the row
@@ -396,31 +396,43 @@ void launch_kmajor(const KmajorOperand& first, const KmajorOperand& second, int 
     else RGB_KMAJOR(256, 16, true);
 #undef RGB_KMAJOR
 }
+template <int S>
+void launch_kmajor(const KmajorOperand& first, const KmajorOperand& second, int K, int Kp, int batch, int* zero_word,
+                   NonFinite nonfinite, cudaStream_t st) {
+    if (nonfinite == NF_MARK) launch_kmajor_as<S, true>(first, second, K, Kp, batch, zero_word, st);
+    else launch_kmajor_as<S, false>(first, second, K, Kp, batch, zero_word, st);
+}
+
+void launch_colmax(const float* src, uint32_t* maxbits, int R, int K, int batch, long long batch_stride, NonFinite nonfinite, cudaStream_t st) {
+    const int chunks = ceil_div(K, COLMAX_K_PER_CTA);
+    const dim3 grid(ceil_div(R, 128), chunks < COLMAX_MAX_GRID_Y ? chunks : COLMAX_MAX_GRID_Y, batch);
+    if (nonfinite == NF_UNDEFINED) colmax_kstrided_kernel<false><<<grid, PREPASS_THREADS, 0, st>>>(src, maxbits, R, K, batch_stride, 0.0f);
+    else colmax_kstrided_kernel<true><<<grid, PREPASS_THREADS, 0, st>>>(src, maxbits, R, K, batch_stride, nonfinite == NF_MARK ? INFINITY : 0.0f);
+}
 
 // One operand through the pre-pass.  k_major: element (r, k) at src[r*K + k].
 template <int S>
 void launch_split(const float* src, bool k_major, const float* given_max, uint32_t* maxbits, int8_t* planes, int* expo,
                   int R, int K, int Kp, int batch, long long batch_stride, int* status, cudaStream_t st, bool overlap = false,
-                  bool zero_maxima = false /* maxbits has not been zeroed: done here if it is needed */) {
+                  bool zero_maxima = false /* maxbits has not been zeroed: done here if it is needed */, NonFinite nonfinite = NF_UNDEFINED) {
     if (k_major) {
         const KmajorOperand op{src, given_max, planes, expo, R, batch_stride};
         const KmajorOperand none{nullptr, nullptr, nullptr, nullptr, 0, 0};
-        launch_kmajor<S>(op, none, K, Kp, batch, nullptr, st);
-    } else if (try_cluster_split<S>(src, given_max, planes, expo, R, K, Kp, batch, batch_stride, status, overlap, st)) {
+        launch_kmajor<S>(op, none, K, Kp, batch, nullptr, nonfinite, st);
+    } else if (try_cluster_split<S>(src, given_max, planes, expo, R, K, Kp, batch, batch_stride, status, overlap, nonfinite, st)) {
         // one read of the operand; the zeroed maxima words stay unused
     } else {
         if (zero_maxima && !given_max) (void)cudaMemsetAsync(maxbits, 0, (size_t)batch * R * sizeof(uint32_t), st);   // an error shows at the launches' check
         if (given_max)
             maxima_to_bits_kernel<<<ceil_div(batch * R, 256), 256, 0, st>>>(given_max, maxbits, batch * R);
         else
-            colmax_kstrided_kernel<<<dim3(ceil_div(R, 128), (ceil_div(K, COLMAX_K_PER_CTA) < COLMAX_MAX_GRID_Y ? ceil_div(K, COLMAX_K_PER_CTA) : COLMAX_MAX_GRID_Y), batch), PREPASS_THREADS, 0, st>>>(
-                src, maxbits, R, K, batch_stride);
+            launch_colmax(src, maxbits, R, K, batch, batch_stride, nonfinite, st);
         // about eight CTAs per SM in total; each walks over the k tiles of its 32 rows
         const int r_blocks = ceil_div(R, 32), k_tiles = Kp / BLOCK_K;
         int walkers = ceil_div(PLAN_SM_COUNT * 8, r_blocks * batch);
         walkers = walkers < 1 ? 1 : (walkers > k_tiles ? k_tiles : walkers);
         split_kstrided_kernel<S><<<dim3(r_blocks, walkers, batch), PREPASS_THREADS, 0, st>>>(
-            src, maxbits, planes, expo, R, K, Kp, batch_stride);
+            src, maxbits, planes, expo, R, K, Kp, batch_stride, nonfinite == NF_MARK);
     }
 }
 
@@ -467,6 +479,7 @@ struct RunArgs {
     bool reuse_a = false;      // op(A)'s planes and exponents are in place (see Prepared in rgb200_gemm.h)
     int* status = nullptr;     // a word of the caller's in place of the workspace's (see Prepared)
     bool zero_status = true;
+    NonFinite nonfinite_a = NF_UNDEFINED, nonfinite_b = NF_UNDEFINED;
     // An epilogue behind the rounding (see Epilogue); such a product takes the general kernel whatever its shape.
     int epi = EPI_NONE;
     const EpilogueParams* epi_params = nullptr;
@@ -499,7 +512,7 @@ cudaError_t run(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
         if (!a.reuse_b) {
             if ((e = cudaMemsetAsync(a.ws, 0, L.zero_b_bytes, a.st)) != cudaSuccess) return e;   // status word + column maxima of B
             record(0);
-            launch_split<S>(a.B, a.trans_b, a.max_b, max_b, qb, eb, L.N, L.K, L.Kp, L.batch, a.stride_b, status, a.st);
+            launch_split<S>(a.B, a.trans_b, a.max_b, max_b, qb, eb, L.N, L.K, L.Kp, L.batch, a.stride_b, status, a.st, false, false, a.nonfinite_b);
         } else {
             record(0);
         }
@@ -510,7 +523,7 @@ cudaError_t run(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
         RowFusedParams Q;
         Q.expo_b = eb; Q.C = a.C; Q.status = status;
         Q.M = L.M; Q.N = L.N; Q.K = L.K; Q.batch = L.batch; Q.stride_c = a.stride_c;
-        Q.m_tiles = ceil_div(L.M, BLOCK_M); Q.k_blocks = L.k_blocks; Q.e0 = e0;
+        Q.m_tiles = ceil_div(L.M, BLOCK_M); Q.k_blocks = L.k_blocks; Q.e0 = e0; Q.mark = a.nonfinite_a == NF_MARK;
         const long long rf_tiles = (long long)L.batch * Q.m_tiles;
         const int rf_grid = (int)(rf_tiles < dev.sm_count ? rf_tiles : dev.sm_count);
         gemm_i8_rowfused_kernel<S><<<rf_grid, RF_THREADS, RowFusedTraits<S>::SMEM_BYTES, a.st>>>(map_a, map_b, Q);
@@ -530,22 +543,22 @@ cudaError_t run(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
         record(0);
         if (!a.reuse_b && both_kmajor) {
             const KmajorOperand opb{a.B, a.max_b, qb, eb, L.N, a.stride_b}, none{nullptr, nullptr, nullptr, nullptr, 0, 0};
-            launch_kmajor<S>(opb, none, L.K, L.Kp, L.batch, clear_status, a.st);
+            launch_kmajor<S>(opb, none, L.K, L.Kp, L.batch, clear_status, a.nonfinite_b, a.st);
         } else if (!a.reuse_b) {
-            launch_split<S>(a.B, a.trans_b, a.max_b, max_b, qb, eb, L.N, L.K, L.Kp, L.batch, a.stride_b, status, a.st, false, true);
+            launch_split<S>(a.B, a.trans_b, a.max_b, max_b, qb, eb, L.N, L.K, L.Kp, L.batch, a.stride_b, status, a.st, false, true, a.nonfinite_b);
         }
         record(1);
     } else if (a.reuse_b) {
         // B's planes and exponents are those of the previous call on this workspace (same N, K, S): only A is split
         if (a.trans_a && (e = cudaMemsetAsync(a.ws + L.max_a, 0, L.zero_a_bytes, a.st)) != cudaSuccess) return e;
         record(0);
-        launch_split<S>(a.A, !a.trans_a, a.max_a, max_a, qa, ea, L.M, L.K, L.Kp, L.batch, a.stride_a, status, a.st);
+        launch_split<S>(a.A, !a.trans_a, a.max_a, max_a, qa, ea, L.M, L.K, L.Kp, L.batch, a.stride_a, status, a.st, false, false, a.nonfinite_a);
         record(1);
     } else if (both_kmajor) {
         record(0);
         const KmajorOperand opa{a.A, a.max_a, qa, ea, L.M, a.stride_a};
         const KmajorOperand opb{a.B, a.max_b, qb, eb, L.N, a.stride_b};
-        launch_kmajor<S>(opa, opb, L.K, L.Kp, L.batch, clear_status, a.st);
+        launch_kmajor<S>(opa, opb, L.K, L.Kp, L.batch, clear_status, a.nonfinite_a, a.st);      // the same for both
         record(1);
     } else {
         if ((e = cudaMemsetAsync(a.ws, 0, L.zero_b_bytes, a.st)) != cudaSuccess) return e;   // status word + column maxima of B
@@ -553,8 +566,8 @@ cudaError_t run(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
         record(0);
         // both splits on the caller's stream, one after the other: each saturates the memory system by itself, and
         // the library keeps no stream or event of its own
-        launch_split<S>(a.A, !a.trans_a, a.max_a, max_a, qa, ea, L.M, L.K, L.Kp, L.batch, a.stride_a, status, a.st);
-        launch_split<S>(a.B, a.trans_b, a.max_b, max_b, qb, eb, L.N, L.K, L.Kp, L.batch, a.stride_b, status, a.st, true);
+        launch_split<S>(a.A, !a.trans_a, a.max_a, max_a, qa, ea, L.M, L.K, L.Kp, L.batch, a.stride_a, status, a.st, false, false, a.nonfinite_a);
+        launch_split<S>(a.B, a.trans_b, a.max_b, max_b, qb, eb, L.N, L.K, L.Kp, L.batch, a.stride_b, status, a.st, true, false, a.nonfinite_b);
         record(1);
     }
 
@@ -691,6 +704,8 @@ cudaError_t gemm_with_epilogue(const float* A, const float* B, float* C, int M, 
     a.epi_params = &E;
     a.reuse_a = prepared.a;
     a.reuse_b = prepared.b;
+    a.nonfinite_a = prepared.nonfinite_a;
+    a.nonfinite_b = prepared.nonfinite_b;
     if (prepared.status) { a.status = prepared.status; a.zero_status = prepared.zero_status; }
     return dispatch(L, a, *dev);
 }
@@ -1254,8 +1269,7 @@ int rgb200_absmax(const float* X, int R, int K, int k_strided, float* out, void*
     } else {
         // non-negative floats order like their bit patterns: accumulate the maxima in place as integers
         if ((e = cudaMemsetAsync(out, 0, (size_t)R * sizeof(float), st)) != cudaSuccess) return e;
-        colmax_kstrided_kernel<<<dim3(ceil_div(R, 128), (ceil_div(K, COLMAX_K_PER_CTA) < COLMAX_MAX_GRID_Y ? ceil_div(K, COLMAX_K_PER_CTA) : COLMAX_MAX_GRID_Y), 1), PREPASS_THREADS, 0, st>>>(
-            X, reinterpret_cast<uint32_t*>(out), R, K, 0);
+        launch_colmax(X, reinterpret_cast<uint32_t*>(out), R, K, 1, 0, NF_UNDEFINED, st);
     }
     return cudaGetLastError();
 }

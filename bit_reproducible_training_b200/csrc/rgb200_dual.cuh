@@ -4,6 +4,7 @@
 // The gradient of a linear layer needs its dZ both ways (dX = dZ W, dW = dZ^T X), the cross entropy its piece of probabilities.
 // Two pre-passes read the matrix once each and find the maxima themselves; here the kernel that produces the matrix has left
 // the maxima of its rows and columns, and one read serves both.  Same exponents, same digits: the products' bits do not change.
+// A maximum that is not finite marks its row or column (NF_MARK).
 // Bound: HBM, (4 + 2 S) bytes a value; beside it about 45 instructions a value.  A CTA turns a 128 x 64 tile: eight 16-byte loads
 // a thread, the row digits straight from the registers, then the tile through shared memory (quads exchanged by row, so that
 // neither side meets bank conflicts) and 32 values of one column a thread, one 32-byte store a plane.
@@ -14,10 +15,11 @@
 namespace rgb200 {
 
 constexpr int DUAL_ROWS = 128, DUAL_COLS = 64, DUAL_THREADS = 256;
+constexpr uint32_t INFINITY_BITS = 0x7F800000u;          // NaN counts as an infinity
 
 struct DualParams {
     const float* src;               // [R][C], rows ld apart
-    const uint32_t *row_max, *col_max;      // bits of the largest magnitudes
+    const uint32_t *row_max, *col_max;      // bits of the largest magnitudes (as integers: infinities and NaN lie above all others)
     int8_t *row_planes, *col_planes;        // [S][R][Cp], [S][C][Rp]
     int *row_expo, *col_expo;
     int R, C, ld, Rp, Cp;
@@ -60,13 +62,15 @@ split_both_kernel(const DualParams P) {
         }
     }
     if (t < DUAL_ROWS) {
-        const int row = r0 + t, e = row < P.R ? scale_exponent(bits_f32(P.row_max[row])) : 0;
+        const int row = r0 + t;
+        const int e = row < P.R ? scale_exponent(bits_f32(min(P.row_max[row], INFINITY_BITS))) : 0;
         row_e[t] = e;
-        if (row < P.R && col_tile == 0) P.row_expo[row] = e;
+        if (row < P.R && col_tile == 0) P.row_expo[row] = recorded_expo(e, true);
     } else if (t < DUAL_ROWS + DUAL_COLS) {
-        const int j = t - DUAL_ROWS, c = c0 + j, e = c < P.C ? scale_exponent(bits_f32(P.col_max[c])) : 0;
+        const int j = t - DUAL_ROWS, c = c0 + j;
+        const int e = c < P.C ? scale_exponent(bits_f32(min(P.col_max[c], INFINITY_BITS))) : 0;
         col_e[j] = e;
-        if (c < P.C && row_tile == 0) P.col_expo[c] = e;
+        if (c < P.C && row_tile == 0) P.col_expo[c] = recorded_expo(e, true);
     }
     __syncthreads();
     const size_t row_plane = (size_t)P.R * P.Cp, col_plane = (size_t)P.C * P.Rp;

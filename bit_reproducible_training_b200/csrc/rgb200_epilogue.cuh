@@ -5,13 +5,15 @@
 //   EPI_PROB     row_scale[row] * exp(c - lse[row]), zero at the row's target word.
 //
 // c is the product rounded once to FP32, as the plain entry points return it; every step after it is one FP32 operation in a
-// fixed order, so the bits do not depend on the tiling (EPI_LSE: on the tile width alone).
+// fixed order, so the bits do not depend on the tiling (EPI_LSE: on the tile width alone).  c is NaN where its row or column is marked
+// as not finite, and the maxima left for a split keep NaN.
 //
 // Why here: an output costs 4 bytes of HBM written by the product and 8 more for every elementwise pass behind it.  In
 // the kernel the extra work of a thread (16 or 32 columns of one row) overlaps the next tile's MMAs, which take about 1150 clocks for each
 // 128 values of k; the residual and the bias are requested before the wait for the accumulators.
 #pragma once
 #include "rgb200_mma.cuh"
+#include "rgb200_prepass.cuh"
 
 namespace rgb200 {
 
@@ -196,12 +198,12 @@ struct EpilogueRow<EPI_PROB, CPT> {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {          // a row without a weight takes no part, whatever its logits are
                 p[i] = j + i == target || scale == 0.0f || col0 + j + i >= P.N ? 0.0f : __expf(p[i] - lse) * scale;
-                row_top = fmaxf(row_top, fabsf(p[i]));
+                row_top = max_nan(row_top, fabsf(p[i]));
             }
             if (P.epi.col_max) {                   // rows that do not exist have no weight and join as zeros
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const unsigned top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(fmaxf(0.0f, fabsf(p[i]))));
+                    const unsigned top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(fabsf(p[i])));     // NaN is the largest
                     if ((threadIdx.x & 31) == j + i) col_top = top;
                 }
             }
@@ -242,7 +244,7 @@ round_partial_linear_kernel(const long long* __restrict__ partial, int parts, co
             float z[W], y[W];
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                z[j] = bits_f32(round_to_f32_bits(t[j], e_r + eb[c + j]));
+                z[j] = bits_f32(round_or_nan(t[j], e_r + eb[c + j]));
                 if (E.bias) z[j] += E.bias[c + j];
                 y[j] = activation<decltype(act)::value>(z[j]);
             }
@@ -329,7 +331,7 @@ activation_backward_kernel(const ActBackwardParams P) {
                 for (int j = 0; j < 4; ++j) {
                     if (ACT != ACT_NONE) d[i][j] = d[i][j] * activation_slope<ACT>(z[i][j]);
                     s[j] += d[i][j];
-                    top[j] = fmaxf(top[j], fabsf(d[i][j]));
+                    top[j] = max_nan(top[j], fabsf(d[i][j]));
                 }
                 if (P.dz) {
                     if (wide) {
@@ -341,7 +343,7 @@ activation_backward_kernel(const ActBackwardParams P) {
                     }
                 }
                 if (P.row_max) {
-                    const float m = fmaxf(fmaxf(fabsf(d[i][0]), fabsf(d[i][1])), fmaxf(fabsf(d[i][2]), fmaxf(fabsf(d[i][3]), 0.0f)));
+                    const float m = max_nan(max_nan(fabsf(d[i][0]), fabsf(d[i][1])), max_nan(fabsf(d[i][2]), fabsf(d[i][3])));
                     const unsigned all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m));
                     if (lane == 0) atomicMax(P.row_max + row, all);
                 }
@@ -356,7 +358,7 @@ activation_backward_kernel(const ActBackwardParams P) {
         if (c < ACTB_COLS && out < P.N) {
             float m = sums[0][c];
 #pragma unroll
-            for (int k = 1; k < ACTB_WARPS; ++k) m = fmaxf(m, sums[k][c]);
+            for (int k = 1; k < ACTB_WARPS; ++k) m = max_nan(m, sums[k][c]);
             atomicMax(P.col_max + out, __float_as_uint(m));
         }
         __syncthreads();

@@ -7,6 +7,15 @@ namespace rgb200 {
 
 struct EpilogueParams;
 
+// What the split of an operand does with infinities and NaN.  The plain products define their bits for finite values alone: a NaN is left out of
+// its row's maximum, and the digits of either are whatever their bits give.  The operators of a training step must not turn them into
+// finite losses and gradients.
+enum NonFinite : int {
+    NF_UNDEFINED = 0,   // the plain products
+    NF_MARK = 1,        // a row that holds one is recorded with NONFINITE_EXPO: every output it takes part in is NaN
+    NF_DROP = 2         // they do not count for the row's scale; for an operand whose partner holds zeros there (k-strided operands only)
+};
+
 // What gemm_with_epilogue may take as prepared in its workspace.
 struct Prepared {
     // op(A)'s digit planes and exponents are in place: from a call with the same M, N, K, slices and transposition, or written
@@ -19,6 +28,8 @@ struct Prepared {
     // both operands k-contiguous) or by the caller.
     int* status = nullptr;
     bool zero_status = false;
+    // how this call splits op(A) and op(B), where it does
+    NonFinite nonfinite_a = NF_MARK, nonfinite_b = NF_MARK;
 };
 
 // Where a product's workspace holds op(A): planes [slices][M][k_padded] and exponents [M].

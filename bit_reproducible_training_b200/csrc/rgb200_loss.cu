@@ -234,10 +234,13 @@ extern "C" int rgb200_linear_xent_backward(const float* X, const float* W, const
                 return e;
             if ((e = launch_split_both(slices, P, E.ldc, N, words, E.row_max, E.col_max, rows, cols, st)) != cudaSuccess) return e;
         }
-        if (dX && (e = gemm_with_epilogue(P, Wp, dX, N, D, words, cx, EPI_LINEAR, add, Prepared{both, false, status}, ws + L.dx, L.dx_bytes, st)) != cudaSuccess)
+        // A row that counts and meets a value that is not finite has a P of NaN; X and W need no marks of their own, and must not have them: the rows
+        // that do not count take no part, whatever they hold
+        if (dX && (e = gemm_with_epilogue(P, Wp, dX, N, D, words, cx, EPI_LINEAR, add, Prepared{both, false, status, false, NF_MARK, NF_UNDEFINED}, ws + L.dx,
+                                          L.dx_bytes, st)) != cudaSuccess)
             return e;
-        if (dW && (e = gemm_with_epilogue(P, X, dW + (size_t)at * D, words, D, N, cw, EPI_NONE, add, Prepared{both, at > 0, status}, ws + L.dw, L.dw_bytes, st)) !=
-                      cudaSuccess)
+        if (dW && (e = gemm_with_epilogue(P, X, dW + (size_t)at * D, words, D, N, cw, EPI_NONE, add, Prepared{both, at > 0, status, false, NF_MARK, NF_DROP},
+                                          ws + L.dw, L.dw_bytes, st)) != cudaSuccess)
             return e;
     }
     if (dW) {

@@ -8,10 +8,10 @@ namespace rgb200 {
 
 constexpr int XENT_ROWS = 32, XENT_WARPS = 16;
 
-// (maximum, sum of exp(value - maximum)) of two sets of values; an empty set is (-inf, 0).
+// (maximum, sum of exp(value - maximum)) of two sets of values; an empty set is (-inf, 0), one of NaN alone (-inf, NaN).
 __device__ __forceinline__ float2 lse_join(float2 a, float2 b) {
     const float top = fmaxf(a.x, b.x);
-    if (top == -INFINITY) return make_float2(top, 0.0f);
+    if (top == -INFINITY) return make_float2(top, a.y + b.y);
     return make_float2(top, a.y * expf(a.x - top) + b.y * expf(b.x - top));
 }
 

@@ -106,6 +106,11 @@ RGB_HD int max_k_per_pass(int S) {
     return S == 1 ? 133143 : (S == 2 ? 132103 : 105516);   // floor((2^31 - 1) / bound), minus one for slack
 }
 
+// Exponent recorded for a row whose values are not all finite, where the split is asked to mark it (NonFinite in rgb200_gemm.h).  It is far
+// outside of what finite rows add up to (below 256), so every kernel's range check sends the outputs of such a row to the exact
+// rounding, round_or_nan.
+constexpr int NONFINITE_EXPO = 1 << 20;
+
 RGB_HD uint64_t shr_rne(uint64_t m, int s) {   // s in [1, 63]
     uint64_t q = m >> s, rest = m & ((1ull << s) - 1), half = 1ull << (s - 1);
     return q + ((rest > half || (rest == half && (q & 1))) ? 1 : 0);
@@ -154,10 +159,13 @@ RGB_HD uint32_t round_to_f32_bits(long long T, int E) {
 #endif
 }
 
+// The same where rows may be marked: their outputs are NaN.
+RGB_HD uint32_t round_or_nan(long long T, int E) { return E > NONFINITE_EXPO / 2 ? 0x7FC00000u : round_to_f32_bits(T, E); }
+
 #ifdef __CUDA_ARCH__
 // Branch-free common case of round_to_f32_bits for unrolled epilogues: returns the result that is
 // valid when *ok stays true (the scaled value is a non-zero normal number); the caller redoes the
-// few outputs with ok == false through round_to_f32_bits.  Keeping branches out of the per-output
+// few outputs with ok == false through round_or_nan.  Keeping branches out of the per-output
 // code lets the compiler interleave the independent outputs of a thread.  The signed hardware conversion
 // rounds the magnitude to nearest-even and carries the sign (round-to-nearest-even is symmetric in the
 // sign), so neither the absolute value nor the sign bit has to be formed separately.

@@ -364,7 +364,7 @@ __device__ __forceinline__ void cursor_next(KCursor& c, const GemmParams& P, lon
 
 __device__ __forceinline__ float sum_to_float(long long t) { return __ll2float_rn(t); }
 __device__ __forceinline__ float sum_to_float(int t) { return __int2float_rn(t); }
-static __device__ __noinline__ float round_to_f32_rare(long long t, int e) { return __uint_as_float(round_to_f32_bits(t, e)); }
+static __device__ __noinline__ float round_to_f32_rare(long long t, int e) { return __uint_as_float(round_or_nan(t, e)); }
 
 // One thread's columns of the finished tile through an epilogue; defined in rgb200_epilogue.cuh, which only the
 // translation unit that builds those kernels includes.
@@ -603,10 +603,10 @@ gemm_i8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                     r[2] = round_to_f32_bits_signed(T[j + 2], ebase + eb_s[j + 2], &k2);
                     r[3] = round_to_f32_bits_signed(T[j + 3], ebase + eb_s[j + 3], &k3);
                     if (!(k0 && k1 && k2 && k3)) {          // zero, subnormal or overflowing results: exact path
-                        r[0] = round_to_f32_bits(T[j + 0], ebase + eb_s[j + 0]);
-                        r[1] = round_to_f32_bits(T[j + 1], ebase + eb_s[j + 1]);
-                        r[2] = round_to_f32_bits(T[j + 2], ebase + eb_s[j + 2]);
-                        r[3] = round_to_f32_bits(T[j + 3], ebase + eb_s[j + 3]);
+                        r[0] = round_or_nan(T[j + 0], ebase + eb_s[j + 0]);
+                        r[1] = round_or_nan(T[j + 1], ebase + eb_s[j + 1]);
+                        r[2] = round_or_nan(T[j + 2], ebase + eb_s[j + 2]);
+                        r[3] = round_or_nan(T[j + 3], ebase + eb_s[j + 3]);
                     }
                 };
                 if (IMAGE_MAJOR_C) {
@@ -756,7 +756,7 @@ round_partial_kernel(const long long* __restrict__ partial, int parts, size_t pa
 #pragma unroll
         for (int j = 0; j < W; ++j) {
             const int e_c = eb ? eb[b * N + c + j] : scale_exponent(max_b[b * N + c + j]);
-            o[j] = round_to_f32_bits(t[j], e_r + e_c);
+            o[j] = round_or_nan(t[j], e_r + e_c);
         }
         float* dst = C + b * (size_t)stride_c + (size_t)r * N + c;
         if (VEC) *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[W > 1 ? 1 : 0], o[W > 2 ? 2 : 0], o[W > 3 ? 3 : 0]);

@@ -9,6 +9,7 @@
 // Reference counterparts: quantize_kmajor / quantize_kstrided (repro_gemm_cuda/repro_gemm.cu:54-121),
 // which read every operand twice with scalar loads and one block per row or 32 rows.
 #pragma once
+#include "rgb200_gemm.h"
 #include "rgb200_math.cuh"
 
 namespace rgb200 {
@@ -19,6 +20,23 @@ constexpr int KMAJOR_MAX_CHUNKS = 16;     // most float4 chunks a thread keeps i
 __device__ __forceinline__ float abs4max(float m, float4 v) {
     return fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
 }
+
+// The same for rows that are marked (NF_MARK): max.NaN keeps a NaN at no extra cost, and behind a thread's own values a NaN counts as an
+// infinity, which the plain maxima behind it keep.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float abs4max_nan(float m, float4 v) {
+    return max_nan(max_nan(m, max_nan(fabsf(v.x), fabsf(v.y))), max_nan(fabsf(v.z), fabsf(v.w)));
+}
+__device__ __forceinline__ float nan_to_infinity(float m) { return m < INFINITY ? m : INFINITY; }
+// |x| for the maxima of an operand whose values that are not finite count as `stand_in`: infinity (NF_MARK) or zero (NF_DROP).
+__device__ __forceinline__ float abs_or(float x, float stand_in) { return fabsf(x) < INFINITY ? fabsf(x) : stand_in; }
+__device__ __forceinline__ float nonfinite_stand_in(int nonfinite) { return nonfinite == NF_MARK ? INFINITY : 0.0f; }
+// The exponent to record for a row with scale exponent e: that of a finite row is at most 122, an infinite maximum has 128.
+__device__ __forceinline__ int recorded_expo(int e, bool mark) { return mark && e > 127 ? NONFINITE_EXPO : e; }
 
 // Fixed-point value of x plus the digit bias, Y = X + 64 * (128^(S-2) + ... + 1), by float arithmetic:
 // clamp in float (RNE commutes with clamping to an integer), then add 1.5 * 2^23 so that the FP32
@@ -110,8 +128,9 @@ struct KmajorOperand {
 // The kernel takes up to two operands of the same row length (op(A) and op(B)^T of one product when
 // both are stored k-contiguous): blocks [0, blocks_first) work on `first`, the rest on `second`, so
 // the forward GEMM of a linear layer needs one pre-pass launch.  `zero_word`, if not null, is cleared
-// by one thread (the workspace's status word, when no memset precedes this launch).
-template <int S, int TPR, int CHUNKS, bool VEC>
+// by one thread (the workspace's status word, when no memset precedes this launch).  MARK: NF_MARK for both operands; a kernel of
+// its own, so that the plain products' keep their registers.
+template <int S, int TPR, int CHUNKS, bool VEC, bool MARK>
 __device__ __forceinline__ void split_kmajor_body(const KmajorOperand& first, const KmajorOperand& second, int blocks_first,
                                                   int K, int Kp, int* zero_word) {
     __shared__ float red[PREPASS_THREADS / 32];
@@ -143,13 +162,19 @@ __device__ __forceinline__ void split_kmajor_body(const KmajorOperand& first, co
             int c = t + i * TPR;
             v[i] = (live && c < nq) ? __ldg(a4 + c) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
+        if (MARK) {
 #pragma unroll
-        for (int i = 0; i < CHUNKS; ++i) m = abs4max(m, v[i]);
+            for (int i = 0; i < CHUNKS; ++i) m = abs4max_nan(m, v[i]);
+            m = nan_to_infinity(m);
+        } else {
+#pragma unroll
+            for (int i = 0; i < CHUNKS; ++i) m = abs4max(m, v[i]);
+        }
         m = row_group_max<TPR>(m, red);
         if (!live) return;
         if (given_max) m = given_max[(size_t)b * R + row];
         const int e = scale_exponent(m);
-        if (t == 0) expo[(size_t)b * R + row] = e;
+        if (t == 0) expo[(size_t)b * R + row] = recorded_expo(e, MARK);
         const QuantScale q = quant_scale(e, S);
         if (plain_row(e)) {                      // uniform over the row group
 #pragma unroll
@@ -165,13 +190,19 @@ __device__ __forceinline__ void split_kmajor_body(const KmajorOperand& first, co
             }
         }
     } else {
-        if (live && !given_max)
-            for (int k = t; k < K; k += TPR) m = fmaxf(m, fabsf(__ldg(a + k)));
+        if (live && !given_max) {
+            if (MARK) {
+                for (int k = t; k < K; k += TPR) m = max_nan(m, fabsf(__ldg(a + k)));
+                m = nan_to_infinity(m);
+            } else {
+                for (int k = t; k < K; k += TPR) m = fmaxf(m, fabsf(__ldg(a + k)));
+            }
+        }
         m = row_group_max<TPR>(m, red);
         if (!live) return;
         if (given_max) m = given_max[(size_t)b * R + row];
         const int e = scale_exponent(m);
-        if (t == 0) expo[(size_t)b * R + row] = e;
+        if (t == 0) expo[(size_t)b * R + row] = recorded_expo(e, MARK);
         const QuantScale q = quant_scale(e, S);
         for (int k = t * 4; k < Kp; k += TPR * 4) {
             float4 v;
@@ -188,12 +219,12 @@ __device__ __forceinline__ void split_kmajor_body(const KmajorOperand& first, co
 // serialization start early (the other operand's split, which does not depend on it), and, when it is itself
 // launched that way, does not complete before the kernel in front of it has: the ordinary launch that follows
 // (the MMA kernel) then finds both operands' planes complete.  Both instructions do nothing in an ordinary launch.
-template <int S, int TPR, int CHUNKS, bool VEC>
+template <int S, int TPR, int CHUNKS, bool VEC, bool MARK>
 __global__ void __launch_bounds__(PREPASS_THREADS)
 split_kmajor_kernel(const KmajorOperand first, const KmajorOperand second, int blocks_first,
                     int K, int Kp, int* zero_word) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    split_kmajor_body<S, TPR, CHUNKS, VEC>(first, second, blocks_first, K, Kp, zero_word);
+    split_kmajor_body<S, TPR, CHUNKS, VEC, MARK>(first, second, blocks_first, K, Kp, zero_word);
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
@@ -203,7 +234,7 @@ split_kmajor_kernel(const KmajorOperand first, const KmajorOperand second, int b
 // one row per warp the launch of tens of thousands of tiny CTAs costs more than the rows' traffic.  Four row
 // slots are in flight per warp.  Same two-operand convention as split_kmajor_kernel.
 // grid = (CTAs, batch); any CTA count works.
-template <int S, bool HALF>
+template <int S, bool HALF, bool MARK>
 __global__ void __launch_bounds__(PREPASS_THREADS)
 split_kmajor_short_kernel(const KmajorOperand first, const KmajorOperand second, int K, int* zero_word) {
     constexpr int KP = 128;
@@ -233,13 +264,13 @@ split_kmajor_short_kernel(const KmajorOperand first, const KmajorOperand second,
         return c < nq ? __ldg(reinterpret_cast<const float4*>(x.src) + c) : make_float4(0.f, 0.f, 0.f, 0.f);
     };
     auto finish = [&](const RowRef& x, float4 v, bool valid) {
-        float m = abs4max(0.0f, v);
+        float m = MARK ? nan_to_infinity(abs4max_nan(0.0f, v)) : abs4max(0.0f, v);
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));     // over the row's lanes
         if (!valid) return;
         if (x.given_max) m = x.given_max[(size_t)b * x.R + x.r];
         const int e = scale_exponent(m);
-        if (c == 0) x.expo[(size_t)b * x.R + x.r] = e;
+        if (c == 0) x.expo[(size_t)b * x.R + x.r] = recorded_expo(e, MARK);
         const size_t plane_stride = (size_t)x.R * KP;
         int8_t* out = x.planes + (size_t)b * S * plane_stride + (size_t)x.r * KP;
         store_quad<S>(v, quant_scale(e, S), plain_row(e), out, plane_stride, (size_t)c * 4);
@@ -275,9 +306,12 @@ split_kmajor_short_kernel(const KmajorOperand first, const KmajorOperand second,
 constexpr int COLMAX_K_PER_CTA = 64;
 constexpr int COLMAX_MAX_GRID_Y = 65535;       // hardware limit on gridDim.y; longer K is walked by the CTAs
 
+// SELECT: values that are not finite count as `stand_in` (see abs_or); else NaN is left out and infinities are as they are.
+template <bool SELECT>
 static __global__ void __launch_bounds__(PREPASS_THREADS)
 colmax_kstrided_kernel(const float* __restrict__ src, uint32_t* __restrict__ maxbits, int R, int K,
-                       long long src_batch_stride) {
+                       long long src_batch_stride, float stand_in) {
+    auto mag = [&](float x) { return SELECT ? abs_or(x, stand_in) : fabsf(x); };
     __shared__ float red[8][128 + 4];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int b = blockIdx.z;
@@ -298,24 +332,24 @@ colmax_kstrided_kernel(const float* __restrict__ src, uint32_t* __restrict__ max
             for (; i + 4 <= n; i += 4) {             // four independent 16-byte loads in flight per thread
                 float4 v0 = __ldg(p), v1 = __ldg(p + step), v2 = __ldg(p + 2 * step), v3 = __ldg(p + 3 * step);
                 p += 4 * step;
-                m0 = fmaxf(fmaxf(m0, fmaxf(fabsf(v0.x), fabsf(v1.x))), fmaxf(fabsf(v2.x), fabsf(v3.x)));
-                m1 = fmaxf(fmaxf(m1, fmaxf(fabsf(v0.y), fabsf(v1.y))), fmaxf(fabsf(v2.y), fabsf(v3.y)));
-                m2 = fmaxf(fmaxf(m2, fmaxf(fabsf(v0.z), fabsf(v1.z))), fmaxf(fabsf(v2.z), fabsf(v3.z)));
-                m3 = fmaxf(fmaxf(m3, fmaxf(fabsf(v0.w), fabsf(v1.w))), fmaxf(fabsf(v2.w), fabsf(v3.w)));
+                m0 = fmaxf(fmaxf(m0, fmaxf(mag(v0.x), mag(v1.x))), fmaxf(mag(v2.x), mag(v3.x)));
+                m1 = fmaxf(fmaxf(m1, fmaxf(mag(v0.y), mag(v1.y))), fmaxf(mag(v2.y), mag(v3.y)));
+                m2 = fmaxf(fmaxf(m2, fmaxf(mag(v0.z), mag(v1.z))), fmaxf(mag(v2.z), mag(v3.z)));
+                m3 = fmaxf(fmaxf(m3, fmaxf(mag(v0.w), mag(v1.w))), fmaxf(mag(v2.w), mag(v3.w)));
             }
             for (; i < n; ++i, p += step) {
                 float4 v = __ldg(p);
-                m0 = fmaxf(m0, fabsf(v.x)); m1 = fmaxf(m1, fabsf(v.y));
-                m2 = fmaxf(m2, fabsf(v.z)); m3 = fmaxf(m3, fabsf(v.w));
+                m0 = fmaxf(m0, mag(v.x)); m1 = fmaxf(m1, mag(v.y));
+                m2 = fmaxf(m2, mag(v.z)); m3 = fmaxf(m3, mag(v.w));
             }
         }
     } else {
         for (int k = k_lo + ty; k < k_hi; k += 8) {
             const float* p = s + (size_t)k * R + r0;
-            if (r0 + 0 < R) m0 = fmaxf(m0, fabsf(__ldg(p + 0)));
-            if (r0 + 1 < R) m1 = fmaxf(m1, fabsf(__ldg(p + 1)));
-            if (r0 + 2 < R) m2 = fmaxf(m2, fabsf(__ldg(p + 2)));
-            if (r0 + 3 < R) m3 = fmaxf(m3, fabsf(__ldg(p + 3)));
+            if (r0 + 0 < R) m0 = fmaxf(m0, mag(__ldg(p + 0)));
+            if (r0 + 1 < R) m1 = fmaxf(m1, mag(__ldg(p + 1)));
+            if (r0 + 2 < R) m2 = fmaxf(m2, mag(__ldg(p + 2)));
+            if (r0 + 3 < R) m3 = fmaxf(m3, mag(__ldg(p + 3)));
         }
     }
     }
@@ -366,7 +400,7 @@ template <int S>
 __global__ void __launch_bounds__(PREPASS_THREADS)
 split_kstrided_kernel(const float* __restrict__ src, const uint32_t* __restrict__ maxbits,
                       int8_t* __restrict__ planes, int* __restrict__ expo,
-                      int R, int K, int Kp, long long src_batch_stride) {
+                      int R, int K, int Kp, long long src_batch_stride, bool mark) {
     __shared__ __align__(16) float tile[32 * 128];
     __shared__ int e_sh[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -380,9 +414,9 @@ split_kstrided_kernel(const float* __restrict__ src, const uint32_t* __restrict_
 
     if (threadIdx.x < 32) {
         int r = r0 + threadIdx.x;
-        int e = r < R ? scale_exponent(bits_f32(maxbits[(size_t)b * R + r])) : 0;
+        const int e = r < R ? scale_exponent(bits_f32(maxbits[(size_t)b * R + r])) : 0;
         e_sh[threadIdx.x] = e;
-        if (r < R && blockIdx.y == 0) expo[(size_t)b * R + r] = e;
+        if (r < R && blockIdx.y == 0) expo[(size_t)b * R + r] = recorded_expo(e, mark);
     }
     const bool vec = (R & 3) == 0 && ((reinterpret_cast<uintptr_t>(s) & 15) == 0);
     // vector path: a warp covers 4 k-rows x 32 r per load, lane = (k sub-row, group of four r);

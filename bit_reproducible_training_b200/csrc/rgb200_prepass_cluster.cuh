@@ -39,11 +39,13 @@ __device__ __forceinline__ void quad_words(float a, float b, float c, float d, c
 // dynamic shared memory = KC * W * 4 bytes.  KC is a multiple of 64; Kp a multiple of 128.
 // tmap: 3-D FP32 map (r, k, batch) with box (W, 64, 1), no swizzle, zero fill.
 // given_max: externally reduced maxima [batch][R] (K-sharded operation) or null.
+// nonfinite: see NonFinite.
 // status: word that receives STATUS_WAIT_FULL if the slab never arrives (the cluster still leaves in step).
 template <int S, int W>
 __global__ void __cluster_dims__(KSC_CLUSTER, 1, 1) __launch_bounds__(PREPASS_THREADS)
 split_kstrided_cluster_kernel(const __grid_constant__ CUtensorMap tmap, const float* __restrict__ given_max,
-                              int8_t* __restrict__ planes, int* __restrict__ expo, int R, int K, int Kp, int KC, int* status) {
+                              int8_t* __restrict__ planes, int* __restrict__ expo, int R, int K, int Kp, int KC, int* status,
+                              int nonfinite) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     extern __shared__ uint8_t slab_raw[];
@@ -90,8 +92,14 @@ split_kstrided_cluster_kernel(const __grid_constant__ CUtensorMap tmap, const fl
 
     // column maxima of this slab
     float m = 0.0f;
-    if (!given_max && arrived)
-        for (int k = g; k < nk; k += G) m = fmaxf(m, fabsf(slab[(size_t)k * W + r]));
+    if (!given_max && arrived) {
+        if (nonfinite == NF_UNDEFINED) {
+            for (int k = g; k < nk; k += G) m = fmaxf(m, fabsf(slab[(size_t)k * W + r]));
+        } else {
+            const float stand_in = nonfinite_stand_in(nonfinite);
+            for (int k = g; k < nk; k += G) m = fmaxf(m, abs_or(slab[(size_t)k * W + r], stand_in));
+        }
+    }
     red[threadIdx.x] = m;
     __syncthreads();
     if (threadIdx.x < W) {
@@ -111,7 +119,7 @@ split_kstrided_cluster_kernel(const __grid_constant__ CUtensorMap tmap, const fl
         }
         const int e = scale_exponent(mm);
         e_sh[threadIdx.x] = e;
-        if (rank == 0 && r_glob < R) expo[(size_t)b * R + r_glob] = e;
+        if (rank == 0 && r_glob < R) expo[(size_t)b * R + r_glob] = recorded_expo(e, nonfinite == NF_MARK);
     }
     cluster.sync();                                          // nobody reads remote shared memory after this point
 

@@ -73,6 +73,7 @@ struct RowFusedParams {
     long long stride_c;
     int m_tiles, k_blocks;
     int e0;
+    bool mark;               // rows of op(A) that are not finite give NaN (NF_MARK)
 };
 
 template <int S>
@@ -281,10 +282,18 @@ gemm_i8_rowfused_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
             got = __all_sync(0xFFFFFFFFu, got);
             if (!got) return false;
             const uint8_t* chunk = borrowed ? gen_a + s * RF_F_STAGE_BYTES : gen_f + s * RF_F_STAGE_BYTES;
+            if (P.mark) {
 #pragma unroll
-            for (int i = 0; i < RF_ROW_ITERS; ++i) {
-                const int r = cw * 8 + rsel * RF_ROW_ITERS + i;
-                m[i] = abs4max(m[i], *reinterpret_cast<const float4*>(chunk + r * (RF_CHUNK_K * 4) + cl * 16));
+                for (int i = 0; i < RF_ROW_ITERS; ++i) {
+                    const int r = cw * 8 + rsel * RF_ROW_ITERS + i;
+                    m[i] = nan_to_infinity(abs4max_nan(m[i], *reinterpret_cast<const float4*>(chunk + r * (RF_CHUNK_K * 4) + cl * 16)));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < RF_ROW_ITERS; ++i) {
+                    const int r = cw * 8 + rsel * RF_ROW_ITERS + i;
+                    m[i] = abs4max(m[i], *reinterpret_cast<const float4*>(chunk + r * (RF_CHUNK_K * 4) + cl * 16));
+                }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(empty);
@@ -309,7 +318,7 @@ gemm_i8_rowfused_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                 e[i] = scale_exponent(m[i]);
                 f1[i] = quant_scale(e[i], S).f1;
                 all_plain = all_plain && plain_row(e[i]);
-                if (cl == 0) ea_rows[cw * 8 + rsel * RF_ROW_ITERS + i] = e[i];    // the previous tile's epilogue has finished reading (done_bar)
+                if (cl == 0) ea_rows[cw * 8 + rsel * RF_ROW_ITERS + i] = recorded_expo(e[i], P.mark);    // the previous tile's epilogue has finished reading (done_bar)
             }
             all_plain = __all_sync(0xFFFFFFFFu, all_plain);
             // every warp has left pass 1 - the borrowed stages are about to be overwritten with digits - and every
@@ -401,10 +410,10 @@ gemm_i8_rowfused_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                     r[2] = round_to_f32_bits_signed(T[j + 2], ebase + eb_s[j + 2], &k2);
                     r[3] = round_to_f32_bits_signed(T[j + 3], ebase + eb_s[j + 3], &k3);
                     if (!(k0 && k1 && k2 && k3)) {
-                        r[0] = round_to_f32_bits(T[j + 0], ebase + eb_s[j + 0]);
-                        r[1] = round_to_f32_bits(T[j + 1], ebase + eb_s[j + 1]);
-                        r[2] = round_to_f32_bits(T[j + 2], ebase + eb_s[j + 2]);
-                        r[3] = round_to_f32_bits(T[j + 3], ebase + eb_s[j + 3]);
+                        r[0] = round_or_nan(T[j + 0], ebase + eb_s[j + 0]);
+                        r[1] = round_or_nan(T[j + 1], ebase + eb_s[j + 1]);
+                        r[2] = round_or_nan(T[j + 2], ebase + eb_s[j + 2]);
+                        r[3] = round_or_nan(T[j + 3], ebase + eb_s[j + 3]);
                     }
                     if (whole) {
                         *reinterpret_cast<uint4*>(dst + j) = make_uint4(r[0], r[1], r[2], r[3]);

@@ -178,7 +178,7 @@ struct SmallKParams {
 // The exact rounding of four sums, kept out of line: the hot loops use it only for rows whose results may be
 // subnormal or overflow.
 __device__ __noinline__ uint4 round4_exact(long long t0, long long t1, long long t2, long long t3, int e0, int e1, int e2, int e3) {
-    return make_uint4(round_to_f32_bits(t0, e0), round_to_f32_bits(t1, e1), round_to_f32_bits(t2, e2), round_to_f32_bits(t3, e3));
+    return make_uint4(round_or_nan(t0, e0), round_or_nan(t1, e1), round_or_nan(t2, e2), round_or_nan(t3, e3));
 }
 
 // STAGED: C takes TMA tensor stores (tmap_cx / tmap_cy are valid); otherwise the threads store their rows.
@@ -397,7 +397,7 @@ gemm_i8_smallk_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
             // (the float of a non-zero sum has a biased exponent of 127..190, so E in [-126, 64] is safe), a sum is
             // converted as soon as it is drained and only the exponent is added afterwards.
             __syncwarp();                               // the previous tile's reads of the slot are over
-            if (lane < CPT) eb_s[lane] = eb << 23;
+            if (lane < CPT) eb_s[lane] = (int)((uint32_t)eb << 23);
             int eb_lo = __reduce_min_sync(0xFFFFFFFFu, col_ok ? eb : 0x7FFFFFFF);
             int eb_hi = __reduce_max_sync(0xFFFFFFFFu, col_ok ? eb : -0x7FFFFFFF);
             if (eb_lo > eb_hi) eb_lo = eb_hi = 0;       // no column of this half lies inside the matrix
@@ -461,7 +461,10 @@ gemm_i8_smallk_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                 }
             } else {
                 // some result of this warp's rows may be subnormal or overflow: exact sums are kept and rounded by the
-                // exact routine (out of line: it is rare and large)
+                // exact routine (out of line: it is rare and large), which takes the exponents themselves
+                __syncwarp();
+                if (lane < CPT) eb_s[lane] = eb;
+                __syncwarp();
                 TAcc T[CPT];
 #pragma unroll
                 for (int c0 = 0; c0 < CPT; c0 += 8) {
@@ -479,8 +482,7 @@ gemm_i8_smallk_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
 #pragma unroll 1
                 for (int j = 0; j < CPT; j += 4) {
                     const int4 e4 = eb4[j >> 2];
-                    const uint4 x = round4_exact(T[j], T[j + 1], T[j + 2], T[j + 3], ebase + (e4.x >> 23), ebase + (e4.y >> 23),
-                                                 ebase + (e4.z >> 23), ebase + (e4.w >> 23));
+                    const uint4 x = round4_exact(T[j], T[j + 1], T[j + 2], T[j + 3], ebase + e4.x, ebase + e4.y, ebase + e4.z, ebase + e4.w);
                     const uint32_t r[4] = {x.x, x.y, x.z, x.w};
                     emit(j, r);
                 }

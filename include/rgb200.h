@@ -5,6 +5,8 @@
  * the reference project's "repro_gemm" arithmetic alone: every row of op(A) and column of op(B)
  * gets a power-of-two scale, every input is rounded once to a 7*S-bit fixed-point integer, the
  * integer dot products are formed exactly, and the exact sum is rounded once to FP32.
+ * This defines finite inputs: an output whose row of op(A) or column of op(B) holds an infinity or NaN is some number (the products
+ * inside the operators of rgb200_train.h make it NaN).
  *
  * Every entry point takes plain pointers and sizes.  All device work is enqueued on the stream
  * that is passed in (a cudaStream_t cast to void*; NULL = the default stream).  Return values are

@@ -6,6 +6,9 @@
  * (0 = success, 1 = cudaErrorInvalidValue, 801 = cudaErrorNotSupported).  Calls that contain products report an expired bounded
  * wait through their workspace: rgb200_workspace_status reads it.  Sums of floats are taken in an order that depends
  * on the sizes alone, so the output bits depend on the inputs and the sizes, not on the stream, the call or the GPU.
+ * Infinities and NaN stay visible: a row of an operand (of op(A), or a column of op(B)) that holds one makes every output of its product that it
+ * takes part in NaN (the plain products of rgb200.h leave such outputs undefined), so a loss or a gradient that meets one is not finite;
+ * rows of the cross entropy that do not count take no part in anything, whatever they hold.
  */
 #ifndef RGB200_TRAIN_H
 #define RGB200_TRAIN_H
