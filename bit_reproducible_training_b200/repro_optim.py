@@ -31,6 +31,11 @@ def _counter(n):
     return torch.tensor(int(n), dtype=torch.int64, device="cpu")
 
 
+def _same(a, b):
+    """Whether two lists hold the same objects (parameters have an == of their own)."""
+    return len(a) == len(b) and all(map(operator.is_, a, b))
+
+
 def _blocks(n):
     return -(-n // STATE_BLOCK)
 
@@ -126,10 +131,14 @@ class AdamW(torch.optim.Optimizer):
         self._tables.clear()
 
     def _table(self, index):
-        """The C ABI's rows for one group; parameter and gradient addresses are filled in at each call."""
+        """The C ABI's rows for one group; parameter and gradient addresses are filled in at each call.  A table belongs to the parameters it was
+        made for: a group that has others by now (exchanged, reordered, more, or another group in its place) gets one of its own."""
         group = self.param_groups[index]
         t = self._tables.get(index)
-        if t is None or t["params"] != len(group["params"]):
+        if t is None or not _same(t["params"], group["params"]):
+            self._settle()
+            t = self._tables.get(index)
+        if t is None:
             states = [self._state(p) for p in group["params"]]
             rows = np.zeros(len(states), _ROW)
             for name in self._names():
@@ -150,9 +159,20 @@ class AdamW(torch.optim.Optimizer):
                 for s in states:
                     s["step"] = _counter(s["step"])
             # `kept`: the rows hold addresses, so the tensors behind them must live as long
-            t = self._tables[index] = dict(params=len(states), rows=rows, counts=counts, bytes=[4 * n for n in counts], states=states, step=shared,
+            t = self._tables[index] = dict(params=list(group["params"]), rows=rows, counts=counts, bytes=[4 * n for n in counts], states=states, step=shared,
                                            kept=[s[n] for s in states for n in self._names()], device_step=device_step)
         return t
+
+    def _settle(self):
+        """Reads every counter back from the device, and keeps the tables of the groups that there are, each at its group's index."""
+        old = list(self._tables.values())
+        for t in old:
+            self._steps(t)
+        self._tables = {}
+        for index, group in enumerate(self.param_groups):
+            for t in old:
+                if _same(t["params"], group["params"]):
+                    self._tables[index] = t
 
     def _steps(self, t):
         if t["device_step"] is not None:
