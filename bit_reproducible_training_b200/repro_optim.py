@@ -46,7 +46,7 @@ class AdamW(torch.optim.Optimizer):
     ``state_bits``: 32, or 8 for codes with one scale per 256 values (2.03 instead of 8 bytes of state a parameter).
     ``capturable``: steps are counted on the device, so that ``step()`` can be captured into a CUDA graph and replayed; all
     parameters must then have gradients, and the captured learning rate and other hyper-parameters stay as they were.
-    Without it a step under capture is refused.  Parameters must not overlap in memory.  The tensors in ``state`` are updated in
+    Without it a step under capture is refused, and so is the first step of a group's parameters: it makes their states.  Parameters must not overlap in memory.  The tensors in ``state`` are updated in
     place; to put others in their place use ``adopt`` or ``load_state_dict``.
 
     ``state_dict()`` holds the moments' values in float32 whatever ``state_bits`` is, and ``load_state_dict`` takes such a
@@ -136,6 +136,8 @@ class AdamW(torch.optim.Optimizer):
         group = self.param_groups[index]
         t = self._tables.get(index)
         if t is None or not _same(t["params"], group["params"]):
+            if torch.cuda.is_current_stream_capturing():      # states and counters made here would be set to zero by every replay
+                raise RuntimeError("AdamW needs a step of these parameters or load_state_dict() before it is captured")
             self._settle()
             t = self._tables.get(index)
         if t is None:
