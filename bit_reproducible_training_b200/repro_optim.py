@@ -56,7 +56,7 @@ class AdamW(torch.optim.Optimizer):
         if state_bits not in (8, 32):
             raise ValueError("state_bits must be 8 or 32")
         self.state_bits, self.capturable = state_bits, capturable
-        self._tables = {}
+        self._tables, self._held = {}, []
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, group):
@@ -86,7 +86,7 @@ class AdamW(torch.optim.Optimizer):
         return {**super().__getstate__(), "state_bits": self.state_bits, "capturable": self.capturable}
 
     def __setstate__(self, state):
-        self._tables = {}                            # addresses of the original's tensors do not travel
+        self._tables, self._held = {}, []            # addresses of the original's tensors do not travel
         super().__setstate__(state)
 
     # -- states --------------------------------------------------------------------------------------------------
@@ -111,7 +111,7 @@ class AdamW(torch.optim.Optimizer):
         """Continues from state tensors the caller already holds, without copying them: for each parameter (in group
         order) ``(exp_avg, exp_avg_sq)`` in float32, or with 8-bit states ``(exp_avg int8, exp_avg_sq uint8, exp_avg_scale,
         exp_avg_sq_scale)``.  ``step``: the number of steps done.  The tensors are updated in place from then on.  A step
-        captured into a CUDA graph before goes on using the states it was captured with: capture it again."""
+        captured into a CUDA graph before goes on using the states it was captured with, which stay allocated: capture it again."""
         params = [p for g in self.param_groups for p in g["params"]]
         names = self._names()
         if len(states) != len(params):
@@ -128,7 +128,12 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError("%s must be a contiguous %s tensor of %d values on %s" % (name, dtype, n, p.device))
         for p, st in zip(params, states):
             self.state[p] = dict(step=int(step), **dict(zip(names, st)))
-        self._tables.clear()
+        old, self._tables = list(self._tables.values()), {}
+        self._hold(old)
+        for index, group in enumerate(self.param_groups):
+            if group["params"]:
+                with _on(group["params"][0].device):
+                    self._table(index)
 
     def _table(self, index):
         """The C ABI's rows for one group; parameter and gradient addresses are filled in at each call.  A table belongs to the parameters it was
@@ -137,7 +142,7 @@ class AdamW(torch.optim.Optimizer):
         t = self._tables.get(index)
         if t is None or not _same(t["params"], group["params"]):
             if torch.cuda.is_current_stream_capturing():      # states and counters made here would be set to zero by every replay
-                raise RuntimeError("AdamW needs a step of these parameters or load_state_dict() before it is captured")
+                raise RuntimeError("AdamW needs a step of these parameters, adopt() or load_state_dict() before it is captured")
             self._settle()
             t = self._tables.get(index)
         if t is None:
@@ -162,7 +167,8 @@ class AdamW(torch.optim.Optimizer):
                     s["step"] = _counter(s["step"])
             # `kept`: the rows hold addresses, so the tensors behind them must live as long
             t = self._tables[index] = dict(params=list(group["params"]), rows=rows, counts=counts, bytes=[4 * n for n in counts], states=states, step=shared,
-                                           kept=[s[n] for s in states for n in self._names()], device_step=device_step)
+                                           kept=[s[n] for s in states for n in self._names()], device_step=device_step,
+                                           captured=False)
         return t
 
     def _settle(self):
@@ -175,6 +181,12 @@ class AdamW(torch.optim.Optimizer):
             for t in old:
                 if _same(t["params"], group["params"]):
                     self._tables[index] = t
+        self._hold(old)
+
+    def _hold(self, tables):
+        """Keeps the memory of tables that go out of use, where a CUDA graph was captured with them: a replay still reads and writes it."""
+        used = [id(t) for t in self._tables.values()]
+        self._held += [t["kept"] + [t["device_step"]] for t in tables if t["captured"] and id(t) not in used]
 
     def _steps(self, t):
         if t["device_step"] is not None:
@@ -204,9 +216,12 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _step_group(self, index, group):
-        if not self.capturable and torch.cuda.is_current_stream_capturing():
+        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing and not self.capturable:
             raise RuntimeError("AdamW.step under CUDA graph capture needs capturable=True")
         t = self._table(index)
+        if capturing:
+            t["captured"] = True
         if t["step"] is None or not self._ready(t, group["params"]):
             return self._step_checked(group, t)
         torch.autograd.graph.increment_version(group["params"])
