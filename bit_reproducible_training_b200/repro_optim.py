@@ -228,7 +228,8 @@ class AdamW(torch.optim.Optimizer):
         if t["device_step"] is not None:
             self._launch(group, t["rows"], 0, t["device_step"].data_ptr())
         else:
-            self._launch(group, t["rows"], int(t["step"].add_(1)), None)
+            self._launch(group, t["rows"], int(t["step"]) + 1, None)
+            t["step"].add_(1)                        # a refused launch is not a step
 
     @staticmethod
     def _ready(t, params):
@@ -275,15 +276,19 @@ class AdamW(torch.optim.Optimizer):
             self._launch(group, rows, 0, t["device_step"].data_ptr())
             return
         if t["step"] is not None and len(live) == len(group["params"]):
-            self._launch(group, rows, int(t["step"].add_(1)), None)
+            self._launch(group, rows, int(t["step"]) + 1, None)
+            t["step"].add_(1)
             return
         if t["step"] is not None:                    # from here on each parameter counts for itself
             t["step"] = None
             for s in t["states"]:
                 s["step"] = s["step"].clone()
-        steps = [int(s["step"].add_(1)) for s in states]
+        steps = [int(s["step"]) + 1 for s in states]
         for n in sorted(set(steps)):
-            self._launch(group, np.ascontiguousarray(rows[[i for i, k in enumerate(steps) if k == n]]), n, None)
+            these = [i for i, k in enumerate(steps) if k == n]
+            self._launch(group, np.ascontiguousarray(rows[these]), n, None)
+            for i in these:
+                states[i]["step"].add_(1)
 
     def _launch(self, group, rows, n, device_step):
         b1, b2 = group["betas"]
