@@ -19,6 +19,11 @@ _torch_optimizer = sys.modules[torch.optim.Optimizer.__module__]        # torch.
 
 STATE_BLOCK = 256           # values of a tensor that share one scale (8-bit states)
 
+# What torch's AdamW keeps in a group beside the hyper-parameters: variants of the step, with the value that means the plain one, and switches between
+# equivalent ways to compute it.
+_VARIANTS = dict(amsgrad=False, maximize=False, differentiable=False, decoupled_weight_decay=True)
+_SWITCHES = ("foreach", "fused", "capturable")
+
 _nbytes = operator.attrgetter("nbytes")
 
 # one row of the C ABI's rgb200_adamw_tensor
@@ -63,11 +68,7 @@ class AdamW(torch.optim.Optimizer):
         super().add_param_group(group)
         group = self.param_groups[-1]
         try:
-            for name in ("lr", "eps", "weight_decay"):
-                if not float(group[name]) >= 0.0:
-                    raise ValueError("%s must not be negative" % name)
-            if len(group["betas"]) != 2 or not all(0.0 <= float(b) < 1.0 for b in group["betas"]):
-                raise ValueError("betas must be two numbers in [0, 1)")
+            _check_hyper(group)
             seen = set()
             for p in group["params"]:
                 if id(p) in seen:
@@ -354,24 +355,37 @@ class AdamW(torch.optim.Optimizer):
         return {"state": state, "param_groups": groups}
 
     def load_state_dict(self, state_dict):
+        """Takes what state_dict returns, or the state_dict of torch.optim.AdamW with the same groups.  A dictionary that cannot be taken as it is
+        (other groups or sizes, hyper-parameters out of range, variants of the step that this class has not) is refused before anything changes."""
         groups, params = state_dict["param_groups"], [p for g in self.param_groups for p in g["params"]]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("the loaded state has other parameter groups")
-        ids = [i for g in groups for i in g["params"]]
-        state = state_dict["state"]
-        for p, i in zip(params, ids):
-            for k in ("exp_avg", "exp_avg_sq"):
-                if i in state and state[i][k].numel() != p.numel():
-                    raise ValueError("the loaded state has other sizes")
+        new = []
         for mine, theirs in zip(self.param_groups, groups):
-            mine.update({k: v for k, v in theirs.items() if k != "params"})
-        ms, vs = [], []
+            other = [name for name, plain in _VARIANTS.items() if bool(theirs.get(name, plain)) != plain]
+            if other:
+                raise ValueError("the loaded state was made with %s, which this AdamW has not" % ", ".join("%s=%s" % (n, theirs[n]) for n in other))
+            new.append({k: v for k, v in theirs.items() if k != "params" and k not in _VARIANTS and k not in _SWITCHES})
+            _check_hyper({**mine, **new[-1]})
+        state = state_dict["state"]
+        ids = [i for g in groups for i in g["params"]]
         for p, i in zip(params, ids):
-            s = self._state(p)
-            got = state.get(i)
-            s["step"] = int(got["step"]) if got else 0
-            for name, to in (("exp_avg", ms), ("exp_avg_sq", vs)):
-                to.append(got[name].to(device=p.device, dtype=torch.float32).contiguous() if got else torch.zeros(p.shape, device=p.device))
+            if i in state:
+                missing = [k for k in ("step", "exp_avg", "exp_avg_sq") if k not in state[i]]
+                if missing:
+                    raise ValueError("the loaded state lacks %s" % ", ".join(missing))
+                if any(state[i][k].numel() != p.numel() for k in ("exp_avg", "exp_avg_sq")):
+                    raise ValueError("the loaded state has other sizes")
+                if int(state[i]["step"]) < 0:
+                    raise ValueError("step must not be negative")
+        if self.capturable and any(len({int(state[i]["step"]) if i in state else 0 for i in g["params"]}) > 1 for g in groups):
+            raise ValueError("capturable: all parameters of a group must have done the same number of steps")
+        ms, vs = ([state[i][name].to(device=p.device, dtype=torch.float32).contiguous() if i in state else torch.zeros(p.shape, device=p.device)
+                   for p, i in zip(params, ids)] for name in ("exp_avg", "exp_avg_sq"))
+        for mine, theirs in zip(self.param_groups, new):
+            mine.update(theirs)
+        for p, i in zip(params, ids):
+            self._state(p)["step"] = int(state[i]["step"]) if i in state else 0
         self.write_states(ms, vs)                    # into the tensors there are: a captured step stays valid
         for t in self._tables.values():
             steps = {int(s["step"]) for s in t["states"]}
@@ -382,11 +396,17 @@ class AdamW(torch.optim.Optimizer):
                 if t["device_step"] is not None:
                     t["device_step"].fill_(int(t["step"]))
             else:
-                if t["device_step"] is not None:
-                    raise ValueError("capturable: all parameters of a group must have done the same number of steps")
                 t["step"] = None
                 for s in t["states"]:
                     s["step"] = _counter(s["step"])
+
+
+def _check_hyper(group):
+    for name in ("lr", "eps", "weight_decay"):
+        if not float(group[name]) >= 0.0:
+            raise ValueError("%s must not be negative" % name)
+    if len(group["betas"]) != 2 or not all(0.0 <= float(b) < 1.0 for b in group["betas"]):
+        raise ValueError("betas must be two numbers in [0, 1)")
 
 
 _hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)
