@@ -340,6 +340,15 @@ class AdamW(torch.optim.Optimizer):
                     raise ReproGemmError(rc, call[7:])
 
     def state_dict(self):
+        for hook in list(self._optimizer_state_dict_pre_hooks.values()):
+            hook(self)
+        made = self._state_dict()
+        for hook in list(self._optimizer_state_dict_post_hooks.values()):
+            changed = hook(self, made)
+            made = made if changed is None else changed
+        return made
+
+    def _state_dict(self):
         params = [p for g in self.param_groups for p in g["params"]]
         ms, vs = ([torch.zeros(p.shape, dtype=torch.float32, device=p.device) for p in params] for _ in range(2))
         self.read_states(ms, vs)
@@ -357,6 +366,15 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """Takes what state_dict returns, or the state_dict of torch.optim.AdamW with the same groups.  A dictionary that cannot be taken as it is
         (other groups or sizes, hyper-parameters out of range, variants of the step that this class has not) is refused before anything changes."""
+        state_dict = dict(state_dict)                # hooks may change the dictionary, not the caller's
+        for hook in list(self._optimizer_load_state_dict_pre_hooks.values()):
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
+        self._load_state_dict(state_dict)
+        for hook in list(self._optimizer_load_state_dict_post_hooks.values()):
+            hook(self)
+
+    def _load_state_dict(self, state_dict):
         groups, params = state_dict["param_groups"], [p for g in self.param_groups for p in g["params"]]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("the loaded state has other parameter groups")
