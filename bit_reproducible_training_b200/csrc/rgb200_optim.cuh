@@ -310,6 +310,8 @@ __device__ __forceinline__ void opt_block(const OptEntry& e, const AdamwScalars&
     } else {
         load8(e.p + at, live, wide, m);
         load8(e.g + at, live, wide, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += 0.0f;                       // -0 is a zero, and its bits are not below all others' (block_scale)
     }
     if (MODE != OPT_READ) encode_block(m, v, qm, qv, sm, sv, lane, live, wide);
 }
