@@ -13,6 +13,7 @@ the caller's column-sum function (``set_bias_grad``); without one, asking for th
 raises instead of silently falling back to a sum whose bits depend on the reduction order.
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import repro_conv as rc
 from . import repro_gemm as rg
@@ -36,6 +37,12 @@ def set_bias_grad(fn):
     [N * OH * OW, F] rows)."""
     global _bias_grad
     _bias_grad = fn
+
+
+def _no_tangents(*tensors):
+    """The fused operators read their tensors' memory, where forward-mode derivatives are not: a tangent would be lost without a word."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("forward-mode derivatives are not supported by this operator")
 
 
 class _LinearFn(torch.autograd.Function):
@@ -114,6 +121,8 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     if k == 0 or n == 0:
         raise ValueError("weight must not be empty")
     rg._activation(activation)
+    if forward_ad._current_level >= 0:
+        _no_tangents(x, weight, bias, residual)
     if x.numel() == 0:                                   # no tokens: nothing to launch, gradients of zeros
         return torch.nn.functional.linear(x, weight, bias) + (0 if residual is None else residual)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
@@ -205,6 +214,8 @@ def block_norm(x, y=None, *, weight, bias=None, post_weight=None, gate=None, res
     """(r, h): the residual stream r = residual_scale * x + gate * (post_weight * N(y)) behind a block with output y, and
     h = weight * N(r) + bias for the next block, differentiable in every tensor.  Without y, r is x.  See repro_norm.block_norm."""
     tensors = (x, y, weight, bias, post_weight, gate)
+    if forward_ad._current_level >= 0:
+        _no_tangents(*tensors)
     if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
         return rn.block_norm(x, y, weight=weight, bias=bias, post_weight=post_weight, gate=gate, residual_scale=residual_scale, kind=kind, eps=eps)[:2]
     out = _BlockNormFn.apply(*tensors, residual_scale, kind, eps)
@@ -255,6 +266,8 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
 def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean"):
     """Cross entropy of the logits x @ weight.T without storing them, differentiable in x and weight.  x [..., dim], weight
     [vocabulary, dim], target [...] int64; reduction "mean", "sum" or "none".  See repro_loss.linear_cross_entropy."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(x, weight)
     if not torch.is_grad_enabled() or not (x.requires_grad or weight.requires_grad):
         if target.numel():
             return rl.linear_cross_entropy(x, weight, target, ignore_index, reduction, _slices)[0]
