@@ -710,6 +710,42 @@ cudaError_t gemm_with_epilogue(const float* A, const float* B, float* C, int M, 
     return dispatch(L, a, *dev);
 }
 
+constexpr int TRANSPOSED_ROWS = 1 << 20;          // at S = 3 a sum of 2^20 products is below 2^62
+static rgb200_config transposed_config(int slices) {
+    rgb200_config c;
+    rgb200_default_config(&c);
+    c.slices = slices; c.trans_a = 1;
+    return c;
+}
+
+bool transposed_in_ranges(int R, int slices) { return slices == 3 && R > TRANSPOSED_ROWS; }
+
+size_t transposed_product_bytes(int M, int N, int R, int slices) {
+    const bool ranges = transposed_in_ranges(R, slices);
+    size_t most = 0;
+    for (int rows : {ranges ? TRANSPOSED_ROWS : R, ranges ? (R - 1) % TRANSPOSED_ROWS + 1 : R}) {
+        Layout L;
+        if (epilogue_layout(M, N, rows, transposed_config(slices), EPI_NONE, L) != cudaSuccess) return 0;
+        if (L.total > most) most = L.total;
+    }
+    return most;
+}
+
+cudaError_t transposed_product(const float* A, const float* B, float* C, int M, int N, int R, int slices, Prepared prepared, void* ws, size_t ws_bytes,
+                               cudaStream_t st) {
+    const rgb200_config cfg = transposed_config(slices);
+    EpilogueParams add = {};
+    if (!transposed_in_ranges(R, slices)) return gemm_with_epilogue(A, B, C, M, N, R, cfg, EPI_NONE, add, prepared, ws, ws_bytes, st);
+    for (int at = 0; at < R; at += TRANSPOSED_ROWS) {
+        const int rows = R - at < TRANSPOSED_ROWS ? R - at : TRANSPOSED_ROWS;
+        const cudaError_t e = gemm_with_epilogue(A + (size_t)at * M, B + (size_t)at * N, C, M, N, rows, cfg, at ? EPI_LINEAR : EPI_NONE, add, prepared, ws, ws_bytes, st);
+        if (e != cudaSuccess) return e;
+        add.residual = C;
+        if (R - at <= TRANSPOSED_ROWS) break;      // at may not pass 2^31
+    }
+    return cudaSuccess;
+}
+
 namespace {
 
 cudaError_t gemm_ws(const float* A, const float* B, float* C, int M, int N, int K, int batch, long long sa, long long sb,

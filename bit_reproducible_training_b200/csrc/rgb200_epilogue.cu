@@ -123,11 +123,12 @@ rgb200_config backward_config(int slices, bool ta) {
 struct LinearBackwardLayout { size_t status, maxima, dz, parts, dx, dw, total, dx_bytes, dw_bytes; };
 bool linear_backward_layout(int M, int N, int K, int act, int S, LinearBackwardLayout& L) {
     if (M < 1 || N < 1 || K < 1 || S < 1 || S > 3 || act < 0 || act >= ACT_COUNT) return false;
-    const rgb200_config cx = backward_config(S, false), cw = backward_config(S, true);
-    rgb200_layout_info ix, iw;
-    if (rgb200_layout(M, K, N, 1, &cx, &ix) != cudaSuccess || rgb200_layout(N, K, M, 1, &cw, &iw) != cudaSuccess) return false;
+    const rgb200_config cx = backward_config(S, false);
+    rgb200_layout_info ix;
+    if (rgb200_layout(M, K, N, 1, &cx, &ix) != cudaSuccess) return false;
     L.dx_bytes = lb_round(ix.workspace_bytes);
-    L.dw_bytes = lb_round(iw.workspace_bytes);
+    L.dw_bytes = lb_round(transposed_product_bytes(N, K, M, S));
+    if (L.dw_bytes == 0) return false;
     L.status = 0;                            // one word, directly in front of the maxima: cleared together
     L.maxima = 4;
     L.dz = lb_round(L.maxima + (size_t)M * 4 + (size_t)N * 4);
@@ -169,7 +170,7 @@ extern "C" int rgb200_linear_backward(const float* dY, const float* Z, const flo
     if (e != cudaSuccess) return e;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     char* ws = static_cast<char*>(workspace);
-    const bool both = dX && dW;
+    const bool both = dX && dW && !transposed_in_ranges(M, slices);
     ActBackwardParams P = {};
     P.dy = dY; P.z = Z;
     P.dz = activation != ACT_NONE && (dX || dW) ? reinterpret_cast<float*>(ws + L.dz) : nullptr;
@@ -182,17 +183,17 @@ extern "C" int rgb200_linear_backward(const float* dY, const float* Z, const flo
     if ((e = cudaMemsetAsync(ws + L.status, 0, L.maxima + (both ? (size_t)M * 4 + (size_t)N * 4 : 0), st)) != cudaSuccess) return e;
     if ((P.dz || db || both) && (e = run_activation_backward(P, db, st)) != cudaSuccess) return e;
     const float* dz = P.dz ? P.dz : dY;
-    const rgb200_config cx = backward_config(slices, false), cw = backward_config(slices, true);
+    const rgb200_config cx = backward_config(slices, false);
     Prepared prepared;
     prepared.status = reinterpret_cast<int*>(ws + L.status);
     if (both) {
         PlaneSlots rows, cols;
-        if ((e = plane_slots(M, K, N, cx, ws + L.dx, &rows)) != cudaSuccess || (e = plane_slots(N, K, M, cw, ws + L.dw, &cols)) != cudaSuccess) return e;
+        if ((e = plane_slots(M, K, N, cx, ws + L.dx, &rows)) != cudaSuccess || (e = plane_slots(N, K, M, backward_config(slices, true), ws + L.dw, &cols)) != cudaSuccess) return e;
         if ((e = launch_split_both(slices, dz, N, M, N, P.row_max, P.col_max, rows, cols, st)) != cudaSuccess) return e;
         prepared.a = true;
     }
     const EpilogueParams none = {};
     if (dX && (e = gemm_with_epilogue(dz, W, dX, M, K, N, cx, EPI_NONE, none, prepared, ws + L.dx, L.dx_bytes, st)) != cudaSuccess) return e;
-    if (dW && (e = gemm_with_epilogue(dz, X, dW, N, K, M, cw, EPI_NONE, none, prepared, ws + L.dw, L.dw_bytes, st)) != cudaSuccess) return e;
+    if (dW && (e = transposed_product(dz, X, dW, N, K, M, slices, prepared, ws + L.dw, L.dw_bytes, st)) != cudaSuccess) return e;
     return cudaSuccess;
 }

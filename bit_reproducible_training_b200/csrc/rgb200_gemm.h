@@ -42,6 +42,14 @@ cudaError_t plane_slots(int M, int N, int K, const rgb200_config& cfg, void* ws,
 cudaError_t gemm_with_epilogue(const float* A, const float* B, float* C, int M, int N, int K, const rgb200_config& cfg, int epi,
                                const EpilogueParams& E, Prepared prepared, void* ws, size_t ws_bytes, cudaStream_t st);
 
+// C [M, N] = A^T B over the rows of A [R, M] and B [R, N]: a weight's gradient.  One EPI_NONE product where the sums of R terms fit INT64; else
+// (S = 3, more than 2^20 rows) one for each range of 2^20 rows, the later ones added in order.  `prepared` holds for one product only: a and b must
+// be false for several.  Bytes of workspace, 0 where the sizes are not supported.
+bool transposed_in_ranges(int R, int slices);
+size_t transposed_product_bytes(int M, int N, int R, int slices);
+cudaError_t transposed_product(const float* A, const float* B, float* C, int M, int N, int R, int slices, Prepared prepared, void* ws, size_t ws_bytes,
+                               cudaStream_t st);
+
 // Digit planes of src [R][C] (rows ld elements apart) as the row-scaled operand (k along the columns) and as the column-scaled one (k along the rows),
 // from the bits of its rows' and columns' largest magnitudes (rgb200_dual.cuh).
 cudaError_t launch_split_both(int slices, const float* src, int ld, int R, int C, const unsigned* row_max, const unsigned* col_max, const PlaneSlots& rows,

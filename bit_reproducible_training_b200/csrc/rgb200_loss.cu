@@ -103,14 +103,14 @@ struct BackwardLayout { int words; size_t status, listed, maxima, weight, coeffi
 bool backward_layout(int N, int V, int D, int S, BackwardLayout& L) {
     L.words = backward_words(N, V, D);
     if (!product_bytes(N, L.words, D, S, false, true, &L.logits_bytes) || !product_bytes(N, D, L.words, S, false, false, &L.dx_bytes) ||
-        !product_bytes(L.words, D, N, S, true, false, &L.dw_bytes))
+        (L.dw_bytes = round_up(transposed_product_bytes(L.words, D, N, S))) == 0)
         return false;
     // the last piece may be narrower, and a narrower product can be planned with more K ranges
     const int rest = V - (V - 1) / L.words * L.words;
     size_t b;
     if (!product_bytes(N, D, rest, S, false, false, &b)) return false;
     if (b > L.dx_bytes) L.dx_bytes = b;
-    if (!product_bytes(rest, D, N, S, true, false, &b)) return false;
+    if ((b = round_up(transposed_product_bytes(rest, D, N, S))) == 0) return false;
     if (b > L.dw_bytes) L.dw_bytes = b;
     L.status = 0;                            // status, listed and the first piece's maxima are cleared together
     L.listed = 4;
@@ -199,7 +199,7 @@ extern "C" int rgb200_linear_xent_backward(const float* X, const float* W, const
     int* listed = reinterpret_cast<int*>(ws + L.listed);
     int* first = reinterpret_cast<int*>(ws + L.first);
     int* not_last = reinterpret_cast<int*>(ws + L.not_last);
-    const bool both = dX && dW;
+    const bool both = dX && dW && !transposed_in_ranges(N, slices);
     const size_t maxima_bytes = (size_t)N * 4 + (size_t)L.words * 4;
     float* P = reinterpret_cast<float*>(ws + L.p);
 
@@ -227,10 +227,10 @@ extern "C" int rgb200_linear_xent_backward(const float* X, const float* W, const
         if ((e = gemm_with_epilogue(X, Wp, P, N, words, D, product_config(slices, false, true), EPI_PROB, E,
                                     Prepared{at > 0 && words == L.words, false, status}, ws + L.logits, L.logits_bytes, st)) != cudaSuccess)
             return e;
-        const rgb200_config cx = product_config(slices, false, false), cw = product_config(slices, true, false);
+        const rgb200_config cx = product_config(slices, false, false);
         if (both) {                                  // P once for both products
             PlaneSlots rows, cols;
-            if ((e = plane_slots(N, D, words, cx, ws + L.dx, &rows)) != cudaSuccess || (e = plane_slots(words, D, N, cw, ws + L.dw, &cols)) != cudaSuccess)
+            if ((e = plane_slots(N, D, words, cx, ws + L.dx, &rows)) != cudaSuccess || (e = plane_slots(words, D, N, product_config(slices, true, false), ws + L.dw, &cols)) != cudaSuccess)
                 return e;
             if ((e = launch_split_both(slices, P, E.ldc, N, words, E.row_max, E.col_max, rows, cols, st)) != cudaSuccess) return e;
         }
@@ -239,7 +239,7 @@ extern "C" int rgb200_linear_xent_backward(const float* X, const float* W, const
         if (dX && (e = gemm_with_epilogue(P, Wp, dX, N, D, words, cx, EPI_LINEAR, add, Prepared{both, false, status, false, NF_MARK, NF_UNDEFINED}, ws + L.dx,
                                           L.dx_bytes, st)) != cudaSuccess)
             return e;
-        if (dW && (e = gemm_with_epilogue(P, X, dW + (size_t)at * D, words, D, N, cw, EPI_NONE, add, Prepared{both, at > 0, status, false, NF_MARK, NF_DROP},
+        if (dW && (e = transposed_product(P, X, dW + (size_t)at * D, words, D, N, slices, Prepared{both, at > 0 && !transposed_in_ranges(N, slices), status, false, NF_MARK, NF_DROP},
                                           ws + L.dw, L.dw_bytes, st)) != cudaSuccess)
             return e;
     }
