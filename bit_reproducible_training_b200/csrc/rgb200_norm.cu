@@ -35,9 +35,9 @@ NormParts norm_parts(int rows, int dim, int groups) {
     const int group_rows = rows / groups, tpr = norm_threads(dim);
     long long want = 148ll * (tpr <= 512 ? 512 / tpr : 1) / groups;
     if (want < 1) want = 1;
-    if (want > (group_rows + 7) / 8) want = (group_rows + 7) / 8;
-    p.rows = (int)((group_rows + want - 1) / want);
-    p.per_group = (group_rows + p.rows - 1) / p.rows;
+    if (want > (group_rows - 1) / 8 + 1) want = (group_rows - 1) / 8 + 1;
+    p.rows = (int)((group_rows - 1) / want + 1);               // group_rows may be 2^31 - 1
+    p.per_group = (group_rows - 1) / p.rows + 1;
     p.total = p.per_group * groups;
     return p;
 }

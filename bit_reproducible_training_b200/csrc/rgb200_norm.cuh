@@ -306,7 +306,7 @@ block_norm_backward_kernel(const NormParams P) {
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
 
     auto fetch = [&](int row) {
-        if (row < row_end) {
+        if ((uint32_t)row < (uint32_t)row_end) {    // behind 2^31 - 1 rows the index has wrapped to a negative one
             const uint32_t at = ring_at + 4 * STAGE_FLOATS * (uint32_t)((row - (int)first) % STAGES);
             const size_t o = (size_t)row * P.dim;
             norm_fetch<TPR, V>(at, src_r + o, P.dim, lane, wide);
@@ -358,7 +358,7 @@ block_norm_backward_kernel(const NormParams P) {
             if (use_y) norm_take<TPR, V>(stage + 3 * TENSOR_FLOATS, y);
         }
         const float m_r = mean, s_r = rstd, m_y = mean_y, s_y = rstd_y;
-        fetch(row + STAGES);                        // the slots just read
+        fetch((int)((uint32_t)row + STAGES));       // the slots just read
         fetch_stats(row + 1);
 #pragma unroll
         for (int j = 0; j < NORM_VALUES; ++j) {
