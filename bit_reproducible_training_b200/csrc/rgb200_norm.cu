@@ -18,7 +18,7 @@ int norm_threads(int dim) {
 bool good_norm(const rgb200_block_norm* n) {
     if (!n || n->rows < 0 || n->dim < 1 || n->dim > NORM_MAX_DIM || n->groups < 1 || (n->kind != RGB200_NORM_RMS && n->kind != RGB200_NORM_LAYER)) return false;
     if (!(n->eps >= 0.0f) || n->scale != n->scale) return false;
-    if (n->rows % n->groups != 0) return false;
+    if (n->rows % n->groups != 0 || n->groups > NORM_MAX_GROUPS) return false;
     if (!n->gate && n->groups != 1) return false;
     if (n->rows > 0 && (!n->x || !n->weight || (!n->y && (n->post_weight || n->gate)))) return false;    // no rows: no tensors needed
     return true;
@@ -120,7 +120,7 @@ extern "C" int rgb200_block_norm_forward(const rgb200_block_norm* n, void* strea
 }
 
 extern "C" size_t rgb200_block_norm_backward_workspace(int rows, int dim, int groups) {
-    if (rows < 0 || dim < 1 || dim > NORM_MAX_DIM || groups < 1 || rows % groups != 0) return 0;
+    if (rows < 0 || dim < 1 || dim > NORM_MAX_DIM || groups < 1 || groups > NORM_MAX_GROUPS || rows % groups != 0) return 0;
     const size_t n = (size_t)norm_parts(rows, dim, groups).total * 3 * dim * sizeof(float);
     return n < 256 ? 256 : n;
 }

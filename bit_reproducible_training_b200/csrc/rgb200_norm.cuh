@@ -28,6 +28,7 @@ namespace rgb200 {
 
 constexpr int NORM_VALUES = 8;                   // values of a row per thread
 constexpr int NORM_MAX_DIM = 1024 * NORM_VALUES;
+constexpr int NORM_MAX_GROUPS = 1 << 30;         // the sums over the groups count in strides of 32 bits
 
 struct NormParams {
     const float *x, *y, *w, *b, *pw, *gate;      // y, b, pw, gate may be null (pw, gate only with y)

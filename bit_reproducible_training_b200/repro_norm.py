@@ -17,6 +17,7 @@ from .repro_gemm import ReproGemmError, _addr, _check, _extent, _on, _raw_stream
 
 KINDS = {"rms": 0, "layer": 1}
 MAX_DIM = 8192
+MAX_GROUPS = 1 << 30
 
 
 @dataclass
@@ -58,6 +59,8 @@ def _sizes(x, y, weight, bias, post_weight, gate, kind, eps):
         groups = 1 if gate.dim() == 1 else gate.shape[0]
         if groups < 1 or rows % groups != 0:
             raise ValueError("the rows must divide into the gate's groups")
+        if groups > MAX_GROUPS:
+            raise ValueError("a gate may have 2^30 rows at most")
     _same_device((x, y, weight, bias, post_weight, gate))
     return rows, dim, groups
 

@@ -123,7 +123,8 @@ int rgb200_adamw_states_write(const rgb200_adamw_tensor* tensors, int count, voi
  * takes the gradients dr (of r from elsewhere; may be NULL) and dh, and writes those outputs that are not NULL: dx[rows, dim],
  * dy, dweight[dim], dbias[dim], dpost_weight[dim], dgate[groups, dim].  Without y, r is x: r is not read, and dr (of x from the
  * residual stream) is added to dx as it is.
- * Sums are taken in an order that depends on (rows, dim, groups) alone.  Asynchronous and allocation-free; dim at most 8192.
+ * Sums are taken in an order that depends on (rows, dim, groups) alone.  Asynchronous and allocation-free; dim at most 8192,
+ * groups at most 2^30.
  * The workspace (16-byte aligned) may be reused by any later call on the same stream.
  * 1 (invalid value): sizes outside those limits, rows not a multiple of groups, negative or NaN eps, post_weight or gate or
  * dy without y, gradients of absent tensors, missing tensors, a short workspace. */
