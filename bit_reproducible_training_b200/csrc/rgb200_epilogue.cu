@@ -42,6 +42,7 @@ cudaError_t launch_slices(int S, int grid, const CUtensorMap& a, const CUtensorM
 
 // Row ranges of the backward pass, from the sizes alone: as many as give the 148 SMs two rounds of three CTAs each (what their registers
 // hold) and not a few more, at least 32 rows each.  8192 x 4096 with gelu: 28 ranges (896 CTAs, a third round of eight) took 88 us, 27 take 74 us (5.4 TB/s).
+constexpr int ACTB_MAX_SIZE = 0x7FFFFFFF - 4096;           // the kernel's indexes run up to a batch or a strip ahead, the ranges' arithmetic by their count
 int backward_ranges(int M, int N) {
     const int strips = (N + ACTB_COLS - 1) / ACTB_COLS;
     int ranges = 148 * 6 / strips;
@@ -84,7 +85,7 @@ extern "C" int rgb200_gemm_epilogue_fp32_ws(const float* A, const float* B, floa
 }
 
 extern "C" size_t rgb200_activation_backward_workspace(int M, int N) {
-    if (M < 0 || N < 1) return 0;
+    if (M < 0 || M > ACTB_MAX_SIZE || N < 1 || N > ACTB_MAX_SIZE) return 0;
     const size_t n = (size_t)backward_ranges(M, N) * N * sizeof(float);
     return n < 256 ? 256 : n;
 }
@@ -122,7 +123,7 @@ rgb200_config backward_config(int slices, bool ta) {
 // Workspace of the linear layer's backward pass: dZ (with an activation), its maxima, the ranges' column sums, and each product's own.
 struct LinearBackwardLayout { size_t status, maxima, dz, parts, dx, dw, total, dx_bytes, dw_bytes; };
 bool linear_backward_layout(int M, int N, int K, int act, int S, LinearBackwardLayout& L) {
-    if (M < 1 || N < 1 || K < 1 || S < 1 || S > 3 || act < 0 || act >= ACT_COUNT) return false;
+    if (M < 1 || M > ACTB_MAX_SIZE || N < 1 || N > ACTB_MAX_SIZE || K < 1 || S < 1 || S > 3 || act < 0 || act >= ACT_COUNT) return false;
     const rgb200_config cx = backward_config(S, false);
     rgb200_layout_info ix;
     if (rgb200_layout(M, K, N, 1, &cx, &ix) != cudaSuccess) return false;
@@ -143,7 +144,7 @@ bool linear_backward_layout(int M, int N, int K, int act, int S, LinearBackwardL
 
 extern "C" int rgb200_activation_backward(const float* dY, const float* Z, float* dZ, float* db, int M, int N, int activation, void* workspace,
                                           size_t workspace_bytes, void* stream) {
-    if (M < 0 || N < 1 || activation < 0 || activation >= ACT_COUNT || (!dZ && !db)) return cudaErrorInvalidValue;
+    if (M < 0 || M > ACTB_MAX_SIZE || N < 1 || N > ACTB_MAX_SIZE || activation < 0 || activation >= ACT_COUNT || (!dZ && !db)) return cudaErrorInvalidValue;
     if (M > 0 && (!dY || (activation != ACT_NONE && !Z))) return cudaErrorInvalidValue;
     if (db && (!workspace || workspace_bytes < rgb200_activation_backward_workspace(M, N))) return cudaErrorInvalidValue;
     cudaError_t e = check_b200();

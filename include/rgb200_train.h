@@ -33,7 +33,8 @@ extern "C" {
  * Slopes are those of the computed Z: relu's is 0 for Z <= 0, so a Z within the product's rounding of zero may pass or stop a gradient that
  * another product, rounded otherwise, would not.
  * rgb200_activation_backward: dZ = dY act'(Z) (dZ may be NULL, or dY itself) and db = column sums of dZ (may be NULL; the
- * workspace, of rgb200_activation_backward_workspace bytes, is needed for db alone).  Z may be NULL without an activation. */
+ * workspace, of rgb200_activation_backward_workspace bytes, is needed for db alone).  Z may be NULL without an activation.  M and N are at most
+ * 2^31 - 4097. */
 enum { RGB200_ACT_NONE = 0, RGB200_ACT_RELU = 1, RGB200_ACT_SILU = 2, RGB200_ACT_GELU = 3, RGB200_ACT_GELU_TANH = 4 };
 typedef struct rgb200_epilogue {
     const float* bias;
