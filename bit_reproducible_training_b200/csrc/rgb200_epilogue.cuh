@@ -40,7 +40,8 @@ __device__ __forceinline__ float activation(float z) {
     return z;
 }
 
-// Derivative of the activation.  Where exp overflows the sigmoid is 0 and the products with z stay finite for finite z below 1e12.
+// Derivative of the activation.  Where exp overflows the sigmoid is 0 and the products with it are 0 for any finite z: gelu_tanh's inner
+// slope, a cube's, would overflow beyond 1e13 and is taken at 64 there, where p (1 - p) is 0 already.
 template <int ACT>
 __device__ __forceinline__ float activation_slope(float z) {
     if (ACT == ACT_RELU) return z <= 0.0f ? 0.0f : 1.0f;
@@ -51,7 +52,8 @@ __device__ __forceinline__ float activation_slope(float z) {
     if (ACT == ACT_GELU) return 0.5f * (1.0f + erff(z * SQRT_HALF)) + z * (expf(-0.5f * (z * z)) * INV_SQRT_2PI);
     if (ACT == ACT_GELU_TANH) {
         const float q = z * z, p = 1.0f / (1.0f + exp2_fast(-z * (GELU_L1 + GELU_L3 * q)));
-        return p + (p * (1.0f - p)) * (z * (GELU_G1 + 3.0f * GELU_G3 * q));
+        const float c = fminf(fmaxf(z, -64.0f), 64.0f);
+        return p + (p * (1.0f - p)) * (c * (GELU_G1 + 3.0f * GELU_G3 * (c * c)));
     }
     return 1.0f;
 }
