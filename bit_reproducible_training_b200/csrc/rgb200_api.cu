@@ -674,6 +674,8 @@ cudaError_t dispatch(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
 }  // namespace
 
 // The product with an epilogue, for the entry points of rgb200_train.h (declared in rgb200_gemm.h).
+// The plan, and so the count of K ranges, is the one rgb200_make_plan gives the caller for the workspace: at S = 1 and 2 it is made for the plain
+// product's wider tiles, where these kernels have 64 columns.  The bits do not depend on it.
 static cudaError_t epilogue_layout(int M, int N, int K, const rgb200_config& cfg, int epi, Layout& L) {
     const bool any_ranges = epi == EPI_NONE || epi == EPI_LINEAR;
     cudaError_t e = plan_layout(M, N, K, K, 1, cfg, false, L, 4611686018427387904.0, any_ranges);

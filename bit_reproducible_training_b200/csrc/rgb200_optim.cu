@@ -74,7 +74,8 @@ cudaError_t adamw_call(const rgb200_adamw_tensor* t, int count, int bits, OptMod
     if (e != cudaSuccess || total == 0) return e;
     const int chunk = pick_chunk(total);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // the smallest table that takes them all: its bytes are copied twice on the way to the GPU
+    // the smallest table that takes them all: its bytes are copied twice on the way to the GPU.  Eager steps over small tensors, medium against large
+    // table: 60 tensors 48.0 us against 49.1, 111 tensors 76.7 against 77.7, 150 tensors 97.4 against 99.1; in a CUDA graph 1 % and less
     if (count <= OPT_SMALL_TABLE) return run_adamw<OPT_SMALL_TABLE>(t, count, chunk, bits, mode, H, st);
     if (count <= OPT_MEDIUM_TABLE) return run_adamw<OPT_MEDIUM_TABLE>(t, count, chunk, bits, mode, H, st);
     return run_adamw<OPT_LARGE_TABLE>(t, count, chunk, bits, mode, H, st);
