@@ -97,18 +97,21 @@ def block_norm_backward(dh, dr, r, y, stats, *, weight, bias=None, post_weight=N
     rows, dim, groups = _sizes(r, y, weight, bias, post_weight, gate, kind, eps)
     _same_device((r, dh, dr, stats))
     shape = r.shape
+    like = {name: t.shape for name, t in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("gate", gate)) if t is not None}
     r, dh, stats, weight = _check(r, rows * dim, "r"), _check(dh, rows * dim, "dh"), _check(stats, 4 * rows, "stats"), _check(weight, dim, "weight")
     dr = None if dr is None else _check(dr, rows * dim, "dr")
     y = None if y is None else _check(y, rows * dim, "y")
     post_weight = None if post_weight is None else _check(post_weight, dim, "post_weight")
-    gate_shape = None if gate is None else gate.shape
     gate = None if gate is None else _check(gate, groups * dim, "gate")
 
-    def out(name, given, of):
-        return torch.empty(of, dtype=torch.float32, device=r.device) if name in wanted and given else None
+    like["x"] = shape
+    if y is not None:
+        like["y"] = shape
 
-    g = NormGrads(out("x", True, shape), out("y", y is not None, shape), out("weight", True, dim), out("bias", bias is not None, dim),
-                  out("post_weight", post_weight is not None, dim), out("gate", gate is not None, gate_shape))
+    def out(name):
+        return torch.empty(like[name], dtype=torch.float32, device=r.device) if name in wanted and name in like else None
+
+    g = NormGrads(out("x"), out("y"), out("weight"), out("bias"), out("post_weight"), out("gate"))
     L = _lib.lib()
     with _on(r.device):
         ws = _scratch(L.rgb200_block_norm_backward_workspace(rows, dim, groups), r.device)
