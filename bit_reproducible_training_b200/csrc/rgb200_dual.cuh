@@ -8,7 +8,7 @@
 // Bound: HBM, (4 + 2 S) bytes a value; beside it about 45 instructions a value.  A CTA turns a 128 x 64 tile: eight 16-byte loads
 // a thread, the row digits straight from the registers, then the tile through shared memory (quads exchanged by row, so that
 // neither side meets bank conflicts) and 32 values of one column a thread, one 32-byte store a plane.
-// S = 3, 8192 x 4096: 68 us = 4.9 TB/s; five CTAs an SM (48 registers) against four: 3 % faster, six: 15 % slower (spills).
+// S = 3, 8192 x 4096: 69 us = 4.9 TB/s; five CTAs an SM (48 registers) against four: 3 % faster, six: 15 % slower (spills).
 #pragma once
 #include "rgb200_prepass_cluster.cuh"
 

@@ -41,7 +41,7 @@ cudaError_t launch_slices(int S, int grid, const CUtensorMap& a, const CUtensorM
 }
 
 // Row ranges of the backward pass, from the sizes alone: as many as give the 148 SMs two rounds of three CTAs each (what their registers
-// hold) and not a few more, at least 32 rows each.  8192 x 4096 with gelu: 28 ranges (896 CTAs, a third round of eight) took 88 us, 27 take 74 us (5.4 TB/s).
+// hold) and not a few more, at least 32 rows each.  8192 x 4096 with gelu: 28 ranges (896 CTAs, a third round of eight) took 88 us, 27 take 75 us (5.4 TB/s).
 constexpr int ACTB_MAX_SIZE = 0x7FFFFFFF - 4096;           // the kernel's indexes run up to a batch or a strip ahead, the ranges' arithmetic by their count
 int backward_ranges(int M, int N) {
     const int strips = (N + ACTB_COLS - 1) / ACTB_COLS;

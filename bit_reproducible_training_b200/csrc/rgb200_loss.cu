@@ -9,8 +9,8 @@
 //
 // Work: 4 products of 2 N V D operations (one more than with stored logits), each at the rate of the library's products; what is
 // moved beside them is a few passes over one piece of P.
-// Measured, 8192 x 50257 x 768: 9.25 ms of kernels, of them the statistics' product 2.06, the probabilities' 2.16 (both at K = 768, where
-// the tensor pipe is 67 % busy), dX 1.91, dW 1.70, the two-way split of P 0.92, the splits of X and W 0.34, the rest 0.15.
+// Measured, 8192 x 50257 x 768: 9.28 ms of kernels, of them the statistics' product 2.05, the probabilities' 2.19 (both at K = 768, where
+// the tensor pipe is 67 % busy), dX 1.91, dW 1.72, the two-way split of P 0.92, the splits of X and W 0.33, the rest 0.15.
 #include <cstdint>
 
 #include "../../include/rgb200_train.h"

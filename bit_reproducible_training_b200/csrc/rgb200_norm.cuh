@@ -13,7 +13,7 @@
 //   dw = sum_rows H r^,  db = sum_rows H,  and with Q = sum_rows D y^ (D y without a post norm) over the rows of a group,
 //   dw' = sum_groups g Q,  dg = w' Q.
 //
-// Bound: HBM (measured, 8192 x 4096 with post norm and gate: forward 83 us = 6.4 TB/s).  A row is read once and stays in registers: its sums are taken from there (for the layer kind the mean first,
+// Bound: HBM (measured, 8192 x 4096 with post norm and gate: forward 84 us = 6.4 TB/s).  A row is read once and stays in registers: its sums are taken from there (for the layer kind the mean first,
 // then the squared differences, so that a large mean costs no precision).
 //
 // Order of the sums, which fixes the bits: a thread adds its values of a row in column order, a warp joins lanes by a
