@@ -88,8 +88,9 @@ int auto_split(int M, int N, int batch, int k_blocks, int tile_n) {
 }
 
 // sum_limit bounds total_k * max|X|^2, the largest magnitude an exact sum can reach.
+constexpr double MAX_SUM = 4611686018427387904.0;    // 2^62
 cudaError_t plan_layout(int M, int N, int K, long long total_k, int batch, const rgb200_config& cfg,
-                        bool partial_out, Layout& L, double sum_limit = 4611686018427387904.0 /* 2^62 */,
+                        bool partial_out, Layout& L, double sum_limit = MAX_SUM,
                         bool auto_ranges = true) {
     if (M <= 0 || N <= 0 || K <= 0 || batch <= 0 || cfg.split_k <= 0 || total_k < K) return cudaErrorInvalidValue;
     if (cfg.slices < 1 || cfg.slices > 3) return cudaErrorInvalidValue;
@@ -678,7 +679,7 @@ cudaError_t dispatch(const Layout& L, const RunArgs& a, const DeviceInfo& dev) {
 // product's wider tiles, where these kernels have 64 columns.  The bits do not depend on it.
 static cudaError_t epilogue_layout(int M, int N, int K, const rgb200_config& cfg, int epi, Layout& L) {
     const bool any_ranges = epi == EPI_NONE || epi == EPI_LINEAR;
-    cudaError_t e = plan_layout(M, N, K, K, 1, cfg, false, L, 4611686018427387904.0, any_ranges);
+    cudaError_t e = plan_layout(M, N, K, K, 1, cfg, false, L, MAX_SUM, any_ranges);
     if (e != cudaSuccess) return e;
     return !any_ranges && L.split != 1 ? cudaErrorNotSupported : cudaSuccess;
 }
@@ -712,7 +713,7 @@ cudaError_t gemm_with_epilogue(const float* A, const float* B, float* C, int M, 
     return dispatch(L, a, *dev);
 }
 
-constexpr int TRANSPOSED_ROWS = 1 << 20;          // at S = 3 a sum of 2^20 products is below 2^62
+constexpr int TRANSPOSED_ROWS = 1 << 20;          // rows of a range, where one product cannot take all of them
 static rgb200_config transposed_config(int slices) {
     rgb200_config c;
     rgb200_default_config(&c);
@@ -720,7 +721,9 @@ static rgb200_config transposed_config(int slices) {
     return c;
 }
 
-bool transposed_in_ranges(int R, int slices) { return slices == 3 && R > TRANSPOSED_ROWS; }
+bool transposed_in_ranges(int R, int slices) {        // 1 056 751 rows at S = 3; more than an int counts below
+    return (double)R * max_fixed_point(slices) * max_fixed_point(slices) > MAX_SUM;
+}
 
 size_t transposed_product_bytes(int M, int N, int R, int slices) {
     const bool ranges = transposed_in_ranges(R, slices);

@@ -43,7 +43,7 @@ cudaError_t gemm_with_epilogue(const float* A, const float* B, float* C, int M, 
                                const EpilogueParams& E, Prepared prepared, void* ws, size_t ws_bytes, cudaStream_t st);
 
 // C [M, N] = A^T B over the rows of A [R, M] and B [R, N]: a weight's gradient.  One EPI_NONE product where the sums of R terms fit INT64; else
-// (S = 3, more than 2^20 rows) one for each range of 2^20 rows, the later ones added in order.  `prepared` holds for one product only: a and b must
+// (S = 3, more than 1 056 751 rows) one for each range of 2^20 rows, the later ones added in order.  `prepared` holds for one product only: a and b must
 // be false for several.  Bytes of workspace, 0 where the sizes are not supported.
 bool transposed_in_ranges(int R, int slices);
 size_t transposed_product_bytes(int M, int N, int R, int slices);

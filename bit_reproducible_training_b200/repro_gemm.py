@@ -328,7 +328,7 @@ def activation_backward(dY, Z, M, N, activation=None, want_dz=True, want_db=Fals
 
 def linear_backward(dY, Z, X, W, M, N, K, activation=None, slices=3, want_dx=True, want_dw=True, want_db=False):
     """(dX, dW, db) of Y = act(X W^T + bias): with dZ = dY * act'(Z), dX [M, K] = dZ W, dW [N, K] = dZ^T X, db [N] = column sums
-    of dZ (see activation_backward); None where not wanted.  The products have the bits of ``gemm`` on dZ (dW of more than 2^20 rows
+    of dZ (see activation_backward); None where not wanted.  The products have the bits of ``gemm`` on dZ (dW of more than 1 056 751 rows
     at three slices, which ``gemm`` does not take: the sum of those of ranges of 2^20 rows)."""
     act = _activation(activation)
     _extent(M, N, K)

@@ -49,8 +49,8 @@ int rgb200_activation_backward(const float* dY, const float* Z, float* dZ, float
                                size_t workspace_bytes, void* stream);
 /* The whole backward pass of Y = act(X W^T + bias) (+ residual, whose gradient is dY): with dZ = dY act'(Z), dX [M, K] = dZ W,
  * dW [N, K] = dZ^T X and db [N] = column sums of dZ; each of the three may be NULL.  The products are those of rgb200_gemm_fp32_ws
- * on dZ, bit for bit; dZ's digits for both come from one pass over it.  More than 2^20 rows at S = 3, which such a product does not take: dW is the
- * FP32 sum, in order, of the products of ranges of 2^20 rows.  Workspace: 256-byte aligned; 0 bytes: sizes not supported. */
+ * on dZ, bit for bit; dZ's digits for both come from one pass over it.  More than 1 056 751 rows at S = 3, which such a product does not take: dW
+ * is the FP32 sum, in order, of the products of ranges of 2^20 rows.  Workspace: 256-byte aligned; 0 bytes: sizes not supported. */
 size_t rgb200_linear_backward_workspace(int M, int N, int K, int activation, int slices);
 int rgb200_linear_backward(const float* dY, const float* Z, const float* X, const float* W, float* dX, float* dW, float* db, int M, int N, int K,
                            int activation, int slices, void* workspace, size_t workspace_bytes, void* stream);
@@ -66,7 +66,7 @@ int rgb200_linear_backward(const float* dY, const float* Z, const float* X, cons
  * Backward: dloss points to one value (SUM, MEAN) or N of them (NONE); lse, target_rest and inv_count are the forward call's.
  *   dX = sum_j g p_j W_j - g W_target,  dW = sum_i g_i (p_i - onehot_i) x_i,  g the row's weight; either may be NULL.
  * The logits are the library's products (S = `slices`); sums are taken in an order that depends on the sizes and targets
- * alone (dW's over ranges of 2^20 rows at S = 3).  D at most 105472 (S = 3).  Workspaces: 256-byte aligned, rgb200_linear_xent_workspace bytes (0: sizes not supported). */
+ * alone (dW's, beyond 1 056 751 rows at S = 3, over ranges of 2^20 rows).  D at most 105472 (S = 3).  Workspaces: 256-byte aligned, rgb200_linear_xent_workspace bytes (0: sizes not supported). */
 enum { RGB200_REDUCE_NONE = 0, RGB200_REDUCE_MEAN = 1, RGB200_REDUCE_SUM = 2 };
 size_t rgb200_linear_xent_workspace(int N, int V, int D, int slices, int backward);
 int rgb200_linear_xent_forward(const float* X, const float* W, const long long* target, long long ignore_index, int reduction, int N, int V,

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from bit_reproducible_training_b200 import layers
+from bit_reproducible_training_b200 import repro_gemm as rg
 from test_gpu_loss import U, case, expected, within
 
 pytestmark = pytest.mark.gpu
@@ -47,3 +48,14 @@ def test_linear(act, slices):
     assert torch.equal(dx.double(), dz @ w.detach().double())
     assert torch.equal(dw.double(), dz.t() @ x.detach().double()) and torch.equal(alone, dw)
     assert torch.equal(db.double(), dz.sum(0))
+
+
+@pytest.mark.parametrize("m", [2 ** 20, 2 ** 20 + 1, 1_056_751])
+def test_as_many_rows_as_one_product_takes(m):
+    """Up to there dW has the bits of the plain product."""
+    n, k = 5, 9
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x, w, dy = (torch.randn(s, device="cuda", generator=g) for s in ((m, k), (n, k), (m, n)))
+    dx, dw, _ = rg.linear_backward(dy, None, x, w, m, n, k)
+    assert torch.equal(dw, rg.gemm(dy, x, n, k, m, True, False)) and torch.equal(dx, rg.gemm(dy, w, m, k, n))
+    assert rg.make_plan(n, k, 1_056_751)[0] == 0 and rg.make_plan(n, k, 1_056_752)[0] == 1
