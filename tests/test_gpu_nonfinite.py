@@ -89,6 +89,29 @@ def test_backward_pass(m, n, k, act, slices, bad):
                 check(dw, clean[1], [col], (), asked)
 
 
+@pytest.mark.parametrize("bad", BAD, ids=str)
+@pytest.mark.parametrize("slices", [1, 2, 3])
+@pytest.mark.parametrize("m,n,k", [(200, 132, 32), (300, 516, 64), (129, 1028, 5), (25000, 8, 12), (30001, 20, 4)])
+def test_narrow_gradients_and_long_sums(m, n, k, slices, bad):
+    """One gradient at a time: dX of at most 64 columns splits dZ inside its product's kernel, dW of many rows finds the columns' maxima in a kernel
+    of its own."""
+    x, w, _, _, dy = operands(m, n, k)
+    row, col, kk = m - 1, n // 2, k - 1
+    d, xb, wb = dy.clone(), x.clone(), w.clone()
+    d[row, col], xb[row, kk], wb[col, kk] = bad, bad, bad
+
+    def run(dy, x, w, dx):
+        return rg.linear_backward(dy, None, x, w, m, n, k, None, slices, dx, not dx)[0 if dx else 1]
+
+    dx, dw = run(dy, x, w, True), run(dy, x, w, False)
+    check(run(d, x, w, True), dx, [row])
+    check(run(dy, x, wb, True), dx, (), [kk])
+    check(run(d, x, w, False), dw, [col])
+    check(run(dy, xb, w, False), dw, (), [kk])
+    check(run(d, xb, wb, True), dx, [row], [kk])
+    check(run(d, xb, wb, False), dw, [col], [kk])
+
+
 LOSS = [(40, 24, 60), (130, 100, 1000), (70, 515, 333), (64, 64, 20000), (40, 16, 70000), (300, 33, 5001)]
 
 
